@@ -106,8 +106,9 @@ def _quantise(x):
     """f32 rows -> integer rows (as f32) and the scale of each row."""
     a = x.abs().amax(dim=1, keepdim=True)
     fine = a >= TINY
-    q = torch.where(fine & torch.isfinite(a), torch.round(x * (127 / a)), 0.0)
-    scale = torch.where(fine, a / 127, 0.0)
+    steps = torch.full_like(a, 127)        # a tensor: torch multiplies by a reciprocal where one side is a number
+    q = torch.where(fine & torch.isfinite(a), torch.round(x * (steps / a)), 0.0)
+    scale = torch.where(fine, a / steps, 0.0)
     return q, torch.where(torch.isfinite(a), scale, float("nan"))
 
 
