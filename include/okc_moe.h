@@ -275,6 +275,78 @@ int okc_ep_mark_arrived(const okc_ep_comm* comm, int which, int from_rank, okc_s
 /* Synchronises `stream`; returns the status kept in this rank's buffer and clears it. */
 int okc_ep_read_status(const okc_ep_comm* comm, okc_stream_t stream, int32_t* detail);
 
+/*
+ * The dense operators around the expert block: the residual stream's norms at its two ends and the products of 8-bit
+ * integers (W8A8) of the layer's dense projections.  The reference runs these steps in its decode layer on bf16
+ * (the boundary of residual + norm around the experts, muse_decode_layer/layer.py; the projections muse_bf16_proj).
+ *
+ * Rows come as bf16 (kind 0), f32 (kind 1) or int8 with an f32 scale per row (kind 2); strides are in elements, columns
+ * are contiguous.  All arithmetic is f32 (the products: exact 32-bit integer sums), rounded once on the way out.
+ * rows / tokens may be 0 (nothing runs).
+ */
+#define OKC_BLOCK_NORM_MAX_HIDDEN 16384
+
+/*
+ * Per row, r = residual, y = block, any of the parts left out by a NULL:
+ *   z = y * rsqrt(mean(y^2) + eps) * post_gain
+ *   r' = residual_scale * r + block_scale * gate * z          -> residual_out (type of residual; may be residual itself,
+ *                                                                not an overlapping other row)
+ *   x = r' * rsqrt(mean(r'^2) + eps) * pre_gain               -> out
+ * block == NULL: only x = norm(residual) (post_gain and gate must be NULL, residual_out is not written).
+ * pre_gain == NULL: only r' (out is not written).
+ */
+typedef struct okc_block_norm_args {
+  const void* residual;      /* bf16 or f32 [rows, residual_stride] */
+  const void* block;         /* bf16 or f32 [rows, block_stride], or NULL */
+  const void* gate;          /* bf16 or f32, or NULL */
+  const float* post_gain;    /* f32 [hidden] or NULL */
+  const float* pre_gain;     /* f32 [hidden] or NULL */
+  void* residual_out;
+  void* out;                 /* out_kind 0 bf16, 1 f32, 2 int8 rows */
+  float* out_scale;          /* f32 [rows] for int8 rows */
+  int64_t rows;
+  int64_t residual_stride, block_stride, gate_stride, residual_out_stride, out_stride;
+  int32_t hidden;            /* 1 .. OKC_BLOCK_NORM_MAX_HIDDEN */
+  int32_t residual_f32, block_f32, gate_f32;
+  int32_t gate_kind;         /* 0 none, 1 per channel [hidden], 2 per row (gate_stride apart), 3 per element */
+  int32_t gate_sigmoid;      /* 1: sigmoid(gate) in its place */
+  int32_t out_kind;
+  float residual_scale, block_scale, eps;
+} okc_block_norm_args;
+int okc_moe_block_norm(const okc_block_norm_args* args, okc_stream_t stream);
+
+/* Rows of bf16 / f32 -> int8 rows and their scales.  With a = max|x| of a row: scale = f32(a / 127),
+ * q = rint(f32(x * f32(127 / a))); a < 2^-120: zeros and scale 0; a row with an infinity or a NaN: zeros and scale NaN.
+ * cols <= 131071. */
+int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t rows, int32_t cols, void* q,
+                          int64_t q_stride, float* scale, okc_stream_t stream);
+
+/*
+ * out[t][n] = (sum_k x[t][k] * w[n][k]) * (x_scale[t] * w_scale[n]) + bias[n]              (okc_moe_int8_linear)
+ * out[t][i] = g / (1 + exp(-g)) * u with g, u = that sum for rows i and n + i of w          (okc_moe_int8_gated)
+ * w: int8, n rows (gated: 2 n, gate rows first), 16-byte aligned, w_stride a multiple of 16; the bytes between k and
+ * w_stride are not used.  x: int8 rows aligned the same way with x_scale, or bf16 / f32 rows, which are quantised as
+ * okc_moe_quantize_rows does, into `scratch` (okc_moe_int8_scratch_bytes; up to 8 tokens need none).  k <= 131071.
+ * The result of a token does not depend on the tokens beside it, bit for bit.
+ */
+typedef struct okc_int8_args {
+  const void* x;
+  const float* x_scale;
+  const void* w;
+  const float* w_scale;
+  const float* bias;         /* f32 [n] or NULL; NULL for the gated product */
+  void* out;                 /* bf16 or, with out_f32, f32 [tokens, out_stride] */
+  void* scratch;
+  int64_t x_stride, w_stride, out_stride;
+  int32_t x_kind, out_f32, tokens, k, n;
+} okc_int8_args;
+uint64_t okc_moe_int8_scratch_bytes(int x_kind, int32_t tokens, int32_t k);
+int okc_moe_int8_linear(const okc_int8_args* args, okc_stream_t stream);
+int okc_moe_int8_gated(const okc_int8_args* args, okc_stream_t stream);
+/* Synchronises `stream`; 0, or OKC_ERR_TIMEOUT with *detail naming a device wait of an int8 product that ran out on the
+ * current device since the last call of this function. */
+int okc_moe_int8_status(okc_stream_t stream, int32_t* detail);
+
 /* Copies the sorted-route tables out of `workspace` for inspection (host or device pointers are
  * NOT interchangeable: all four are device pointers; any may be NULL).  counts: int32
  * [expert_slots]; sorted: int32 [T*routes_per_token] (route index t*routes_per_token+slot per

@@ -50,6 +50,21 @@ class Router(C.Structure):
                 ("w_split", C.c_void_p)]
 
 
+class BlockNormArgs(C.Structure):
+    """okc_block_norm_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("residual", "block", "gate", "post_gain", "pre_gain", "residual_out", "out", "out_scale")] + \
+               [(n, C.c_int64) for n in ("rows", "residual_stride", "block_stride", "gate_stride", "residual_out_stride", "out_stride")] + \
+               [(n, C.c_int32) for n in ("hidden", "residual_f32", "block_f32", "gate_f32", "gate_kind", "gate_sigmoid", "out_kind")] + \
+               [(n, C.c_float) for n in ("residual_scale", "block_scale", "eps")]
+
+
+class Int8Args(C.Structure):
+    """okc_int8_args"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "x_scale", "w", "w_scale", "bias", "out", "scratch")] + \
+               [(n, C.c_int64) for n in ("x_stride", "w_stride", "out_stride")] + \
+               [(n, C.c_int32) for n in ("x_kind", "out_f32", "tokens", "k", "n")]
+
+
 _P = C.c_void_p
 _PLAN = C.POINTER(Plan)
 _COMM = C.POINTER(EpComm)
@@ -79,6 +94,12 @@ SIGNATURES = {
     "okc_moe_unpack_bf16": (C.c_int, [_PLAN, _P, C.c_int, C.c_int, _P, _P]),
     "okc_moe_probe_wait_timeout": (C.c_int, [_P, _P]),
     "okc_moe_read_status": (C.c_int, [_P, _P, C.POINTER(C.c_int32)]),
+    "okc_moe_block_norm": (C.c_int, [C.POINTER(BlockNormArgs), _P]),
+    "okc_moe_quantize_rows": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, _P, _P]),
+    "okc_moe_int8_scratch_bytes": (C.c_uint64, [C.c_int, C.c_int32, C.c_int32]),
+    "okc_moe_int8_linear": (C.c_int, [C.POINTER(Int8Args), _P]),
+    "okc_moe_int8_gated": (C.c_int, [C.POINTER(Int8Args), _P]),
+    "okc_moe_int8_status": (C.c_int, [_P, C.POINTER(C.c_int32)]),
     "okc_ep_buffer_bytes": (C.c_uint64, [C.c_int32, C.c_int32, C.c_int32]),
     "okc_ep_views": (C.c_int, [_COMM, C.POINTER(_P), C.POINTER(_P), C.POINTER(_P)]),
     "okc_ep_gather_tokens": (C.c_int, [_COMM, _P, C.c_int64, _P, _P]),

@@ -43,6 +43,18 @@ static bool encode_rows_map(CUtensorMap* map, void* base, uint64_t rows, uint64_
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t row_stride, uint32_t box_rows) {
+  EncodeFn f = encode_fn();
+  if (!f) return false;
+  const cuuint64_t dims[2] = {K, rows};
+  const cuuint64_t strides[1] = {row_stride};
+  const cuuint32_t box[2] = {128, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 static int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -1;
@@ -159,7 +171,7 @@ using namespace okc;
 
 extern "C" {
 
-int okc_moe_version(void) { return 101; }
+int okc_moe_version(void) { return 102; }
 
 const char* okc_moe_strerror(int code) {
   switch (code) {
@@ -611,6 +623,114 @@ int okc_moe_read_status_static(okc_stream_t stream, int32_t* detail) {
   const int rc = static_scratch_address(&scratch);
   if (rc != OKC_OK) return rc;
   return okc_moe_read_status(scratch, stream, detail);
+}
+
+// ---------------------------------------------------------------------------------------------
+// The dense operators around the experts.
+// Rows that 16-byte accesses can read or write: `bytes` is the size of an element.
+static bool rows_vec(const void* p, int64_t stride, int64_t rows, int bytes) {
+  return aligned(p, 16) && (rows <= 1 || (stride * bytes) % 16 == 0);
+}
+
+int okc_moe_block_norm(const okc_block_norm_args* a, okc_stream_t stream) {
+  if (!a || a->rows < 0 || a->rows > INT32_MAX || a->hidden <= 0) return OKC_ERR_BAD_ARG;
+  if (a->hidden > OKC_BLOCK_NORM_MAX_HIDDEN) return OKC_ERR_TOO_LARGE;
+  if (!(a->eps >= 0.0f) || a->out_kind < 0 || a->out_kind > 2 || a->gate_kind < 0 || a->gate_kind > 3) return OKC_ERR_BAD_ARG;
+  if (a->rows == 0) return OKC_OK;
+  const int H = a->hidden;
+  const int64_t rows = a->rows;
+  const bool many_rows = rows > 1;
+  if (!a->residual || (many_rows && a->residual_stride < H)) return OKC_ERR_BAD_ARG;
+  if (a->block) {
+    if (!a->residual_out || (many_rows && (a->block_stride < H || a->residual_out_stride < H))) return OKC_ERR_BAD_ARG;
+  } else if (a->gate || a->post_gain || !a->pre_gain) {
+    return OKC_ERR_BAD_ARG;
+  }
+  if ((a->gate != nullptr) != (a->gate_kind != 0)) return OKC_ERR_BAD_ARG;
+  if (a->gate_kind == 3 && many_rows && a->gate_stride < H) return OKC_ERR_BAD_ARG;
+  if (a->pre_gain && (!a->out || (many_rows && a->out_stride < H) || (a->out_kind == kRowsInt8 && !a->out_scale))) return OKC_ERR_BAD_ARG;
+  if (!is_sm100()) return OKC_ERR_NO_DEVICE;
+  BlockNormParams p;
+  memset(&p, 0, sizeof(p));
+  p.res = a->residual; p.blk = a->block; p.gate = a->gate; p.res_out = a->residual_out; p.out = a->out; p.out_scale = a->out_scale;
+  p.post_gain = a->post_gain; p.pre_gain = a->pre_gain;
+  p.res_stride = a->residual_stride; p.blk_stride = a->block_stride; p.res_out_stride = a->residual_out_stride; p.out_stride = a->out_stride;
+  p.gate_stride = a->gate_kind == 1 ? 0 : a->gate_stride;
+  p.gate_col_stride = a->gate_kind == 2 ? 0 : 1;
+  p.H = H; p.res_f32 = a->residual_f32 ? 1 : 0; p.blk_f32 = a->block_f32 ? 1 : 0; p.gate_f32 = a->gate_f32 ? 1 : 0;
+  p.gate_sigmoid = a->gate_sigmoid ? 1 : 0; p.out_kind = a->out_kind;
+  p.res_scale = a->residual_scale; p.blk_scale = a->block_scale; p.eps = a->eps;
+  bool vec = (H % 8) == 0 && rows_vec(p.res, p.res_stride, rows, p.res_f32 ? 4 : 2);
+  if (p.blk) vec = vec && rows_vec(p.blk, p.blk_stride, rows, p.blk_f32 ? 4 : 2) && rows_vec(p.res_out, p.res_out_stride, rows, p.res_f32 ? 4 : 2);
+  if (p.gate && p.gate_col_stride) vec = vec && rows_vec(p.gate, p.gate_stride, rows, p.gate_f32 ? 4 : 2);
+  if (p.post_gain) vec = vec && aligned(p.post_gain, 16);
+  if (p.pre_gain)
+    vec = vec && aligned(p.pre_gain, 16) && rows_vec(p.out, p.out_stride, rows, p.out_kind == kRowsInt8 ? 1 : p.out_kind == kRowsF32 ? 4 : 2);
+  return launch_block_norm(p, rows, vec, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
+}
+
+int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t rows, int32_t cols, void* q, int64_t q_stride,
+                          float* scale, okc_stream_t stream) {
+  if (rows < 0 || rows > INT32_MAX || cols <= 0) return OKC_ERR_BAD_ARG;
+  if (cols > kInt8MaxK) return OKC_ERR_TOO_LARGE;
+  if (rows == 0) return OKC_OK;
+  if (!x || !q || !scale || (rows > 1 && (x_stride < cols || q_stride < cols))) return OKC_ERR_BAD_ARG;
+  if (!is_sm100()) return OKC_ERR_NO_DEVICE;
+  QuantizeParams p;
+  p.x = x; p.q = static_cast<int8_t*>(q); p.scale = scale; p.x_stride = x_stride; p.q_stride = q_stride; p.cols = cols; p.x_f32 = x_f32 ? 1 : 0;
+  const bool vec = (cols % 8) == 0 && rows_vec(x, x_stride, rows, x_f32 ? 4 : 2) && rows_vec(q, q_stride, rows, 1);
+  return launch_quantize_rows(p, rows, vec, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
+}
+
+// Scratch of a product on bf16 / f32 tokens: their int8 rows, then the scales.
+static uint64_t int8_row_bytes(int K) { return (static_cast<uint64_t>(K) + 15) / 16 * 16; }
+
+uint64_t okc_moe_int8_scratch_bytes(int x_kind, int32_t tokens, int32_t k) {
+  if (x_kind == kRowsInt8 || tokens <= kInt8FewTokens || k <= 0) return 0;
+  return static_cast<uint64_t>(tokens) * (int8_row_bytes(k) + 4);
+}
+
+static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  if (!a || a->tokens < 0 || a->k <= 0 || a->n <= 0 || a->x_kind < 0 || a->x_kind > 2) return OKC_ERR_BAD_ARG;
+  if (a->k > kInt8MaxK || a->n > (1 << 30)) return OKC_ERR_TOO_LARGE;
+  if (a->tokens == 0) return OKC_OK;
+  const int T = a->tokens, K = a->k, N = a->n;
+  if (!a->x || !a->w || !a->w_scale || !a->out || (gated && a->bias)) return OKC_ERR_BAD_ARG;
+  if (a->w_stride < K || (a->w_stride % 16) != 0 || !aligned(a->w, 16) || (T > 1 && (a->x_stride < K || a->out_stride < N))) return OKC_ERR_BAD_ARG;
+  if (a->x_kind == kRowsInt8 && (!a->x_scale || !aligned(a->x, 16) || a->x_stride < K || (a->x_stride % 16) != 0)) return OKC_ERR_BAD_ARG;
+  const bool few = T <= kInt8FewTokens;
+  if (!few && a->x_kind != kRowsInt8 && (!a->scratch || !aligned(a->scratch, 16))) return OKC_ERR_BAD_ARG;
+  if (!is_sm100()) return OKC_ERR_NO_DEVICE;
+  Int8Params p;
+  p.x = a->x; p.x_scale = a->x_scale; p.w = static_cast<const int8_t*>(a->w); p.w_scale = a->w_scale; p.bias = a->bias; p.out = a->out;
+  p.x_stride = a->x_stride; p.w_stride = a->w_stride; p.out_stride = a->out_stride; p.x_kind = a->x_kind;
+  p.x_vec = p.x_kind != kRowsInt8 && rows_vec(p.x, p.x_stride, T, p.x_kind == kRowsF32 ? 4 : 2) ? 1 : 0;
+  p.out_f32 = a->out_f32 ? 1 : 0;
+  p.out_vec = rows_vec(p.out, p.out_stride, T, p.out_f32 ? 4 : 2) ? 1 : 0;
+  p.T = T; p.K = K; p.N = N;
+  if (few) return launch_int8_few(p, gated, stream) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
+  bool pdl = false;
+  if (p.x_kind != kRowsInt8) {
+    const int64_t q_stride = static_cast<int64_t>(int8_row_bytes(K));
+    float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(a->scratch) + static_cast<size_t>(T) * q_stride);
+    const int rc = okc_moe_quantize_rows(p.x, p.x_kind == kRowsF32, p.x_stride, T, K, a->scratch, q_stride, scale, stream_);
+    if (rc != OKC_OK) return rc;
+    p.x = a->scratch; p.x_scale = scale; p.x_stride = q_stride; p.x_kind = kRowsInt8;
+    pdl = true;
+  }
+  const cudaError_t e = int8_use_many(T, K, N, gated) ? launch_int8_many(p, gated, pdl, stream) : launch_int8_mid(p, gated, pdl, stream);
+  return e == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
+}
+
+int okc_moe_int8_linear(const okc_int8_args* args, okc_stream_t stream) { return int8_product(args, false, stream); }
+int okc_moe_int8_gated(const okc_int8_args* args, okc_stream_t stream) { return int8_product(args, true, stream); }
+
+int okc_moe_int8_status(okc_stream_t stream, int32_t* detail) {
+  int32_t code = 0;
+  if (int8_read_status(reinterpret_cast<cudaStream_t>(stream), &code) != cudaSuccess) return OKC_ERR_CUDA;
+  if (detail) *detail = code;
+  return code ? OKC_ERR_TIMEOUT : OKC_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,678 @@
+// Products of int8 rows with a scale per token and per weight row (W8A8):
+//   y[t][n] = (sum_k qx[t][k] * qw[n][k]) * (sx[t] * sw[n]) (+ bias[n])         okc_moe_int8_linear
+//   h[t][i] = g / (1 + exp(-g)) * u,  g = y[t][i], u = y[t][I + i]              okc_moe_int8_gated
+// The integer sum is exact in 32 bits (K <= 131071), so its value does not depend on how K is split, and every kernel
+// below turns it into the result with the same f32 operations: a token's bits do not depend on the batch it is in.
+//
+// Three kernels, by what bounds the product:
+//   okc_int8_few   up to 8 tokens   the weights are read once by plain 16-byte loads and multiplied on the integer
+//                                   dot-product units; the token rows are quantised in the kernel (one launch)
+//   okc_int8_mid   some hundred     the weights fill M of a tcgen05.mma (kind::i8), the tokens are N; K is split over a
+//                                   cluster of CTAs that add their integer sums through distributed shared memory
+//   okc_int8_many  beyond           CTA pairs (cta_group::2) on tiles of 256 tokens x up to 256 weight rows, persistent
+// Every wait on a barrier is bounded; one that runs out is reported through a status word (okc_moe_int8_status).
+#include <cooperative_groups.h>
+
+#include "rows.cuh"
+
+namespace okc {
+
+namespace cg = cooperative_groups;
+
+__device__ int32_t g_int8_status;      // code of the first wait that ran out since the last read
+
+// ------------------------------------------------------------------ what every kernel does with an integer sum
+__device__ __forceinline__ float int8_value(int acc, float sx, float sw) { return __fmul_rn(__int2float_rn(acc), __fmul_rn(sx, sw)); }
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fmul_rn(__fdividef(g, 1.f + __expf(-g)), u); }
+
+// ------------------------------------------------------------------ few tokens
+constexpr int kFewThreads = 1024;
+constexpr int kFewChunk = 512;         // K elements of one warp-wide 16-byte load
+constexpr int kFewRowsMax = 512;       // most weight rows a CTA owns (its integer sums live in shared memory)
+
+// Sixteen values of a token row at column k (zeros past K), as f32.
+__device__ __forceinline__ void few_load_x(const Int8Params& p, int t, int k, float (&v)[16]) {
+  const int64_t o = t * p.x_stride + k;
+  if (p.x_vec && k + 16 <= p.K) {
+    if (p.x_kind == kRowsF32) {
+      const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { const float4 a = s[j]; v[4 * j] = a.x; v[4 * j + 1] = a.y; v[4 * j + 2] = a.z; v[4 * j + 3] = a.w; }
+    } else {
+      const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + o);
+      float a[8], b[8];
+      unpack_bf16x8(s[0], a); unpack_bf16x8(s[1], b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) { v[j] = a[j]; v[8 + j] = b[j]; }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      v[j] = 0.f;
+      if (k + j < p.K)
+        v[j] = p.x_kind == kRowsF32 ? static_cast<const float*>(p.x)[o + j]
+                                    : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p.x)[o + j]) << 16);
+    }
+  }
+}
+// Sixteen int8 values at column k of an aligned row, zeros past K (the bytes behind a row's end are never used).
+__device__ __forceinline__ uint4 load_q16(const int8_t* row, int k, int K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (k + j < K) w[j >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + j])) << (8 * (j & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A CTA owns `rows_per_cta` neighbouring outputs and all of K.  A warp keeps one 512-wide chunk of K: its 16 bytes of
+// every token row stay in registers (quantised there), and it walks over the CTA's weight rows with one 16-byte load a
+// lane and row; `kTok` integer dot products, a warp sum each, and one shared-memory add.  With all 32 warps loading
+// four rows ahead an SM has 64 KB in flight, above what the HBM rate needs.
+template <int kTok, bool kGated>
+__global__ void __launch_bounds__(kFewThreads) okc_int8_few(const Int8Params p, int rows_per_cta) {
+  extern __shared__ int few_acc[];      // [rows][kTok]
+  __shared__ uint32_t amax_s[kTok];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n0 = blockIdx.x * rows_per_cta;
+  const int nr = min(rows_per_cta, p.N - n0);
+  const int rows = kGated ? 2 * nr : nr;
+  const int chunks = (p.K + kFewChunk - 1) / kFewChunk;
+  const int groups = chunks >= 32 ? 1 : 32 / chunks;
+  const int group = chunks >= 32 ? 0 : warp / chunks;
+  for (int i = tid; i < rows * kTok; i += kFewThreads) few_acc[i] = 0;
+  if (tid < kTok) amax_s[tid] = 0;
+  __syncthreads();
+
+  const bool raw = p.x_kind != kRowsInt8;
+  if (raw) {
+    if (group == 0)
+      for (int c = warp; c < chunks; c += 32) {
+        const int k = c * kFewChunk + lane * 16;
+#pragma unroll
+        for (int t = 0; t < kTok; ++t) {
+          uint32_t m = 0;
+          if (t < p.T && k < p.K) {
+            float v[16];
+            few_load_x(p, t, k, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) m = max(m, abs_bits(v[j]));
+          }
+          m = __reduce_max_sync(0xffffffffu, m);
+          if (lane == 0) atomicMax(&amax_s[t], m);
+        }
+      }
+    __syncthreads();
+  }
+  if (group < groups) {
+    for (int c = chunks >= 32 ? warp : warp % chunks; c < chunks; c += chunks >= 32 ? 32 : chunks) {
+      const int k = c * kFewChunk + lane * 16;
+      uint4 xq[kTok];
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) {
+        xq[t] = make_uint4(0, 0, 0, 0);
+        if (t < p.T && k < p.K) {
+          if (raw) {
+            float v[16];
+            few_load_x(p, t, k, v);
+            const float inv = row_scale(amax_s[t]).inv;
+            xq[t].x = quant8x4(v[0], v[1], v[2], v[3], inv);
+            xq[t].y = quant8x4(v[4], v[5], v[6], v[7], inv);
+            xq[t].z = quant8x4(v[8], v[9], v[10], v[11], inv);
+            xq[t].w = quant8x4(v[12], v[13], v[14], v[15], inv);
+          } else {
+            xq[t] = load_q16(static_cast<const int8_t*>(p.x) + t * p.x_stride, k, p.K);
+          }
+        }
+      }
+      for (int r0 = group; r0 < rows; r0 += 4 * groups) {
+        uint4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int r = r0 + u * groups;
+          w[u] = make_uint4(0, 0, 0, 0);
+          if (r < rows && k < p.K) {
+            const int n = kGated ? (r < nr ? n0 + r : p.N + n0 + r - nr) : n0 + r;
+            w[u] = load_q16(p.w + n * p.w_stride, k, p.K);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int r = r0 + u * groups;
+          if (r >= rows) break;
+          int mine = 0;
+#pragma unroll
+          for (int t = 0; t < kTok; ++t) {
+            int d = __dp4a(static_cast<int>(w[u].x), static_cast<int>(xq[t].x), 0);
+            d = __dp4a(static_cast<int>(w[u].y), static_cast<int>(xq[t].y), d);
+            d = __dp4a(static_cast<int>(w[u].z), static_cast<int>(xq[t].z), d);
+            d = __dp4a(static_cast<int>(w[u].w), static_cast<int>(xq[t].w), d);
+            d = __reduce_add_sync(0xffffffffu, d);
+            if (lane == t) mine = d;
+          }
+          if (lane < kTok) atomicAdd(&few_acc[r * kTok + lane], mine);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < nr * p.T; i += kFewThreads) {
+    const int t = i / nr, j = i - t * nr, n = n0 + j;
+    const float sx = raw ? row_scale(amax_s[t]).scale : p.x_scale[t];
+    float v = int8_value(few_acc[j * kTok + t], sx, p.w_scale[n]);
+    if (kGated) v = silu_mul(v, int8_value(few_acc[(nr + j) * kTok + t], sx, p.w_scale[p.N + n]));
+    else if (p.bias) v = __fadd_rn(v, p.bias[n]);
+    if (p.out_f32) static_cast<float*>(p.out)[t * p.out_stride + n] = v;
+    else static_cast<__nv_bfloat16*>(p.out)[t * p.out_stride + n] = __float2bfloat16_rn(v);
+  }
+}
+
+static int few_tok(int T) { return T <= 1 ? 1 : T <= 2 ? 2 : T <= 4 ? 4 : 8; }
+
+cudaError_t launch_int8_few(const Int8Params& p, bool gated, cudaStream_t stream) {
+  int rpc = (p.N + 147) / 148;
+  const int most = gated ? kFewRowsMax / 2 : kFewRowsMax;
+  if (rpc > most) rpc = most;
+  const int tok = few_tok(p.T);
+  const size_t smem = static_cast<size_t>(gated ? 2 : 1) * rpc * tok * sizeof(int);
+  const dim3 grid((p.N + rpc - 1) / rpc), block(kFewThreads);
+#define OKC_FEW(TOK) return gated ? launch_kernel(okc_int8_few<TOK, true>, grid, block, smem, stream, false, p, rpc) : launch_kernel(okc_int8_few<TOK, false>, grid, block, smem, stream, false, p, rpc)
+  if (tok == 1) OKC_FEW(1);
+  if (tok == 2) OKC_FEW(2);
+  if (tok == 4) OKC_FEW(4);
+  OKC_FEW(8);
+#undef OKC_FEW
+}
+
+// ------------------------------------------------------------------ tcgen05 pieces shared by the two tiled kernels
+// Instruction descriptor: int8 x int8 -> int32, both operands K-major, M = m, N = n.
+__device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void store_out(const Int8Params& p, int64_t o, float v) {
+  if (p.out_f32) static_cast<float*>(p.out)[o] = v;
+  else static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v);
+}
+
+// ------------------------------------------------------------------ some hundred tokens
+constexpr int kMidThreads = 192;       // warps 0..3 epilogue, 4 TMA producer, 5 MMA issuer
+constexpr int kMidMaxStages = 8;
+constexpr int kKb = 128;               // K elements of a stage: one 128-byte swizzled row
+constexpr int kTileW = 128;            // weight rows of a tile
+
+struct Int8MidParams {
+  CUtensorMap wmap;      // int8 weight rows, box 128 x 128 rows (64 for the gated product: a gate and an up box)
+  CUtensorMap xmap;      // int8 token rows, box 128 x tn
+  Int8Params p;
+  int tn, stages, n_kb, splits, tmem_cols;
+};
+
+template <bool kGated>
+__global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constant__ Int8MidParams q) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = smem_u32(smem_raw);
+  const uint32_t smem0 = (smem_base + 1023u) & ~1023u;
+  __shared__ uint64_t bar_full[kMidMaxStages], bar_empty[kMidMaxStages], bar_done;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_code;
+  const Int8Params& p = q.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x % q.splits, tile = blockIdx.x / q.splits;
+  const int w0 = tile * (kGated ? kTileW / 2 : kTileW);      // first output of the tile
+  const int t0 = blockIdx.y * q.tn;
+  const int kb0 = static_cast<int>(static_cast<long long>(q.n_kb) * rank / q.splits);
+  const int nkb = static_cast<int>(static_cast<long long>(q.n_kb) * (rank + 1) / q.splits) - kb0;
+  const uint32_t stage_bytes = kTileW * kKb + static_cast<uint32_t>(q.tn) * kKb;
+
+  if (tid == 0) {
+    for (int i = 0; i < kMidMaxStages; ++i) { mbar_init(smem_u32(&bar_full[i]), 1); mbar_init(smem_u32(&bar_empty[i]), 1); }
+    mbar_init(smem_u32(&bar_done), 1);
+    abort_code = 0;
+    mbar_fence_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(smem_u32(&tmem_base_s), static_cast<uint32_t>(q.tmem_cols));
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      auto load_w = [&](int i) {
+        const uint32_t bar = smem_u32(&bar_full[i % q.stages]), dst = smem0 + (i % q.stages) * stage_bytes;
+        mbar_expect_tx(bar, stage_bytes);
+        tma_2d_g2s(dst, &q.wmap, (kb0 + i) * kKb, w0, bar);
+        if (kGated) tma_2d_g2s(dst + kTileW / 2 * kKb, &q.wmap, (kb0 + i) * kKb, p.N + w0, bar);
+      };
+      auto load_x = [&](int i) {
+        const uint32_t bar = smem_u32(&bar_full[i % q.stages]), dst = smem0 + (i % q.stages) * stage_bytes;
+        tma_2d_g2s(dst + kTileW * kKb, &q.xmap, (kb0 + i) * kKb, t0, bar);
+      };
+      // the weights of the first stages do not depend on the kernel before this one, the token rows may
+      const int first = min(nkb, q.stages);
+      for (int i = 0; i < first; ++i) load_w(i);
+      griddep_wait();
+      for (int i = 0; i < first; ++i) load_x(i);
+      int i = first;
+      for (; i < nkb; ++i) {
+        if (!mbar_wait(smem_u32(&bar_empty[i % q.stages]), ((i / q.stages) & 1) ^ 1, &abort_code, 0x61)) break;
+        load_w(i);
+        load_x(i);
+      }
+      if (i < nkb) {
+        // give the copies in flight a bounded chance to land before the CTA retires
+        for (int j = max(0, i - q.stages); j < i; ++j) {
+          const long long c0 = clock64();
+          while (!mbar_try(smem_u32(&bar_full[j % q.stages]), (j / q.stages) & 1) && clock64() - c0 < kWaitLimitCycles) {}
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    if (lane == 0) {
+      const uint32_t idesc = idesc_i8(128, static_cast<uint32_t>(q.tn));
+      bool ok = true;
+      for (int i = 0; i < nkb; ++i) {
+        ok = mbar_wait(smem_u32(&bar_full[i % q.stages]), (i / q.stages) & 1, &abort_code, 0x62);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t a = smem0 + (i % q.stages) * stage_bytes;
+        const uint64_t ad = smem_desc_sw128(a), bd = smem_desc_sw128(a + kTileW * kKb);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) mma_i8(tmem, ad + 2 * ks, bd + 2 * ks, idesc, (i | ks) != 0 ? 1u : 0u);   // K = 32 each
+        mma_commit(smem_u32(&bar_empty[i % q.stages]));
+      }
+      mma_commit(smem_u32(&bar_done));
+    }
+    __syncwarp();
+  } else {
+    griddep_wait();        // the token scales come from the kernel before this one
+    const bool ok = mbar_wait<40>(smem_u32(&bar_done), 0, &abort_code, 0x63);
+    tc_fence_after();
+    if (ok) {
+      // this CTA's sums, [token][weight row], over the ring slots (every copy has landed and every MMA has read them)
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+      int* part = reinterpret_cast<int*>(smem_raw + (smem0 - smem_base));
+      for (int c0 = 0; c0 < q.tn; c0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(taddr + c0, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c0 + j) * kTileW + warp * 32 + lane] = static_cast<int>(r[j]);
+      }
+    }
+    tc_fence_before();
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  if (q.splits > 1) cluster.sync(); else __syncthreads();
+
+  // Each CTA of the cluster finishes tn / splits tokens: it adds the integer sums of all CTAs and stores the rows.
+  if (warp < 4) {
+    const int per = q.tn / q.splits;
+    int* part = reinterpret_cast<int*>(smem_raw + (smem0 - smem_base));
+    const int quads = kGated ? kTileW / 8 : kTileW / 4;
+    for (int i = tid; i < per * quads; i += 128) {
+      const int col = rank * per + i / quads, o4 = (i % quads) * 4, t = t0 + col;
+      if (t >= p.T) break;
+      int4 a = make_int4(0, 0, 0, 0), b = a;
+      for (int s = 0; s < q.splits; ++s) {
+        const int* src = q.splits > 1 ? cluster.map_shared_rank(part, s) : part;
+        const int4 v = *reinterpret_cast<const int4*>(src + col * kTileW + o4);
+        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        if (kGated) {
+          const int4 u = *reinterpret_cast<const int4*>(src + col * kTileW + kTileW / 2 + o4);
+          b.x += u.x; b.y += u.y; b.z += u.z; b.w += u.w;
+        }
+      }
+      const float sx = p.x_scale[t];
+      const int av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+      const int n = w0 + o4;
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = 0.f;
+        if (n + j < p.N) {
+          v[j] = int8_value(av[j], sx, p.w_scale[n + j]);
+          if (kGated) v[j] = silu_mul(v[j], int8_value(bv[j], sx, p.w_scale[p.N + n + j]));
+          else if (p.bias) v[j] = __fadd_rn(v[j], p.bias[n + j]);
+        }
+      }
+      const int64_t o = t * p.out_stride + n;
+      if (p.out_vec && n + 4 <= p.N) {
+        if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = make_float4(v[0], v[1], v[2], v[3]);
+        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) store_out(p, o + j, v[j]);
+      }
+    }
+  }
+  if (q.splits > 1) cluster.sync(); else __syncthreads();   // no CTA leaves while another reads its sums
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, static_cast<uint32_t>(q.tmem_cols));
+  }
+  if (tid == 0 && abort_code != 0) atomicCAS(&g_int8_status, 0, abort_code);
+}
+
+static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
+
+cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream) {
+  Int8MidParams q;
+  q.p = p;
+  const int per_tile = gated ? kTileW / 2 : kTileW;
+  const int tiles = (p.N + per_tile - 1) / per_tile;
+  const int ttiles = (p.T + 255) / 256;
+  q.tn = ((p.T + ttiles - 1) / ttiles + 15) & ~15;
+  q.n_kb = (p.K + kKb - 1) / kKb;
+  q.splits = 1;
+  while (q.splits < 8 && 2 * q.splits <= q.n_kb && 2LL * q.splits * tiles * ttiles <= 2 * 148) q.splits *= 2;
+  const int stage = kTileW * kKb + q.tn * kKb;
+  const int budget = q.tn <= 64 ? 108 * 1024 : 216 * 1024;
+  q.stages = budget / stage;
+  if (q.stages > kMidMaxStages) q.stages = kMidMaxStages;
+  q.tmem_cols = tmem_cols_for(q.tn);
+  if (!encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(gated ? 2 : 1) * p.N, p.K, p.w_stride, per_tile) ||
+      !encode_bytes_map(&q.xmap, p.x, p.T, p.K, p.x_stride, q.tn))
+    return cudaErrorInvalidValue;
+  size_t smem = 1024 + static_cast<size_t>(q.stages) * stage;
+  const size_t sums = 1024 + static_cast<size_t>(q.tn) * kTileW * 4;
+  if (smem < sums) smem = sums;
+  auto kernel = gated ? okc_int8_mid<true> : okc_int8_mid<false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles * q.splits, ttiles);
+  cfg.blockDim = dim3(kMidThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  attr[n].id = cudaLaunchAttributeClusterDimension;
+  attr[n].val.clusterDim.x = q.splits; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
+  ++n;
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, q);
+}
+
+// ------------------------------------------------------------------ many tokens
+constexpr int kManyThreads = 256;      // warps 0 TMA producer, 1 MMA issuer (leader CTA), 2 TMEM, 4..7 epilogue
+constexpr int kManyStages = 6;
+constexpr int kManyStageBytes = 2 * 128 * kKb;
+constexpr int kManySmem = 1024 + kManyStages * kManyStageBytes;
+
+struct Int8ManyParams {
+  CUtensorMap xmap;      // int8 token rows, box 128 x 128 rows
+  CUtensorMap wmap;      // int8 weight rows, box 128 x bn / 2 rows
+  Int8Params p;
+  int bn;                // weight rows of a pair's tile (columns of its accumulator): a multiple of 32, at most 256
+  int n_kb, tiles_t, tiles_n;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// The same shared-memory address in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait on a barrier that the other CTA of the pair takes part in (see mbar_wait).
+__device__ __forceinline__ bool pair_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  if (mbar_try_cluster(bar, parity)) return true;
+  const uint32_t c0 = static_cast<uint32_t>(clock());
+#pragma unroll 1
+  for (;;) {
+    if (mbar_try_cluster(bar, parity)) return true;
+    if (*abort_flag != 0) return false;
+    if (static_cast<uint32_t>(clock()) - c0 > kWaitLimit) break;
+  }
+  atomicCAS(const_cast<int*>(abort_flag), 0, code);
+  return false;
+}
+// TMA load into this CTA's shared memory whose bytes count on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs once every MMA of the pair issued so far has completed.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .b16 m;\n\t"
+      "mov.b16 m, 3;\n\t"
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}"
+      ::"r"(bar)
+      : "memory");
+}
+
+template <bool kGated>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_int8_many(const __grid_constant__ Int8ManyParams q) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  __shared__ uint64_t bar_full[kManyStages], bar_empty[kManyStages], bar_acc_full[2], bar_acc_empty[2];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_code;
+  const Int8Params& p = q.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = q.tiles_t * q.tiles_n;
+
+  if (tid == 0) {
+    for (int i = 0; i < kManyStages; ++i) { mbar_init(smem_u32(&bar_full[i]), 1); mbar_init(smem_u32(&bar_empty[i]), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&bar_acc_full[i]), 1); mbar_init(smem_u32(&bar_acc_empty[i]), 8); }
+    abort_code = 0;
+    mbar_fence_init();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cg::this_cluster().sync();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      griddep_wait();
+      const uint32_t half_bytes = 128u * kKb + static_cast<uint32_t>(q.bn / 2) * kKb;
+      int it = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        const int tt = tile % q.tiles_t, tw = tile / q.tiles_t;
+        const int xrow = tt * 256 + static_cast<int>(rank) * 128;
+        const int wrow = kGated ? static_cast<int>(rank) * p.N + tw * (q.bn / 2) : tw * q.bn + static_cast<int>(rank) * (q.bn / 2);
+        for (int kb = 0; kb < q.n_kb; ++kb, ++it) {
+          const int s = it % kManyStages;
+          if (it >= kManyStages && !pair_wait(smem_u32(&bar_empty[s]), ((it / kManyStages) & 1) ^ 1, &abort_code, 0x71)) { ok = false; break; }
+          // the bytes of both CTAs count on the leader's barrier
+          const uint32_t bar = map_rank(smem_u32(&bar_full[s]), 0);
+          if (rank == 0) mbar_expect_tx(smem_u32(&bar_full[s]), 2 * half_bytes);
+          const uint32_t dst = smem0 + s * kManyStageBytes;
+          tma_2d_pair(dst, &q.xmap, kb * kKb, xrow, bar);
+          tma_2d_pair(dst + 128 * kKb, &q.wmap, kb * kKb, wrow, bar);
+        }
+      }
+      // The copies still in flight have landed once the MMA issuer has seen them; it waits for all of them unless it
+      // gave up, and then they get a bounded time here.
+      if (!ok) {
+        const long long c0 = clock64();
+        while (clock64() - c0 < kWaitLimitCycles / 100) {}
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_i8(256, static_cast<uint32_t>(q.bn));
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs, ++n) {
+        const int buf = n & 1;
+        if (n >= 2 && !pair_wait(smem_u32(&bar_acc_empty[buf]), ((n >> 1) & 1) ^ 1, &abort_code, 0x72)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * 256;
+        for (int kb = 0; kb < q.n_kb; ++kb, ++it) {
+          const int s = it % kManyStages;
+          ok = pair_wait(smem_u32(&bar_full[s]), (it / kManyStages) & 1, &abort_code, 0x73);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a = smem0 + s * kManyStageBytes;
+          const uint64_t ad = smem_desc_sw128(a), bd = smem_desc_sw128(a + 128 * kKb);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) mma_i8_pair(d, ad + 2 * ks, bd + 2 * ks, idesc, (kb | ks) != 0 ? 1u : 0u);
+          mma_commit_pair(smem_u32(&bar_empty[s]));
+        }
+        if (ok) mma_commit_pair(smem_u32(&bar_acc_full[buf]));
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    griddep_wait();        // the token scales come from the kernel before this one
+    const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int half = q.bn / 2;
+    int n = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++n) {
+      const int buf = n & 1;
+      if (!pair_wait(smem_u32(&bar_acc_full[buf]), (n >> 1) & 1, &abort_code, 0x74)) break;
+      tc_fence_after();
+      const int tt = tile % q.tiles_t, tw = tile / q.tiles_t;
+      const int t = tt * 256 + static_cast<int>(rank) * 128 + (warp & 3) * 32 + lane;
+      const float sx = t < p.T ? p.x_scale[t] : 0.f;
+      const int width = kGated ? half : q.bn;        // outputs of the tile
+      for (int c0 = 0; c0 < width; c0 += 16) {
+        uint32_t r[16], u[16];
+        tmem_ld16(taddr + buf * 256 + c0, r);
+        if (kGated) tmem_ld16(taddr + buf * 256 + half + c0, u);
+        tmem_wait_ld();
+        const int n0 = tw * width + c0;
+        const bool live = t < p.T;
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[j] = 0.f;
+          if (n0 + j < p.N) {
+            v[j] = int8_value(static_cast<int>(r[j]), sx, __ldg(p.w_scale + n0 + j));
+            if (kGated) v[j] = silu_mul(v[j], int8_value(static_cast<int>(u[j]), sx, __ldg(p.w_scale + p.N + n0 + j)));
+            else if (p.bias) v[j] = __fadd_rn(v[j], __ldg(p.bias + n0 + j));
+          }
+        }
+        const int64_t o = t * p.out_stride + n0;
+        if (live && p.out_vec && n0 + 16 <= p.N) {
+          if (p.out_f32) {
+            float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.out) + o);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          } else {
+            uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              d[j] = make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                                pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+          }
+        } else if (live) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (n0 + j < p.N) store_out(p, o + j, v[j]);
+        }
+        __syncwarp();      // the next load from tensor memory is one of the whole warp
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&bar_acc_empty[buf]), 0));
+    }
+  }
+  tc_fence_before();
+  cg::this_cluster().sync();     // no CTA frees its tensor memory or leaves while the pair's MMAs and arrivals may touch it
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+  if (tid == 0 && abort_code != 0) atomicCAS(&g_int8_status, 0, abort_code);
+}
+
+bool int8_use_many(int T, int K, int N, bool gated) { (void)K; (void)N; (void)gated; return T > 256; }
+
+cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream) {
+  Int8ManyParams q;
+  q.p = p;
+  q.n_kb = (p.K + kKb - 1) / kKb;
+  q.tiles_t = (p.T + 255) / 256;
+  const int64_t cols = static_cast<int64_t>(gated ? 2 : 1) * p.N;
+  // The tile width that leaves the least work in the last round of the 74 pairs.
+  q.bn = 256;
+  long long best = -1;
+  for (int bn = 256; bn >= 128; bn -= 32) {
+    const long long tn = (cols + bn - 1) / bn;
+    const long long cost = ((tn * q.tiles_t + 73) / 74) * (bn + 16);
+    if (best < 0 || cost < best) { best = cost; q.bn = bn; q.tiles_n = static_cast<int>(tn); }
+  }
+  if (gated) q.tiles_n = (p.N + q.bn / 2 - 1) / (q.bn / 2);
+  if (!encode_bytes_map(&q.xmap, p.x, p.T, p.K, p.x_stride, 128) ||
+      !encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(cols), p.K, p.w_stride, q.bn / 2))
+    return cudaErrorInvalidValue;
+  const long long tiles = static_cast<long long>(q.tiles_t) * q.tiles_n;
+  const int grid = static_cast<int>(tiles < 74 ? 2 * tiles : 148);
+  auto kernel = gated ? okc_int8_many<true> : okc_int8_many<false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kernel, dim3(grid), dim3(kManyThreads), kManySmem, stream, pdl, q);
+}
+
+__global__ void okc_int8_clear_status() { g_int8_status = 0; }
+
+cudaError_t int8_read_status(cudaStream_t stream, int32_t* code) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(code, g_int8_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, stream);
+  if (e != cudaSuccess) return e;
+  okc_int8_clear_status<<<1, 1, 0, stream>>>();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return cudaStreamSynchronize(stream);
+}
+
+}  // namespace okc

@@ -129,6 +129,57 @@ cudaError_t launch_ep_combine_reduce(const EpParams& p, const CombineParams& c, 
 cudaError_t launch_cast(const float* in, void* out_bf16, int64_t n, cudaStream_t stream);
 cudaError_t launch_wait_timeout_probe(int32_t* status, cudaStream_t stream);
 
+// The residual stream around a block (norm.cu).
+enum RowsKind { kRowsBf16 = 0, kRowsF32 = 1, kRowsInt8 = 2 };
+struct BlockNormParams {
+  const void* res;            // residual rows (bf16 or f32), row strides in elements
+  const void* blk;            // block output rows or null: only the norm before a block runs
+  const void* gate;           // or null
+  void* res_out;
+  void* out;
+  float* out_scale;           // int8 rows only
+  const float* post_gain;     // f32 [H] or null: no norm after the block
+  const float* pre_gain;      // f32 [H] or null: no norm before the next block
+  int64_t res_stride, blk_stride, gate_stride, res_out_stride, out_stride;
+  int gate_col_stride;        // 0: one value a row, 1: one a channel
+  int H, res_f32, blk_f32, gate_f32, gate_sigmoid, out_kind;
+  float res_scale, blk_scale, eps;
+};
+cudaError_t launch_block_norm(const BlockNormParams& p, int64_t rows, bool vec, cudaStream_t stream);
+
+struct QuantizeParams {
+  const void* x;
+  int8_t* q;
+  float* scale;
+  int64_t x_stride, q_stride;
+  int cols, x_f32;
+};
+cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool vec, cudaStream_t stream);
+
+// The int8 products (int8.cu).
+struct Int8Params {
+  const void* x;              // token rows: int8 with x_scale, or (few tokens only) bf16 / f32 rows quantised in the kernel
+  const float* x_scale;
+  const int8_t* w;            // weight rows, K int8 values each
+  const float* w_scale;       // f32, one per weight row
+  const float* bias;          // f32 [N] or null
+  void* out;
+  int64_t x_stride, w_stride, out_stride;
+  int x_kind;                 // RowsKind
+  int x_vec;                  // 16-byte loads of the token rows are possible
+  int out_f32, out_vec;       // out_vec: 16-byte stores of an output row are possible from any column that is a multiple of 8
+  int T, K, N;                // N = outputs: weight rows, or half of them for the gated product
+};
+constexpr int kInt8FewTokens = 8;
+constexpr int kInt8MaxK = 131071;          // 128 * 128 * K stays below 2^31
+cudaError_t launch_int8_few(const Int8Params& p, bool gated, cudaStream_t stream);
+cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream);
+cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream);
+bool int8_use_many(int T, int K, int N, bool gated);
+cudaError_t int8_read_status(cudaStream_t stream, int32_t* code);
+// Tensor map of int8 rows (abi.cu): box = 128 bytes x box_rows, 128-byte swizzle, zero fill outside.
+bool encode_bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t row_stride, uint32_t box_rows);
+
 // Launch with (pdl = true) or without the programmatic-serialization attribute.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,

@@ -1,0 +1,143 @@
+// Row helpers shared by the norm, quantising and int8 product kernels: loads of eight consecutive values as f32, the
+// rounding to bf16 and to int8, and sums / maxima over the threads of a CTA that share a row.
+#pragma once
+#include <cuda_bf16.h>
+
+#include <cstdint>
+
+#include "params.cuh"
+
+namespace okc {
+
+// Rows of int8 values.  With a = max |x| of the row: scale = a / 127, value = rint(x * (127 / a)), both quotients
+// rounded to f32 once per row and the product rounded to f32 once, so every kernel that quantises (and a caller that
+// does it elsewhere) gets the same integers.  A row with a < 2^-120 (127 / a would leave the range of f32) counts as
+// zeros: scale 0.  A row that holds an infinity or a NaN gets scale NaN and zeros, so that every product of the row
+// is NaN instead of a number made from part of it.
+struct RowScale {
+  float scale, inv;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
+  RowScale s;
+  const float a = __uint_as_float(amax_bits);
+  if (amax_bits >= 0x7F800000u) { s.scale = __uint_as_float(0x7FC00000u); s.inv = 0.f; }
+  else if (a < 7.52316385e-37f) { s.scale = 0.f; s.inv = 0.f; }
+  else { s.scale = __fdiv_rn(a, 127.f); s.inv = __fdiv_rn(127.f, a); }
+  return s;
+}
+// x * inv is within 127 * (1 + 2^-23) of zero, so the rounded value needs no clamp.  A row that is not finite has
+// inv = 0: infinity * 0 is NaN, which the conversion to an integer makes 0.
+__device__ __forceinline__ uint32_t quant8(float x, float inv) { return static_cast<uint32_t>(__float2int_rn(__fmul_rn(x, inv))) & 0xFFu; }
+__device__ __forceinline__ uint32_t quant8x4(float a, float b, float c, float d, float inv) {
+  return quant8(a, inv) | (quant8(b, inv) << 8) | (quant8(c, inv) << 16) | (quant8(d, inv) << 24);
+}
+// Bits of |x|: compared as integers a NaN is above every number, so a maximum of these never loses one.
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+__device__ __forceinline__ void unpack_bf16x8(uint4 u, float (&v)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(w[j] << 16);
+    v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// The columns of a row belong to threads in chunks of eight.  With kVec a chunk is eight neighbours (16- and 32-byte
+// accesses; the host checks that the width and every stride and address allow them); without, neighbouring threads
+// take neighbouring columns, so that single-element accesses still coalesce.
+template <bool kVec>
+__device__ __forceinline__ int row_col(int chunk, int e, int tid, int nt) {
+  return kVec ? (chunk * nt + tid) * 8 + e : (chunk * 8 + e) * nt + tid;
+}
+template <bool kVec>
+__device__ __forceinline__ void load_chunk(const void* row, bool f32, int chunk, int tid, int nt, int cols, float (&v)[8]) {
+  if (kVec) {
+    const int c = row_col<true>(chunk, 0, tid, nt);
+    if (c < cols) {
+      if (f32) {
+        const float4 a = reinterpret_cast<const float4*>(static_cast<const float*>(row) + c)[0];
+        const float4 b = reinterpret_cast<const float4*>(static_cast<const float*>(row) + c)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      } else {
+        unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c), v);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = row_col<false>(chunk, e, tid, nt);
+      v[e] = 0.f;
+      if (c < cols) v[e] = f32 ? static_cast<const float*>(row)[c] : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(row)[c]) << 16);
+    }
+  }
+}
+template <bool kVec>
+__device__ __forceinline__ void store_chunk(void* row, bool f32, int chunk, int tid, int nt, int cols, const float (&v)[8]) {
+  if (kVec) {
+    const int c = row_col<true>(chunk, 0, tid, nt);
+    if (c >= cols) return;
+    if (f32) {
+      float4* d = reinterpret_cast<float4*>(static_cast<float*>(row) + c);
+      d[0] = make_float4(v[0], v[1], v[2], v[3]);
+      d[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + c) =
+          make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = row_col<false>(chunk, e, tid, nt);
+      if (c < cols) {
+        if (f32) static_cast<float*>(row)[c] = v[e];
+        else static_cast<__nv_bfloat16*>(row)[c] = __float2bfloat16_rn(v[e]);
+      }
+    }
+  }
+}
+template <bool kVec>
+__device__ __forceinline__ void store_chunk_q(int8_t* row, int chunk, int tid, int nt, int cols, const float (&v)[8], float inv) {
+  if (kVec) {
+    const int c = row_col<true>(chunk, 0, tid, nt);
+    if (c < cols) *reinterpret_cast<uint2*>(row + c) = make_uint2(quant8x4(v[0], v[1], v[2], v[3], inv), quant8x4(v[4], v[5], v[6], v[7], inv));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = row_col<false>(chunk, e, tid, nt);
+      if (c < cols) row[c] = static_cast<int8_t>(quant8(v[e], inv));
+    }
+  }
+}
+
+// Sum / maximum over all threads of the CTA (a multiple of 32, at most 1024).  `red` is 32 words of shared memory that
+// no other call of the kernel uses, so one barrier is enough.  The order of the additions depends on the thread count
+// alone.
+__device__ __forceinline__ float cta_sum(float x, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if (blockDim.x == 32) return x;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = (threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+__device__ __forceinline__ uint32_t cta_max(uint32_t x, uint32_t* red) {
+  x = __reduce_max_sync(0xffffffffu, x);
+  if (blockDim.x == 32) return x;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = (threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0u;
+  return __reduce_max_sync(0xffffffffu, x);
+}
+
+}  // namespace okc

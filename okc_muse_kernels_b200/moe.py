@@ -18,9 +18,10 @@ import torch
 
 from . import _lib
 from ._lib import OkcError, Plan, Sizes
+from .dense import block_norm
 
 __all__ = ["MoEPlan", "prepare", "kernel_fn", "moe_step", "route", "sorted_routes", "unpack_bf16", "read_status", "split_router",
-           "experts_profiled", "experts_ep", "cast_bf16", "HostStep", "route_hidden", "moe_layer_step", "OkcError"]
+           "experts_profiled", "experts_ep", "cast_bf16", "HostStep", "route_hidden", "moe_layer_step", "moe_block_step", "OkcError"]
 
 
 @dataclass(frozen=True)
@@ -377,6 +378,22 @@ def moe_layer_step(hidden_states: torch.Tensor, router_w: torch.Tensor, state: d
         out = torch.empty((T, plan.hidden), dtype=torch.float32 if out_f32 else torch.bfloat16, device=hidden.device)
     _experts(hidden, stride, T, state, out, out_f32)
     return out
+
+
+def moe_block_step(residual: torch.Tensor, router_w: torch.Tensor, state: dict, *, pre_gain: torch.Tensor,
+                   post_gain: torch.Tensor | None = None, gate: torch.Tensor | None = None, gate_sigmoid: bool = False,
+                   residual_scale: float = 1.0, block_scale: float = 1.0, next_gain: torch.Tensor | None = None,
+                   eps: float = 1e-5, out: str = "bf16", residual_out: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, mode: str = "softmax", multiplier: float = SIGMOID_MULTIPLIER,
+                   own_tokens=None):
+    """The whole expert block on the residual stream (bf16 or f32 [T, H]): the norm before it (``pre_gain``), router and
+    experts as ``moe_layer_step`` (their f32 sums, not rounded in between), then the norm after it with gate, scales and
+    residual sum, and, with ``next_gain``, the norm before the next block.  Returns ``(r', x)`` as ``block_norm``, whose
+    arguments the others are; ``out="int8"`` gives x as int8 rows for the next layer's ``int8_linear``."""
+    _, hidden = block_norm(residual, pre_gain=pre_gain, eps=eps)
+    y = moe_layer_step(hidden, router_w, state, bias=bias, mode=mode, multiplier=multiplier, out_f32=True, own_tokens=own_tokens)
+    return block_norm(residual, y, post_gain=post_gain, gate=gate, gate_sigmoid=gate_sigmoid, residual_scale=residual_scale,
+                      block_scale=block_scale, pre_gain=next_gain, eps=eps, out=out, residual_out=residual_out)
 
 
 def moe_step(hidden_states: torch.Tensor, router_logits: torch.Tensor, state: dict, *, out_f32: bool = False,
