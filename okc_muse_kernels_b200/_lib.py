@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 # OKC_MOE_LIB selects another build of the same ABI (the instrumented libokc_moe_b200_prof.so)
@@ -58,12 +59,18 @@ class BlockNormArgs(C.Structure):
                [(n, C.c_float) for n in ("residual_scale", "block_scale", "eps")]
 
 
+# The same structs as bytes: filling a ctypes Structure costs more than the rest of a call.
+pack_block_norm = struct.Struct("8P6q7i3f").pack
+
+
 class Int8Args(C.Structure):
     """okc_int8_args"""
     _fields_ = [(n, C.c_void_p) for n in ("x", "x_scale", "w", "w_scale", "bias", "out", "scratch")] + \
                [(n, C.c_int64) for n in ("x_stride", "w_stride", "out_stride")] + \
                [(n, C.c_int32) for n in ("x_kind", "out_f32", "tokens", "k", "n")]
 
+
+pack_int8 = struct.Struct("7P3q5i4x").pack
 
 _P = C.c_void_p
 _PLAN = C.POINTER(Plan)
@@ -94,11 +101,11 @@ SIGNATURES = {
     "okc_moe_unpack_bf16": (C.c_int, [_PLAN, _P, C.c_int, C.c_int, _P, _P]),
     "okc_moe_probe_wait_timeout": (C.c_int, [_P, _P]),
     "okc_moe_read_status": (C.c_int, [_P, _P, C.POINTER(C.c_int32)]),
-    "okc_moe_block_norm": (C.c_int, [C.POINTER(BlockNormArgs), _P]),
+    "okc_moe_block_norm": (C.c_int, [_P, _P]),     # okc_block_norm_args as bytes or byref
     "okc_moe_quantize_rows": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, _P, _P]),
     "okc_moe_int8_scratch_bytes": (C.c_uint64, [C.c_int, C.c_int32, C.c_int32]),
-    "okc_moe_int8_linear": (C.c_int, [C.POINTER(Int8Args), _P]),
-    "okc_moe_int8_gated": (C.c_int, [C.POINTER(Int8Args), _P]),
+    "okc_moe_int8_linear": (C.c_int, [_P, _P]),
+    "okc_moe_int8_gated": (C.c_int, [_P, _P]),
     "okc_moe_int8_status": (C.c_int, [_P, C.POINTER(C.c_int32)]),
     "okc_ep_buffer_bytes": (C.c_uint64, [C.c_int32, C.c_int32, C.c_int32]),
     "okc_ep_views": (C.c_int, [_COMM, C.POINTER(_P), C.POINTER(_P), C.POINTER(_P)]),

@@ -189,20 +189,40 @@ cudaError_t launch_int8_few(const Int8Params& p, bool gated, cudaStream_t stream
 __device__ __forceinline__ uint32_t idesc_i8(uint32_t m, uint32_t n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
-__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// The shared-memory descriptors come as halves: only the low ones, which hold the addresses, change.
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 ad, bd;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 ad, {%1, %3};\n\t"
+      "mov.b64 bd, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], ad, bd, %4, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 ad, bd;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 ad, {%1, %3};\n\t"
+      "mov.b64 bd, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], ad, bd, %4, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Low half of smem_desc_sw128 (ptx.cuh), and its high half, which is the same for every address.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr) { return ((saddr & 0x3FFFF) >> 4) | (1u << 16); }
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// 32 consecutive 32-bit columns of this thread's lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
       : "memory");
 }
 __device__ __forceinline__ void store_out(const Int8Params& p, int64_t o, float v) {
@@ -211,7 +231,7 @@ __device__ __forceinline__ void store_out(const Int8Params& p, int64_t o, float 
 }
 
 // ------------------------------------------------------------------ some hundred tokens
-constexpr int kMidThreads = 192;       // warps 0..3 epilogue, 4 TMA producer, 5 MMA issuer
+constexpr int kMidThreads = 256;       // warps 0..3 read the accumulator, 4 TMA producer, 5 MMA issuer; all finish the rows
 constexpr int kMidMaxStages = 8;
 constexpr int kKb = 128;               // K elements of a stage: one 128-byte swizzled row
 constexpr int kTileW = 128;            // weight rows of a tile
@@ -220,24 +240,28 @@ struct Int8MidParams {
   CUtensorMap wmap;      // int8 weight rows, box 128 x 128 rows (64 for the gated product: a gate and an up box)
   CUtensorMap xmap;      // int8 token rows, box 128 x tn
   Int8Params p;
-  int tn, stages, n_kb, splits, tmem_cols;
+  int tn, stages, n_kb, tmem_cols;
 };
 
-template <bool kGated>
+// The producer and the issuer run as whole warps with one elected lane acting: in code that only one thread runs, every
+// MMA costs it about 100 cycles (its operands go through vector registers), which with four MMAs and a commit a stage was
+// more than the stage's copy takes (K = 4096, N = 4096, 16 tokens, no split: 20.0 us).
+template <bool kGated, int kSplits>
 __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constant__ Int8MidParams q) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = smem_u32(smem_raw);
   const uint32_t smem0 = (smem_base + 1023u) & ~1023u;
   __shared__ uint64_t bar_full[kMidMaxStages], bar_empty[kMidMaxStages], bar_done;
+  __shared__ float xs[256];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_code;
   const Int8Params& p = q.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = blockIdx.x % q.splits, tile = blockIdx.x / q.splits;
+  const int rank = blockIdx.x % kSplits, tile = blockIdx.x / kSplits;
   const int w0 = tile * (kGated ? kTileW / 2 : kTileW);      // first output of the tile
   const int t0 = blockIdx.y * q.tn;
-  const int kb0 = static_cast<int>(static_cast<long long>(q.n_kb) * rank / q.splits);
-  const int nkb = static_cast<int>(static_cast<long long>(q.n_kb) * (rank + 1) / q.splits) - kb0;
+  const int kb0 = static_cast<int>(static_cast<long long>(q.n_kb) * rank / kSplits);
+  const int nkb = static_cast<int>(static_cast<long long>(q.n_kb) * (rank + 1) / kSplits) - kb0;
   const uint32_t stage_bytes = kTileW * kKb + static_cast<uint32_t>(q.tn) * kKb;
 
   if (tid == 0) {
@@ -254,109 +278,131 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
+  const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
+  cg::cluster_group cluster = cg::this_cluster();
+  int* const part = reinterpret_cast<int*>(smem_raw + (smem0 - smem_base));
+  // a thread finishes four neighbouring outputs of every few tokens
+  constexpr int kQuads = kGated ? kTileW / 8 : kTileW / 4;
+  const int o4 = (tid % kQuads) * 4, n = w0 + o4;
+  float sw[4], su[4] = {}, sb[4] = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool in = n + j < p.N;
+    sw[j] = in ? __ldg(p.w_scale + n + j) : 0.f;
+    if (kGated) su[j] = in ? __ldg(p.w_scale + p.N + n + j) : 0.f;
+    else if (p.bias) sb[j] = in ? __ldg(p.bias + n + j) : 0.f;
+  }
 
   if (warp == 4) {
-    if (lane == 0) {
-      auto load_w = [&](int i) {
-        const uint32_t bar = smem_u32(&bar_full[i % q.stages]), dst = smem0 + (i % q.stages) * stage_bytes;
+    auto load_w = [&](int i, uint32_t st) {
+      const uint32_t bar = full0 + 8 * st, dst = smem0 + st * stage_bytes;
+      if (elect_one()) {
         mbar_expect_tx(bar, stage_bytes);
         tma_2d_g2s(dst, &q.wmap, (kb0 + i) * kKb, w0, bar);
         if (kGated) tma_2d_g2s(dst + kTileW / 2 * kKb, &q.wmap, (kb0 + i) * kKb, p.N + w0, bar);
-      };
-      auto load_x = [&](int i) {
-        const uint32_t bar = smem_u32(&bar_full[i % q.stages]), dst = smem0 + (i % q.stages) * stage_bytes;
-        tma_2d_g2s(dst + kTileW * kKb, &q.xmap, (kb0 + i) * kKb, t0, bar);
-      };
-      // the weights of the first stages do not depend on the kernel before this one, the token rows may
-      const int first = min(nkb, q.stages);
-      for (int i = 0; i < first; ++i) load_w(i);
-      griddep_wait();
-      for (int i = 0; i < first; ++i) load_x(i);
-      int i = first;
-      for (; i < nkb; ++i) {
-        if (!mbar_wait(smem_u32(&bar_empty[i % q.stages]), ((i / q.stages) & 1) ^ 1, &abort_code, 0x61)) break;
-        load_w(i);
-        load_x(i);
       }
-      if (i < nkb) {
-        // give the copies in flight a bounded chance to land before the CTA retires
-        for (int j = max(0, i - q.stages); j < i; ++j) {
-          const long long c0 = clock64();
-          while (!mbar_try(smem_u32(&bar_full[j % q.stages]), (j / q.stages) & 1) && clock64() - c0 < kWaitLimitCycles) {}
-        }
-      }
+    };
+    auto load_x = [&](int i, uint32_t st) {
+      if (elect_one()) tma_2d_g2s(smem0 + st * stage_bytes + kTileW * kKb, &q.xmap, (kb0 + i) * kKb, t0, full0 + 8 * st);
+    };
+    // the weights of the first stages do not depend on the kernel before this one, the token rows may
+    const int first = min(nkb, q.stages);
+    for (int i = 0; i < first; ++i) load_w(i, i);
+    griddep_wait();
+    for (int i = 0; i < first; ++i) load_x(i, i);
+    int i = first;
+    uint32_t st = 0, ph = 0;
+    for (; i < nkb; ++i) {
+      if (!mbar_wait(empty0 + 8 * st, ph, &abort_code, 0x61)) break;
+      load_w(i, st);
+      load_x(i, st);
+      if (++st == static_cast<uint32_t>(q.stages)) { st = 0; ph ^= 1; }
+    }
+    if (i < nkb) {
+      // giving up: the copies in flight get a bounded chance to land before the CTA retires
+      const long long c0 = clock64();
+      for (int j = max(0, i - q.stages); j < i; ++j)
+        while (!mbar_try(full0 + 8 * (j % q.stages), (j / q.stages) & 1) && clock64() - c0 < kWaitLimitCycles) {}
     }
     __syncwarp();
   } else if (warp == 5) {
-    if (lane == 0) {
-      const uint32_t idesc = idesc_i8(128, static_cast<uint32_t>(q.tn));
-      bool ok = true;
-      for (int i = 0; i < nkb; ++i) {
-        ok = mbar_wait(smem_u32(&bar_full[i % q.stages]), (i / q.stages) & 1, &abort_code, 0x62);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t a = smem0 + (i % q.stages) * stage_bytes;
-        const uint64_t ad = smem_desc_sw128(a), bd = smem_desc_sw128(a + kTileW * kKb);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) mma_i8(tmem, ad + 2 * ks, bd + 2 * ks, idesc, (i | ks) != 0 ? 1u : 0u);   // K = 32 each
-        mma_commit(smem_u32(&bar_empty[i % q.stages]));
+    const uint32_t idesc = idesc_i8(128, static_cast<uint32_t>(q.tn));
+    const uint32_t lo0 = desc_lo(smem0);
+    uint32_t st = 0, ph = 0;
+    for (int i = 0; i < nkb; ++i) {
+      if (!mbar_wait(full0 + 8 * st, ph, &abort_code, 0x62)) break;
+      tc_fence_after();
+      const uint32_t a = lo0 + st * (stage_bytes >> 4), b = a + (kTileW * kKb >> 4);
+      if (elect_one()) {
+        mma_i8(tmem, a, b, kDescHi, idesc, i != 0);          // K = 32 each: 32 bytes further along the swizzled rows
+        mma_i8(tmem, a + 2, b + 2, kDescHi, idesc, 1);
+        mma_i8(tmem, a + 4, b + 4, kDescHi, idesc, 1);
+        mma_i8(tmem, a + 6, b + 6, kDescHi, idesc, 1);
+        mma_commit(empty0 + 8 * st);
       }
-      mma_commit(smem_u32(&bar_done));
+      if (++st == static_cast<uint32_t>(q.stages)) { st = 0; ph ^= 1; }
     }
+    if (elect_one()) mma_commit(smem_u32(&bar_done));
     __syncwarp();
-  } else {
+  } else if (warp < 4) {
     griddep_wait();        // the token scales come from the kernel before this one
-    const bool ok = mbar_wait<40>(smem_u32(&bar_done), 0, &abort_code, 0x63);
+    for (int i = tid; i < q.tn; i += 128) xs[i] = t0 + i < p.T ? p.x_scale[t0 + i] : 0.f;
+    const bool ok = mbar_wait<20>(smem_u32(&bar_done), 0, &abort_code, 0x63);
     tc_fence_after();
     if (ok) {
       // this CTA's sums, [token][weight row], over the ring slots (every copy has landed and every MMA has read them)
       const uint32_t taddr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-      int* part = reinterpret_cast<int*>(smem_raw + (smem0 - smem_base));
-      for (int c0 = 0; c0 < q.tn; c0 += 16) {
+      int* mine = part + warp * 32 + lane;
+      int c0 = 0;
+      for (; c0 + 32 <= q.tn; c0 += 32) {
+        uint32_t r[32];
+        tmem_ld32(taddr + c0, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) mine[(c0 + j) * kTileW] = static_cast<int>(r[j]);
+      }
+      if (c0 < q.tn) {
         uint32_t r[16];
         tmem_ld16(taddr + c0, r);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c0 + j) * kTileW + warp * 32 + lane] = static_cast<int>(r[j]);
+        for (int j = 0; j < 16; ++j) mine[(c0 + j) * kTileW] = static_cast<int>(r[j]);
       }
     }
     tc_fence_before();
   }
-  cg::cluster_group cluster = cg::this_cluster();
-  if (q.splits > 1) cluster.sync(); else __syncthreads();
+  if (kSplits > 1) cluster.sync(); else __syncthreads();
 
-  // Each CTA of the cluster finishes tn / splits tokens: it adds the integer sums of all CTAs and stores the rows.
-  if (warp < 4) {
-    const int per = q.tn / q.splits;
-    int* part = reinterpret_cast<int*>(smem_raw + (smem0 - smem_base));
-    const int quads = kGated ? kTileW / 8 : kTileW / 4;
-    for (int i = tid; i < per * quads; i += 128) {
-      const int col = rank * per + i / quads, o4 = (i % quads) * 4, t = t0 + col;
-      if (t >= p.T) break;
-      int4 a = make_int4(0, 0, 0, 0), b = a;
-      for (int s = 0; s < q.splits; ++s) {
-        const int* src = q.splits > 1 ? cluster.map_shared_rank(part, s) : part;
-        const int4 v = *reinterpret_cast<const int4*>(src + col * kTileW + o4);
-        a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-        if (kGated) {
-          const int4 u = *reinterpret_cast<const int4*>(src + col * kTileW + kTileW / 2 + o4);
-          b.x += u.x; b.y += u.y; b.z += u.z; b.w += u.w;
-        }
+  // Each CTA of the cluster finishes tn / kSplits tokens: it adds the integer sums of all CTAs (the loads from all of them
+  // under way at once) and stores the rows.
+  {
+    const int* src[kSplits];
+#pragma unroll
+    for (int s = 0; s < kSplits; ++s) src[s] = (kSplits > 1 ? cluster.map_shared_rank(part, s) : part) + o4;
+    const int per = q.tn / kSplits, last = min((rank + 1) * per, p.T - t0);
+#pragma unroll 2
+    for (int col = rank * per + tid / kQuads; col < last; col += kMidThreads / kQuads) {
+      int4 a[kSplits], b[kSplits];
+#pragma unroll
+      for (int s = 0; s < kSplits; ++s) {
+        a[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW);
+        if (kGated) b[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW + kTileW / 2);
       }
-      const float sx = p.x_scale[t];
-      const int av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
-      const int n = w0 + o4;
+#pragma unroll
+      for (int s = 1; s < kSplits; ++s) {
+        a[0].x += a[s].x; a[0].y += a[s].y; a[0].z += a[s].z; a[0].w += a[s].w;
+        if (kGated) { b[0].x += b[s].x; b[0].y += b[s].y; b[0].z += b[s].z; b[0].w += b[s].w; }
+      }
+      const float sx = xs[col];
+      const int av[4] = {a[0].x, a[0].y, a[0].z, a[0].w}, bv[4] = {b[0].x, b[0].y, b[0].z, b[0].w};
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        v[j] = 0.f;
-        if (n + j < p.N) {
-          v[j] = int8_value(av[j], sx, p.w_scale[n + j]);
-          if (kGated) v[j] = silu_mul(v[j], int8_value(bv[j], sx, p.w_scale[p.N + n + j]));
-          else if (p.bias) v[j] = __fadd_rn(v[j], p.bias[n + j]);
-        }
+        v[j] = int8_value(av[j], sx, sw[j]);
+        if (kGated) v[j] = silu_mul(v[j], int8_value(bv[j], sx, su[j]));
+        else if (p.bias) v[j] = __fadd_rn(v[j], sb[j]);
       }
-      const int64_t o = t * p.out_stride + n;
+      const int64_t o = static_cast<int64_t>(t0 + col) * p.out_stride + n;
       if (p.out_vec && n + 4 <= p.N) {
         if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = make_float4(v[0], v[1], v[2], v[3]);
         else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
@@ -367,7 +413,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
       }
     }
   }
-  if (q.splits > 1) cluster.sync(); else __syncthreads();   // no CTA leaves while another reads its sums
+  if (kSplits > 1) cluster.sync(); else __syncthreads();   // no CTA leaves while another reads its sums
   if (warp == 4) {
     tc_fence_after();
     tmem_dealloc(tmem, static_cast<uint32_t>(q.tmem_cols));
@@ -385,11 +431,12 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStrea
   const int ttiles = (p.T + 255) / 256;
   q.tn = ((p.T + ttiles - 1) / ttiles + 15) & ~15;
   q.n_kb = (p.K + kKb - 1) / kKb;
-  q.splits = 1;
-  while (q.splits < 8 && 2 * q.splits <= q.n_kb && 2LL * q.splits * tiles * ttiles <= 2 * 148) q.splits *= 2;
+  // As many CTAs a cluster as one round of them fits the SMs.  K = 4096, N = 4096, 16 tokens (32 tiles), 1 / 2 / 4 / 8 CTAs
+  // a cluster: 10.5 / 7.8 / 6.6 / 13.9 us; gated, K = 7168, 2 x 2048 rows, 128 tokens: 18.4 / 12.9 / 10.6 / 26.0 us.
+  int splits = 1;
+  while (splits < 8 && 2 * splits <= q.n_kb && 2LL * splits * tiles * ttiles <= 148) splits *= 2;
   const int stage = kTileW * kKb + q.tn * kKb;
-  const int budget = q.tn <= 64 ? 108 * 1024 : 216 * 1024;
-  q.stages = budget / stage;
+  q.stages = 216 * 1024 / stage;
   if (q.stages > kMidMaxStages) q.stages = kMidMaxStages;
   q.tmem_cols = tmem_cols_for(q.tn);
   if (!encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(gated ? 2 : 1) * p.N, p.K, p.w_stride, per_tile) ||
@@ -398,18 +445,19 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStrea
   size_t smem = 1024 + static_cast<size_t>(q.stages) * stage;
   const size_t sums = 1024 + static_cast<size_t>(q.tn) * kTileW * 4;
   if (smem < sums) smem = sums;
-  auto kernel = gated ? okc_int8_mid<true> : okc_int8_mid<false>;
+  auto kernel = gated ? (splits == 1 ? okc_int8_mid<true, 1> : splits == 2 ? okc_int8_mid<true, 2> : splits == 4 ? okc_int8_mid<true, 4> : okc_int8_mid<true, 8>)
+                      : (splits == 1 ? okc_int8_mid<false, 1> : splits == 2 ? okc_int8_mid<false, 2> : splits == 4 ? okc_int8_mid<false, 4> : okc_int8_mid<false, 8>);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * q.splits, ttiles);
+  cfg.gridDim = dim3(tiles * splits, ttiles);
   cfg.blockDim = dim3(kMidThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;
   attr[n].id = cudaLaunchAttributeClusterDimension;
-  attr[n].val.clusterDim.x = q.splits; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
+  attr[n].val.clusterDim.x = splits; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
   ++n;
   if (pdl) {
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -425,14 +473,16 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStrea
 constexpr int kManyThreads = 256;      // warps 0 TMA producer, 1 MMA issuer (leader CTA), 2 TMEM, 4..7 epilogue
 constexpr int kManyStages = 6;
 constexpr int kManyStageBytes = 2 * 128 * kKb;
-constexpr int kManySmem = 1024 + kManyStages * kManyStageBytes;
+constexpr int kManyStore = 4096;       // staging of an epilogue warp: 32 rows x 32 results
+constexpr int kManySmem = 1024 + kManyStages * kManyStageBytes + 4 * kManyStore;
 
 struct Int8ManyParams {
   CUtensorMap xmap;      // int8 token rows, box 128 x 128 rows
   CUtensorMap wmap;      // int8 weight rows, box 128 x bn / 2 rows
+  CUtensorMap omap;      // output rows, box 32 columns x 32 rows (only with tma_out)
   Int8Params p;
-  int bn;                // weight rows of a pair's tile (columns of its accumulator): a multiple of 32, at most 256
-  int n_kb, tiles_t, tiles_n;
+  int bn;                // weight rows of a pair's tile (columns of its accumulator): a multiple of 32 (gated: 64), at most 256
+  int n_kb, tiles_t, tiles_n, tma_out;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -490,11 +540,21 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
       : "memory");
 }
 
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// 2-D tiled tensor store shared -> global; elements outside the tensor are not written.
+__device__ __forceinline__ void tma_2d_s2g(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(src)
+               : "memory");
+}
+
 template <bool kGated>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_int8_many(const __grid_constant__ Int8ManyParams q) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   __shared__ uint64_t bar_full[kManyStages], bar_empty[kManyStages], bar_acc_full[2], bar_acc_empty[2];
+  __shared__ __align__(16) float scale_s[2][256], bias_s[2][256];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_code;
   const Int8Params& p = q.p;
@@ -519,113 +579,158 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
   const uint32_t tmem = tmem_base_s;
 
   if (warp == 0) {
-    if (lane == 0) {
-      griddep_wait();
-      const uint32_t half_bytes = 128u * kKb + static_cast<uint32_t>(q.bn / 2) * kKb;
-      int it = 0;
-      bool ok = true;
-      for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        const int tt = tile % q.tiles_t, tw = tile / q.tiles_t;
-        const int xrow = tt * 256 + static_cast<int>(rank) * 128;
-        const int wrow = kGated ? static_cast<int>(rank) * p.N + tw * (q.bn / 2) : tw * q.bn + static_cast<int>(rank) * (q.bn / 2);
-        for (int kb = 0; kb < q.n_kb; ++kb, ++it) {
-          const int s = it % kManyStages;
-          if (it >= kManyStages && !pair_wait(smem_u32(&bar_empty[s]), ((it / kManyStages) & 1) ^ 1, &abort_code, 0x71)) { ok = false; break; }
-          // the bytes of both CTAs count on the leader's barrier
-          const uint32_t bar = map_rank(smem_u32(&bar_full[s]), 0);
-          if (rank == 0) mbar_expect_tx(smem_u32(&bar_full[s]), 2 * half_bytes);
-          const uint32_t dst = smem0 + s * kManyStageBytes;
+    griddep_wait();
+    const uint32_t half_bytes = 128u * kKb + static_cast<uint32_t>(q.bn / 2) * kKb;
+    const uint32_t full0 = map_rank(smem_u32(&bar_full[0]), 0);      // the bytes of both CTAs count on the leader's barriers
+    const uint32_t empty0 = smem_u32(&bar_empty[0]);
+    uint32_t st = 0, ph = 1;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += pairs) {
+      const int tt = tile % q.tiles_t, tw = tile / q.tiles_t;
+      const int xrow = tt * 256 + static_cast<int>(rank) * 128;
+      const int wrow = kGated ? static_cast<int>(rank) * p.N + tw * (q.bn / 2) : tw * q.bn + static_cast<int>(rank) * (q.bn / 2);
+      for (int kb = 0; kb < q.n_kb; ++kb) {
+        ok = pair_wait(empty0 + 8 * st, ph, &abort_code, 0x71);      // (the first round finds the slots empty)
+        if (!ok) break;
+        const uint32_t bar = full0 + 8 * st, dst = smem0 + st * kManyStageBytes;
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(smem_u32(&bar_full[st]), 2 * half_bytes);
           tma_2d_pair(dst, &q.xmap, kb * kKb, xrow, bar);
           tma_2d_pair(dst + 128 * kKb, &q.wmap, kb * kKb, wrow, bar);
         }
+        if (++st == kManyStages) { st = 0; ph ^= 1; }
       }
-      // The copies still in flight have landed once the MMA issuer has seen them; it waits for all of them unless it
-      // gave up, and then they get a bounded time here.
-      if (!ok) {
-        const long long c0 = clock64();
-        while (clock64() - c0 < kWaitLimitCycles / 100) {}
-      }
+    }
+    // Every copy has landed once the epilogue has seen the last tile; a producer that gave up leaves them some time.
+    if (!ok) {
+      const long long c0 = clock64();
+      while (clock64() - c0 < kWaitLimitCycles / 100) {}
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint32_t idesc = idesc_i8(256, static_cast<uint32_t>(q.bn));
-      int it = 0, n = 0;
+      const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]), lo0 = desc_lo(smem0);
+      uint32_t st = 0, ph = 0, buf = 0, bph = 1;
       bool ok = true;
-      for (int tile = pair; tile < tiles && ok; tile += pairs, ++n) {
-        const int buf = n & 1;
-        if (n >= 2 && !pair_wait(smem_u32(&bar_acc_empty[buf]), ((n >> 1) & 1) ^ 1, &abort_code, 0x72)) break;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        ok = pair_wait(smem_u32(&bar_acc_empty[buf]), bph, &abort_code, 0x72);     // (the first two tiles find it empty)
         tc_fence_after();
         const uint32_t d = tmem + buf * 256;
-        for (int kb = 0; kb < q.n_kb; ++kb, ++it) {
-          const int s = it % kManyStages;
-          ok = pair_wait(smem_u32(&bar_full[s]), (it / kManyStages) & 1, &abort_code, 0x73);
+        for (int kb = 0; ok && kb < q.n_kb; ++kb) {
+          ok = pair_wait(full0 + 8 * st, ph, &abort_code, 0x73);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t a = smem0 + s * kManyStageBytes;
-          const uint64_t ad = smem_desc_sw128(a), bd = smem_desc_sw128(a + 128 * kKb);
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) mma_i8_pair(d, ad + 2 * ks, bd + 2 * ks, idesc, (kb | ks) != 0 ? 1u : 0u);
-          mma_commit_pair(smem_u32(&bar_empty[s]));
+          const uint32_t a = lo0 + st * (kManyStageBytes >> 4), b = a + (128 * kKb >> 4);
+          if (elect_one()) {
+            mma_i8_pair(d, a, b, kDescHi, idesc, kb != 0);
+            mma_i8_pair(d, a + 2, b + 2, kDescHi, idesc, 1);
+            mma_i8_pair(d, a + 4, b + 4, kDescHi, idesc, 1);
+            mma_i8_pair(d, a + 6, b + 6, kDescHi, idesc, 1);
+            mma_commit_pair(empty0 + 8 * st);
+          }
+          if (++st == kManyStages) { st = 0; ph ^= 1; }
         }
-        if (ok) mma_commit_pair(smem_u32(&bar_acc_full[buf]));
+        if (ok && elect_one()) mma_commit_pair(smem_u32(&bar_acc_full[buf]));
+        buf ^= 1;
+        if (buf == 0) bph ^= 1;
       }
     }
     __syncwarp();
   } else if (warp >= 4) {
     griddep_wait();        // the token scales come from the kernel before this one
-    const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const int half = q.bn / 2;
+    const int ew = warp & 3, half = q.bn / 2;
+    const int width = kGated ? half : q.bn;        // outputs of a tile
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(ew * 32) << 16);
+    const uint32_t stage = smem0 + kManyStages * kManyStageBytes + ew * kManyStore;
     int n = 0;
+    bool ok = true;
     for (int tile = pair; tile < tiles; tile += pairs, ++n) {
       const int buf = n & 1;
-      if (!pair_wait(smem_u32(&bar_acc_full[buf]), (n >> 1) & 1, &abort_code, 0x74)) break;
-      tc_fence_after();
       const int tt = tile % q.tiles_t, tw = tile / q.tiles_t;
-      const int t = tt * 256 + static_cast<int>(rank) * 128 + (warp & 3) * 32 + lane;
+      const int row0 = tt * 256 + static_cast<int>(rank) * 128 + ew * 32, t = row0 + lane;
       const float sx = t < p.T ? p.x_scale[t] : 0.f;
-      const int width = kGated ? half : q.bn;        // outputs of the tile
-      for (int c0 = 0; c0 < width; c0 += 16) {
-        uint32_t r[16], u[16];
-        tmem_ld16(taddr + buf * 256 + c0, r);
-        if (kGated) tmem_ld16(taddr + buf * 256 + half + c0, u);
-        tmem_wait_ld();
-        const int n0 = tw * width + c0;
-        const bool live = t < p.T;
-        float v[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          v[j] = 0.f;
-          if (n0 + j < p.N) {
-            v[j] = int8_value(static_cast<int>(r[j]), sx, __ldg(p.w_scale + n0 + j));
-            if (kGated) v[j] = silu_mul(v[j], int8_value(static_cast<int>(u[j]), sx, __ldg(p.w_scale + p.N + n0 + j)));
-            else if (p.bias) v[j] = __fadd_rn(v[j], __ldg(p.bias + n0 + j));
-          }
-        }
-        const int64_t o = t * p.out_stride + n0;
-        if (live && p.out_vec && n0 + 16 <= p.N) {
-          if (p.out_f32) {
-            float4* d = reinterpret_cast<float4*>(static_cast<float*>(p.out) + o);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          } else {
-            uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              d[j] = make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                                pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-          }
-        } else if (live) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (n0 + j < p.N) store_out(p, o + j, v[j]);
-        }
-        __syncwarp();      // the next load from tensor memory is one of the whole warp
+      // the tile's weight scales (and bias) once into shared memory; by the next write to this half of the array every
+      // warp has passed the barrier of the tile between, so it has finished reading
+      for (int c = tid - 128; c < q.bn; c += 128) {
+        const int o = tw * width + (kGated && c >= half ? c - half : c);
+        const bool in = o < p.N;
+        scale_s[buf][c] = in ? __ldg(p.w_scale + (kGated && c >= half ? p.N + o : o)) : 0.f;
+        if (!kGated && p.bias) bias_s[buf][c] = in ? __ldg(p.bias + o) : 0.f;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&bar_acc_empty[buf]), 0));
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // (a warp that gives up goes on to meet the others at the barrier of each tile)
+      ok = ok && pair_wait(smem_u32(&bar_acc_full[buf]), (n >> 1) & 1, &abort_code, 0x74);
+      tc_fence_after();
+      for (int c0 = 0; ok && c0 < width; c0 += 32) {
+        uint32_t r[32], u[32];
+        tmem_ld32(taddr + buf * 256 + c0, r);
+        if (kGated) tmem_ld32(taddr + buf * 256 + half + c0, u);
+        tmem_wait_ld();
+        if (c0 + 32 >= width) {       // the accumulator has been read: the pair's next tile but one may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&bar_acc_empty[buf]), 0));
+        }
+        const float* ws = scale_s[buf] + c0;
+        const float* bs = bias_s[buf] + c0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          float v = int8_value(static_cast<int>(r[j]), sx, ws[j]);
+          if (kGated) v = silu_mul(v, int8_value(static_cast<int>(u[j]), sx, ws[half + j]));
+          else if (p.bias) v = __fadd_rn(v, bs[j]);
+          r[j] = __float_as_uint(v);
+        }
+        // A thread has 32 neighbouring results of its own row; they leave through shared memory so that whole pieces of
+        // rows are written: by one TMA store a warp, or, for rows it cannot address, 32 columns a warp store.
+        const int col = tw * width + c0;
+        const uint32_t at = stage + (p.out_f32 ? 0u : static_cast<uint32_t>((c0 >> 5) & 1) * 2048u);
+        if (lane == 0) {
+          if (p.out_f32) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        }
+        __syncwarp();
+        if (p.out_f32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            st_shared_v4(at + lane * 128 + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
+            st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
+          }
+        }
+        if (q.tma_out) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < p.T && col < p.N) tma_2d_s2g(&q.omap, at, col, row0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          __syncwarp();
+          if (col + lane < p.N)
+            for (int i = 0; i < 32 && row0 + i < p.T; ++i) {
+              const int64_t o = static_cast<int64_t>(row0 + i) * p.out_stride + col + lane;
+              if (p.out_f32) {
+                uint32_t v;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4));
+                static_cast<float*>(p.out)[o] = __uint_as_float(v);
+              } else {
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at + i * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2));
+                static_cast<uint16_t*>(p.out)[o] = v;
+              }
+            }
+          __syncwarp();
+        }
+      }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
   tc_fence_before();
   cg::this_cluster().sync();     // no CTA frees its tensor memory or leaves while the pair's MMAs and arrivals may touch it
@@ -647,7 +752,7 @@ cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStre
   // The tile width that leaves the least work in the last round of the 74 pairs.
   q.bn = 256;
   long long best = -1;
-  for (int bn = 256; bn >= 128; bn -= 32) {
+  for (int bn = 256; bn >= 128; bn -= gated ? 64 : 32) {
     const long long tn = (cols + bn - 1) / bn;
     const long long cost = ((tn * q.tiles_t + 73) / 74) * (bn + 16);
     if (best < 0 || cost < best) { best = cost; q.bn = bn; q.tiles_n = static_cast<int>(tn); }
@@ -656,6 +761,8 @@ cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStre
   if (!encode_bytes_map(&q.xmap, p.x, p.T, p.K, p.x_stride, 128) ||
       !encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(cols), p.K, p.w_stride, q.bn / 2))
     return cudaErrorInvalidValue;
+  q.tma_out = p.out_vec;
+  if (q.tma_out && !encode_out_map(&q.omap, p.out, p.T, p.N, p.out_stride, p.out_f32 != 0)) return cudaErrorInvalidValue;
   const long long tiles = static_cast<long long>(q.tiles_t) * q.tiles_n;
   const int grid = static_cast<int>(tiles < 74 ? 2 * tiles : 148);
   auto kernel = gated ? okc_int8_many<true> : okc_int8_many<false>;

@@ -17,14 +17,15 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from ._lib import BlockNormArgs, Int8Args
 
 __all__ = ["QuantRows", "quantize_rows", "int8_rows", "int8_linear", "int8_gated", "int8_ffn", "block_norm", "int8_status"]
 
 BLOCK_NORM_MAX_HIDDEN = 16384
 INT8_MAX_K = 131071           # the integer sums stay in 32 bits
-_ROWS_KIND = {torch.bfloat16: 0, torch.float32: 1, torch.int8: 2}
-_OUT = {"bf16": (0, torch.bfloat16), "f32": (1, torch.float32), "int8": (2, torch.int8)}
+INT8_FEW_TOKENS = 8           # up to here a product quantises its tokens itself and needs no scratch
+_BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
+_ROWS_KIND = {_BF16: 0, _F32: 1, _I8: 2}
+_OUT = {"bf16": (0, _BF16), "f32": (1, _F32), "int8": (2, _I8)}
 
 
 class QuantRows(NamedTuple):
@@ -34,41 +35,52 @@ class QuantRows(NamedTuple):
     scale: torch.Tensor
 
 
-def _device(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    if not first.is_cuda:
+# A decode step makes these calls by the hundred and its kernels take a few microseconds, so the checks below are written
+# to cost little: each property is read once, and what can be compared as an integer is.
+def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The index of the CUDA device that all tensors are on."""
+    dev = first.get_device()
+    if dev < 0:
         raise ValueError("okc_muse_kernels_b200 runs on CUDA tensors only (there is no CPU path)")
-    dev = first.device
     for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}: all have to be on one device")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {first.device} and {t.device}: all have to be on one device")
     return dev
 
 
-def _call(fn, name: str, dev: torch.device, *args) -> None:
+_raw_stream = torch._C._cuda_getCurrentRawStream     # the current stream of a device as an integer
+
+
+def _call(fn, name: str, dev: int, *args) -> None:
     """The C entry on the tensors' device (made current for the call if it is not) and its current stream."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         _lib.check(rc, name)
 
 
-def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
-    if t.dim() != 2 or (t.dtype is not torch.bfloat16 and t.dtype is not torch.float32):
+def _rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]:
+    """bf16 or f32 rows with contiguous columns (a copy if need be): tensor, rows, columns, row stride."""
+    if t.dim() != 2 or (t.dtype is not _BF16 and t.dtype is not _F32):
         raise ValueError(f"{what} must be bf16 or f32 [rows, columns]")
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
+    R, cols = t.shape
+    stride, one = t.stride()
+    if one != 1 or stride < cols:
+        if R > 1 or (one != 1 and cols > 1):
+            t = t.contiguous()
+        stride = cols
+    return t, R, cols, stride
 
 
 def _vector(t: torch.Tensor | None, n: int, what: str) -> torch.Tensor | None:
     if t is None:
         return None
-    if t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != n:
+    if t.dtype is not _F32 or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{what} must be f32 [{n}]")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -82,23 +94,23 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def _out_rows(out: torch.Tensor | None, shape: tuple[int, int], dtype: torch.dtype, dev: torch.device, what: str, *inputs) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    if tuple(out.shape) != shape or out.dtype != dtype or out.device != dev:
-        raise ValueError(f"{what} must be {dtype} {list(shape)} on {dev}")
-    if (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1]):
+def _check_out(out: torch.Tensor, R: int, cols: int, dtype: torch.dtype, what: str, inputs) -> int:
+    """Checks a caller's output rows; returns their stride."""
+    if tuple(out.shape) != (R, cols) or out.dtype is not dtype:
+        raise ValueError(f"{what} must be {dtype} [{R}, {cols}]")
+    stride, one = out.stride()
+    if (cols > 1 and one != 1) or (R > 1 and stride < cols):
         raise ValueError(f"{what} needs contiguous columns and rows that do not overlap")
     for t in inputs:
         if t is not None and _overlap(out, t):
             raise ValueError(f"{what} overlaps an input")
-    return out
+    return max(stride, cols)
 
 
 # ------------------------------------------------------------------------------------------------ int8 rows
-def _empty_rows(rows: int, cols: int, dev: torch.device) -> torch.Tensor:
+def _empty_rows(like: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     pad = (cols + 15) // 16 * 16
-    q = torch.empty((rows, pad), dtype=torch.int8, device=dev)
+    q = like.new_empty((rows, pad), dtype=_I8)
     return q if pad == cols else q[:, :cols]
 
 
@@ -107,16 +119,15 @@ def quantize_rows(x: torch.Tensor) -> QuantRows:
     q = rint(x * (127 / a)), halves to even, quotients and product in f32.  A row whose a is below 2**-120 becomes zeros
     with scale 0; a row that holds an infinity or a NaN becomes zeros with scale NaN, so that it makes NaN of every product.
     Weights are quantised with the same call once, a row per output channel.  C <= 131071."""
-    x = _rows(x, "x")
-    R, cols = x.shape
+    x, R, cols, stride = _rows(x, "x")
     if cols < 1 or cols > INT8_MAX_K:
         raise ValueError(f"rows of 1 to {INT8_MAX_K} columns, got {cols}")
     dev = _device(x)
-    q = _empty_rows(R, cols, dev)
-    scale = torch.empty(R, dtype=torch.float32, device=dev)
+    q = _empty_rows(x, R, cols)
+    scale = x.new_empty(R, dtype=_F32)
     if R:
         _call(_lib.lib().okc_moe_quantize_rows, "okc_moe_quantize_rows", dev, x.data_ptr(), _ROWS_KIND[x.dtype],
-              max(x.stride(0), cols), R, cols, q.data_ptr(), max(q.stride(0), cols), scale.data_ptr())
+              stride, R, cols, q.data_ptr(), max(q.stride(0), cols), scale.data_ptr())
     return QuantRows(q, scale)
 
 
@@ -125,53 +136,55 @@ def int8_rows(q: torch.Tensor, scale: torch.Tensor) -> QuantRows:
     rows 16 bytes aligned.  Once, at load time."""
     if q.dtype is not torch.int8 or q.dim() != 2 or scale.dtype is not torch.float32 or scale.shape != q.shape[:1]:
         raise ValueError("int8_rows wants int8 [R, C] and f32 [R]")
-    dev = _device(q, scale)
-    rows = _empty_rows(q.shape[0], q.shape[1], dev)
+    _device(q, scale)
+    rows = _empty_rows(q, *q.shape)
     rows.copy_(q)
     return QuantRows(rows, scale.contiguous())
 
 
-def _check_quant(rows, what: str) -> tuple[torch.Tensor, torch.Tensor, int]:
-    """The int8 tensor, its scales and the row stride to pass on."""
+def _check_quant(rows, what: str) -> tuple[torch.Tensor, torch.Tensor, int, int, int]:
+    """int8 tensor, scales, rows, columns and the row stride to pass on."""
     q, scale = rows
-    if q.dtype is not torch.int8 or q.dim() != 2 or scale.dtype is not torch.float32 or scale.dim() != 1 or scale.shape[0] != q.shape[0]:
+    if q.dtype is not _I8 or q.dim() != 2 or scale.dtype is not _F32 or scale.dim() != 1 or scale.shape[0] != q.shape[0]:
         raise ValueError(f"{what} must be int8 [rows, columns] with f32 [rows] scales")
     R, cols = q.shape
-    stride = q.stride(0)
+    stride, one = q.stride()
     if R <= 1:
         stride = (cols + 15) // 16 * 16
-    if (cols > 1 and q.stride(1) != 1) or stride < cols or stride % 16 or q.data_ptr() % 16:
+    if (one != 1 and cols > 1) or stride < cols or stride % 16 or q.data_ptr() % 16:
         raise ValueError(f"{what} needs rows that start on 16-byte boundaries: lay them out with int8_rows() once")
-    return q, scale.contiguous(), stride
+    return q, scale if scale.is_contiguous() else scale.contiguous(), R, cols, stride
 
 
-def _product(fn, name: str, x, weight, bias, out_f32: bool, out, halves: int) -> torch.Tensor:
-    w, w_scale, w_stride = _check_quant(weight, "weight")
-    rows, K = w.shape
-    if rows < halves or rows % halves:
+def _product(name: str, x, weight, bias, out_f32: bool, out, halves: int) -> torch.Tensor:
+    w, w_scale, N, K, w_stride = _check_quant(weight, "weight")
+    if N < halves or N % halves:
         raise ValueError("a gated weight holds the gate rows and then as many up rows" if halves == 2 else "weight has no rows")
-    N = rows // halves
+    N //= halves
+    x_scale = None
     if isinstance(x, tuple):
-        xt, x_scale, x_stride = _check_quant(x, "x")
+        x, x_scale, T, cols, x_stride = _check_quant(x, "x")
     else:
-        xt, x_scale = _rows(x, "x"), None
-        x_stride = max(xt.stride(0), K)
-    T = xt.shape[0]
-    if xt.shape[1] != K or K < 1 or K > INT8_MAX_K:
-        raise ValueError(f"x has {xt.shape[1]} columns and weight {K}; 1 to {INT8_MAX_K}, and as many in both")
-    dev = _device(xt, x_scale, w, w_scale, bias, out)
+        x, T, cols, x_stride = _rows(x, "x")
+    if cols != K or K < 1 or K > INT8_MAX_K:
+        raise ValueError(f"x has {cols} columns and weight {K}; 1 to {INT8_MAX_K}, and as many in both")
+    dev = _device(x, x_scale, w, w_scale, bias, out)
     bias = _vector(bias, N, "bias")
-    out = _out_rows(out, (T, N), torch.float32 if out_f32 else torch.bfloat16, dev, "out", xt, x_scale, w, w_scale, bias)
+    dtype = _F32 if out_f32 else _BF16
+    if out is None:
+        out, out_stride = x.new_empty((T, N), dtype=dtype), N
+    else:
+        out_stride = _check_out(out, T, N, dtype, "out", (x, x_scale, w, w_scale, bias))
     if T == 0:
         return out
     lib = _lib.lib()
-    kind = _ROWS_KIND[xt.dtype]
-    n = lib.okc_moe_int8_scratch_bytes(kind, T, K)
-    scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _call(getattr(lib, fn), name, dev, Int8Args(
-        xt.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
-        None if bias is None else bias.data_ptr(), out.data_ptr(), None if scratch is None else scratch.data_ptr(),
-        x_stride, w_stride, max(out.stride(0), N), kind, int(out_f32), T, K, N))
+    scratch = None
+    if x_scale is None and T > INT8_FEW_TOKENS:
+        scratch = x.new_empty(lib.okc_moe_int8_scratch_bytes(0, T, K), dtype=_I8)
+    _call(getattr(lib, name), name, dev, _lib.pack_int8(
+        x.data_ptr(), 0 if x_scale is None else x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+        0 if bias is None else bias.data_ptr(), out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+        x_stride, w_stride, out_stride, _ROWS_KIND[x.dtype], out_f32, T, K, N))
     return out
 
 
@@ -183,7 +196,7 @@ def int8_linear(x, weight, *, bias: torch.Tensor | None = None, out_f32: bool = 
     y[t, n] = (sum_k x.q[t, k] * weight.q[n, k]) * (x.scale[t] * weight.scale[n]) + bias[n]; the sum is exact, the rest is
     f32 and rounded once, so a token's bits do not depend on the other tokens of the call.  T may be 0; K <= 131071.
     ``out``: a tensor to write, which may not overlap an input."""
-    return _product("okc_moe_int8_linear", "okc_moe_int8_linear", x, weight, bias, out_f32, out, 1)
+    return _product("okc_moe_int8_linear", x, weight, bias, out_f32, out, 1)
 
 
 def int8_gated(x, weight, *, out_f32: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -191,7 +204,7 @@ def int8_gated(x, weight, *, out_f32: bool = False, out: torch.Tensor | None = N
 
     ``weight``: int8 [2 I, K] and f32 [2 I], the gate rows first (the order of the experts' ``w13``).  Otherwise as
     ``int8_linear``."""
-    return _product("okc_moe_int8_gated", "okc_moe_int8_gated", x, weight, None, out_f32, out, 2)
+    return _product("okc_moe_int8_gated", x, weight, None, out_f32, out, 2)
 
 
 def int8_ffn(x, w13, w2, *, bias: torch.Tensor | None = None, out_f32: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -229,58 +242,67 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
         raise ValueError('out is "bf16", "f32" or "int8"')
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    res = _rows(residual, "residual")
-    T, H = res.shape
+    res, T, H, res_stride = _rows(residual, "residual")
     if H < 1 or H > BLOCK_NORM_MAX_HIDDEN:
         raise ValueError(f"rows of 1 to {BLOCK_NORM_MAX_HIDDEN} columns, got {H}")
     dev = _device(res, block, post_gain, gate, pre_gain, residual_out)
     post_gain, pre_gain = _vector(post_gain, H, "post_gain"), _vector(pre_gain, H, "pre_gain")
-    kind, gate_stride = 0, 0
+    dtype = res.dtype
+    kind = gate_stride = gate_f32 = blk_stride = new_stride = blk_ptr = blk_f32 = 0
     if block is None:
         if post_gain is not None or gate is not None or residual_out is not None or residual_scale != 1.0 or block_scale != 1.0:
             raise ValueError("post_gain, gate, residual_out and the scales belong to a block's output")
         if pre_gain is None:
             raise ValueError("nothing to do: neither block nor pre_gain is given")
-        new, blk = residual, None
+        new = residual
     else:
-        blk = _rows(block, "block")
-        if blk.shape != res.shape:
+        blk, rows, cols, blk_stride = _rows(block, "block")
+        if rows != T or cols != H:
             raise ValueError(f"block must be [{T}, {H}] like residual")
+        blk_ptr, blk_f32 = blk.data_ptr(), blk.dtype is _F32
         if gate is not None:
-            if gate.dtype is not torch.bfloat16 and gate.dtype is not torch.float32:
-                raise ValueError("gate must be bf16 or f32")
-            shape = tuple(gate.shape)
-            if shape == (H,) or shape == (1, H):
-                kind = 1
-            elif shape == (T, 1):
-                kind = 2
-            elif shape == (T, H):
-                kind = 3
-            else:
-                raise ValueError(f"gate must be [{H}], [{T}, 1] or [{T}, {H}]")
-            if kind != 2 and H > 1 and gate.stride(-1) != 1 or kind == 3 and T > 1 and gate.stride(0) < H:
-                gate = gate.contiguous()
-            if kind != 1:
-                gate_stride = gate.stride(0)
-        # a thread reads its elements of every tensor before it writes r': the same memory element for element is fine
-        apart = (t for t in (res, blk, gate, post_gain, pre_gain) if t is not None and not (
-            residual_out is not None and t.data_ptr() == residual_out.data_ptr() and t.dtype == residual_out.dtype
-            and t.shape == residual_out.shape and t.stride() == residual_out.stride()))
-        new = _out_rows(residual_out, (T, H), res.dtype, dev, "residual_out", *apart)
+            gate, kind, gate_stride = _gate(gate, T, H)
+            gate_f32 = gate.dtype is _F32
+        if residual_out is None:
+            new, new_stride = res.new_empty((T, H)), H
+        else:
+            # a thread reads its elements of every tensor before it writes r': the same memory element for element is fine
+            new, new_stride = residual_out, _check_out(residual_out, T, H, dtype, "residual_out", (
+                t for t in (res, blk, gate, post_gain, pre_gain) if t is not None and not (
+                    t.data_ptr() == residual_out.data_ptr() and t.dtype is dtype and t.shape == residual_out.shape
+                    and t.stride() == residual_out.stride())))
     x = scale = None
-    code, dtype = _OUT[out]
+    x_stride = 0
+    code, kind_of_x = _OUT[out]
     if pre_gain is not None:
         if code == 2:
-            x, scale = _empty_rows(T, H, dev), torch.empty(T, dtype=torch.float32, device=dev)
+            x, scale = _empty_rows(res, T, H), res.new_empty(T, dtype=_F32)
+            x_stride = max(x.stride(0), H)
         else:
-            x = torch.empty((T, H), dtype=dtype, device=dev)
+            x, x_stride = res.new_empty((T, H), dtype=kind_of_x), H
     if T:
-        f32 = torch.float32
-        _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, BlockNormArgs(
-            res.data_ptr(), None if blk is None else blk.data_ptr(), gate.data_ptr() if kind else None,
-            None if post_gain is None else post_gain.data_ptr(), None if pre_gain is None else pre_gain.data_ptr(),
-            None if blk is None else new.data_ptr(), None if x is None else x.data_ptr(), None if scale is None else scale.data_ptr(),
-            T, max(res.stride(0), H), H if blk is None else max(blk.stride(0), H), gate_stride, max(new.stride(0), H),
-            H if x is None else max(x.stride(0), H), H, res.dtype is f32, blk is not None and blk.dtype is f32,
-            kind != 0 and gate.dtype is f32, kind, gate_sigmoid, code, residual_scale, block_scale, eps))
+        _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, _lib.pack_block_norm(
+            res.data_ptr(), blk_ptr, gate.data_ptr() if kind else 0,
+            0 if post_gain is None else post_gain.data_ptr(), 0 if pre_gain is None else pre_gain.data_ptr(),
+            new.data_ptr() if blk_ptr else 0, 0 if x is None else x.data_ptr(), 0 if scale is None else scale.data_ptr(),
+            T, res_stride, blk_stride, gate_stride, new_stride, x_stride, H, dtype is _F32, blk_f32, gate_f32, kind,
+            bool(gate_sigmoid), code, residual_scale, block_scale, eps))
     return new, (QuantRows(x, scale) if scale is not None else x)
+
+
+def _gate(gate: torch.Tensor, T: int, H: int) -> tuple[torch.Tensor, int, int]:
+    """A gate with contiguous columns, its kind (1 per channel, 2 per token, 3 per element) and its row stride."""
+    if gate.dtype is not _BF16 and gate.dtype is not _F32:
+        raise ValueError("gate must be bf16 or f32")
+    shape = tuple(gate.shape)
+    if shape == (H,) or shape == (1, H):
+        kind = 1
+    elif shape == (T, 1):
+        kind = 2
+    elif shape == (T, H):
+        kind = 3
+    else:
+        raise ValueError(f"gate must be [{H}], [{T}, 1] or [{T}, {H}]")
+    if (kind != 2 and H > 1 and gate.stride(-1) != 1) or (kind == 3 and T > 1 and gate.stride(0) < H):
+        gate = gate.contiguous()
+    return gate, kind, 0 if kind == 1 else gate.stride(0)

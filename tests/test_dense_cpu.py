@@ -132,3 +132,11 @@ def test_calls_without_a_device_are_errors_not_crashes():
     assert lib.okc_moe_block_norm(C.byref(_norm_args()), None) == NO_DEVICE
     assert lib.okc_moe_int8_linear(C.byref(_int8_args()), None) == NO_DEVICE
     assert lib.okc_moe_quantize_rows(0x1000, 0, 64, 4, 64, 0x2000, 64, 0x3000, None) == NO_DEVICE
+
+
+def test_packed_arguments_are_the_structs():
+    """The byte strings the Python side passes are the ctypes (and so the C) structs, field for field."""
+    for cls, pack in ((_lib.BlockNormArgs, _lib.pack_block_norm), (_lib.Int8Args, _lib.pack_int8)):
+        n = len(cls._fields_)
+        values = [float(i + 1) if t is C.c_float else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+        assert bytes(cls(*values)) == pack(*values) and len(pack(*values)) == C.sizeof(cls), n
