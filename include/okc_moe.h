@@ -343,9 +343,9 @@ typedef struct okc_int8_args {
 uint64_t okc_moe_int8_scratch_bytes(int x_kind, int32_t tokens, int32_t k);
 int okc_moe_int8_linear(const okc_int8_args* args, okc_stream_t stream);
 int okc_moe_int8_gated(const okc_int8_args* args, okc_stream_t stream);
-/* Synchronises `stream`; 0, or OKC_ERR_TIMEOUT with *detail naming a device wait of an int8 product that ran out on the
- * current device since the last call of this function. */
-int okc_moe_int8_status(okc_stream_t stream, int32_t* detail);
+/* Synchronises `stream`; 0, or OKC_ERR_TIMEOUT with *detail naming a device wait of these operators that ran out on the
+ * current device since the last call of this function (the call it happened in has undefined results). */
+int okc_moe_dense_status(okc_stream_t stream, int32_t* detail);
 
 /* Copies the sorted-route tables out of `workspace` for inspection (host or device pointers are
  * NOT interchangeable: all four are device pointers; any may be NULL).  counts: int32

@@ -9,9 +9,9 @@
 The CUDA kernels live in csrc/ and are reached through the C ABI of include/okc_moe.h
 (libokc_moe_b200.so, built by ``python -m okc_muse_kernels_b200.build``).
 """
-from .dense import QuantRows, block_norm, int8_ffn, int8_gated, int8_linear, int8_rows, int8_status, quantize_rows
+from .dense import QuantRows, block_norm, int8_ffn, int8_gated, int8_linear, int8_rows, dense_status, quantize_rows
 from .moe import HostStep, MoEPlan, OkcError, cast_bf16, experts_ep, experts_profiled, kernel_fn, moe_block_step, moe_layer_step, moe_step, prepare, read_status, route, route_hidden, sorted_routes, split_router, unpack_bf16
 
-__all__ = ["HostStep", "MoEPlan", "OkcError", "QuantRows", "block_norm", "cast_bf16", "experts_ep", "experts_profiled", "int8_ffn", "int8_gated", "int8_linear", "int8_rows", "int8_status",
+__all__ = ["HostStep", "MoEPlan", "OkcError", "QuantRows", "block_norm", "cast_bf16", "experts_ep", "experts_profiled", "int8_ffn", "int8_gated", "int8_linear", "int8_rows", "dense_status",
            "kernel_fn", "moe_block_step", "moe_layer_step", "moe_step", "prepare", "quantize_rows", "read_status", "route", "route_hidden", "sorted_routes",
            "split_router", "unpack_bf16"]

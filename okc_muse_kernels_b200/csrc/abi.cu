@@ -55,18 +55,6 @@ bool encode_bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool encode_out_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t row_stride, bool f32) {
-  EncodeFn f = encode_fn();
-  if (!f) return false;
-  const cuuint64_t dims[2] = {cols, rows};
-  const cuuint64_t strides[1] = {row_stride * (f32 ? 4 : 2)};
-  const cuuint32_t box[2] = {32, 32};
-  const cuuint32_t estr[2] = {1, 1};
-  return f(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-           CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 static int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -1;
@@ -738,9 +726,12 @@ static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_
 int okc_moe_int8_linear(const okc_int8_args* args, okc_stream_t stream) { return int8_product(args, false, stream); }
 int okc_moe_int8_gated(const okc_int8_args* args, okc_stream_t stream) { return int8_product(args, true, stream); }
 
-int okc_moe_int8_status(okc_stream_t stream, int32_t* detail) {
-  int32_t code = 0;
-  if (int8_read_status(reinterpret_cast<cudaStream_t>(stream), &code) != cudaSuccess) return OKC_ERR_CUDA;
+int okc_moe_dense_status(okc_stream_t stream, int32_t* detail) {
+  int32_t norm = 0, product = 0;
+  if (norm_read_status(reinterpret_cast<cudaStream_t>(stream), &norm) != cudaSuccess ||
+      int8_read_status(reinterpret_cast<cudaStream_t>(stream), &product) != cudaSuccess)
+    return OKC_ERR_CUDA;
+  const int32_t code = product ? product : norm;
   if (detail) *detail = code;
   return code ? OKC_ERR_TIMEOUT : OKC_OK;
 }

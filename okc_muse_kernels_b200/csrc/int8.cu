@@ -10,7 +10,7 @@
 //   okc_int8_mid   some hundred     the weights fill M of a tcgen05.mma (kind::i8), the tokens are N; K is split over a
 //                                   cluster of CTAs that add their integer sums through distributed shared memory
 //   okc_int8_many  beyond           CTA pairs (cta_group::2) on tiles of 256 tokens x up to 256 weight rows, persistent
-// Every wait on a barrier is bounded; one that runs out is reported through a status word (okc_moe_int8_status).
+// Every wait on a barrier is bounded; one that runs out is reported through a status word (okc_moe_dense_status).
 #include <cooperative_groups.h>
 
 #include "rows.cuh"
@@ -115,11 +115,11 @@ __global__ void __launch_bounds__(kFewThreads) okc_int8_few(const Int8Params p, 
           if (raw) {
             float v[16];
             few_load_x(p, t, k, v);
-            const float inv = row_scale(amax_s[t]).inv;
-            xq[t].x = quant8x4(v[0], v[1], v[2], v[3], inv);
-            xq[t].y = quant8x4(v[4], v[5], v[6], v[7], inv);
-            xq[t].z = quant8x4(v[8], v[9], v[10], v[11], inv);
-            xq[t].w = quant8x4(v[12], v[13], v[14], v[15], inv);
+            const RowScale rs = row_scale(amax_s[t]);
+            xq[t].x = quant8x4(v[0], v[1], v[2], v[3], rs);
+            xq[t].y = quant8x4(v[4], v[5], v[6], v[7], rs);
+            xq[t].z = quant8x4(v[8], v[9], v[10], v[11], rs);
+            xq[t].w = quant8x4(v[12], v[13], v[14], v[15], rs);
           } else {
             xq[t] = load_q16(static_cast<const int8_t*>(p.x) + t * p.x_stride, k, p.K);
           }
@@ -431,10 +431,12 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStrea
   const int ttiles = (p.T + 255) / 256;
   q.tn = ((p.T + ttiles - 1) / ttiles + 15) & ~15;
   q.n_kb = (p.K + kKb - 1) / kKb;
-  // As many CTAs a cluster as one round of them fits the SMs.  K = 4096, N = 4096, 16 tokens (32 tiles), 1 / 2 / 4 / 8 CTAs
-  // a cluster: 10.5 / 7.8 / 6.6 / 13.9 us; gated, K = 7168, 2 x 2048 rows, 128 tokens: 18.4 / 12.9 / 10.6 / 26.0 us.
-  int splits = 1;
-  while (splits < 8 && 2 * splits <= q.n_kb && 2LL * splits * tiles * ttiles <= 148) splits *= 2;
+  // As many CTAs a cluster as one round of them fits the SMs (a cluster lives in one group of 16 to 20 SMs: 33 clusters of
+  // 4 and 15 of 8 fit at once).  K = 4096, N = 4096, 16 tokens (32 tiles), 1 / 2 / 4 / 8 CTAs a cluster: 10.5 / 7.8 / 6.6 /
+  // 13.9 us; gated, K = 7168, 2 x 2048 rows, 128 tokens: 18.4 / 12.9 / 10.6 / 26.0 us.
+  const int64_t clusters = static_cast<int64_t>(tiles) * ttiles;
+  int splits = clusters <= 14 ? 8 : clusters <= 32 ? 4 : clusters <= 74 ? 2 : 1;
+  while (splits > q.n_kb) splits /= 2;
   const int stage = kTileW * kKb + q.tn * kKb;
   q.stages = 216 * 1024 / stage;
   if (q.stages > kMidMaxStages) q.stages = kMidMaxStages;
@@ -470,19 +472,19 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStrea
 }
 
 // ------------------------------------------------------------------ many tokens
-constexpr int kManyThreads = 256;      // warps 0 TMA producer, 1 MMA issuer (leader CTA), 2 TMEM, 4..7 epilogue
+constexpr int kManyThreads = 384;      // warps 0 TMA producer, 1 MMA issuer (leader CTA), 2 TMEM, 3 weight scales, 4..11 epilogue
+constexpr int kManyEpilogueWarps = 8;  // one warp a scheduler kept up with one instruction in five cycles only
 constexpr int kManyStages = 6;
 constexpr int kManyStageBytes = 2 * 128 * kKb;
-constexpr int kManyStore = 4096;       // staging of an epilogue warp: 32 rows x 32 results
-constexpr int kManySmem = 1024 + kManyStages * kManyStageBytes + 4 * kManyStore;
+constexpr int kManyStore = 2048;       // staging of an epilogue warp: 32 rows x 64 bytes
+constexpr int kManySmem = 1024 + kManyStages * kManyStageBytes + kManyEpilogueWarps * kManyStore;
 
 struct Int8ManyParams {
   CUtensorMap xmap;      // int8 token rows, box 128 x 128 rows
   CUtensorMap wmap;      // int8 weight rows, box 128 x bn / 2 rows
-  CUtensorMap omap;      // output rows, box 32 columns x 32 rows (only with tma_out)
   Int8Params p;
   int bn;                // weight rows of a pair's tile (columns of its accumulator): a multiple of 32 (gated: 64), at most 256
-  int n_kb, tiles_t, tiles_n, tma_out;
+  int n_kb, tiles_t, tiles_n;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -543,17 +545,11 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// 2-D tiled tensor store shared -> global; elements outside the tensor are not written.
-__device__ __forceinline__ void tma_2d_s2g(const CUtensorMap* map, uint32_t src, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(src)
-               : "memory");
-}
-
 template <bool kGated>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_int8_many(const __grid_constant__ Int8ManyParams q) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  __shared__ uint64_t bar_full[kManyStages], bar_empty[kManyStages], bar_acc_full[2], bar_acc_empty[2];
+  __shared__ uint64_t bar_full[kManyStages], bar_empty[kManyStages], bar_acc_full[2], bar_acc_empty[2], bar_sc_full[2], bar_sc_empty[2];
   __shared__ __align__(16) float scale_s[2][256], bias_s[2][256];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_code;
@@ -565,7 +561,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
 
   if (tid == 0) {
     for (int i = 0; i < kManyStages; ++i) { mbar_init(smem_u32(&bar_full[i]), 1); mbar_init(smem_u32(&bar_empty[i]), 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&bar_acc_full[i]), 1); mbar_init(smem_u32(&bar_acc_empty[i]), 8); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_acc_full[i]), 1); mbar_init(smem_u32(&bar_acc_empty[i]), 2 * kManyEpilogueWarps);
+      mbar_init(smem_u32(&bar_sc_full[i]), 1); mbar_init(smem_u32(&bar_sc_empty[i]), kManyEpilogueWarps);
+    }
     abort_code = 0;
     mbar_fence_init();
   }
@@ -637,40 +636,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
       }
     }
     __syncwarp();
+  } else if (warp == 3) {
+    // the weight scales (and bias) of the tiles ahead of the epilogue, into shared memory
+    const int half = q.bn / 2, width = kGated ? half : q.bn;
+    uint32_t buf = 0, ph = 1;
+    for (int tile = pair; tile < tiles; tile += pairs) {
+      if (!pair_wait(smem_u32(&bar_sc_empty[buf]), ph, &abort_code, 0x75)) break;
+      const int tw = tile / q.tiles_t;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = i * 32 + lane;
+        const bool up = kGated && c >= half;
+        const int o = tw * width + (up ? c - half : c);
+        if (c < q.bn) {
+          scale_s[buf][c] = o < p.N ? __ldg(p.w_scale + (up ? p.N + o : o)) : 0.f;
+          if (!kGated && p.bias) bias_s[buf][c] = o < p.N ? __ldg(p.bias + o) : 0.f;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_sc_full[buf]));
+      buf ^= 1;
+      if (buf == 0) ph ^= 1;
+    }
   } else if (warp >= 4) {
     griddep_wait();        // the token scales come from the kernel before this one
-    const int ew = warp & 3, half = q.bn / 2;
+    const int ew = warp - 4, half = q.bn / 2;
     const int width = kGated ? half : q.bn;        // outputs of a tile
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(ew * 32) << 16);
-    const uint32_t stage = smem0 + kManyStages * kManyStageBytes + ew * kManyStore;
-    int n = 0;
-    bool ok = true;
-    for (int tile = pair; tile < tiles; tile += pairs, ++n) {
-      const int buf = n & 1;
-      const int tt = tile % q.tiles_t, tw = tile / q.tiles_t;
-      const int row0 = tt * 256 + static_cast<int>(rank) * 128 + ew * 32, t = row0 + lane;
-      const float sx = t < p.T ? p.x_scale[t] : 0.f;
-      // the tile's weight scales (and bias) once into shared memory; by the next write to this half of the array every
-      // warp has passed the barrier of the tile between, so it has finished reading
-      for (int c = tid - 128; c < q.bn; c += 128) {
-        const int o = tw * width + (kGated && c >= half ? c - half : c);
-        const bool in = o < p.N;
-        scale_s[buf][c] = in ? __ldg(p.w_scale + (kGated && c >= half ? p.N + o : o)) : 0.f;
-        if (!kGated && p.bias) bias_s[buf][c] = in ? __ldg(p.bias + o) : 0.f;
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      // (a warp that gives up goes on to meet the others at the barrier of each tile)
-      ok = ok && pair_wait(smem_u32(&bar_acc_full[buf]), (n >> 1) & 1, &abort_code, 0x74);
+    const int first = (ew >> 2) * 32;              // two warps share a quarter of the rows: every second 32 columns each
+    const int row_in = static_cast<int>(rank) * 128 + (ew & 3) * 32;
+    const uint32_t taddr = tmem + (static_cast<uint32_t>((ew & 3) * 32) << 16);
+    const uint32_t at = smem0 + kManyStages * kManyStageBytes + ew * kManyStore;
+    uint32_t buf = 0, ph = 0;
+    int t = (pair % q.tiles_t) * 256 + row_in + lane;
+    float sx_next = pair < tiles && t < p.T ? p.x_scale[t] : 0.f;
+    for (int tile = pair; tile < tiles; tile += pairs) {
+      const int tw = tile / q.tiles_t, row0 = (tile % q.tiles_t) * 256 + row_in;
+      const float sx = sx_next;
+      t = ((tile + pairs) % q.tiles_t) * 256 + row_in + lane;
+      if (tile + pairs < tiles && t < p.T) sx_next = p.x_scale[t];
+      t = row0 + lane;
+      if (!pair_wait(smem_u32(&bar_sc_full[buf]), ph, &abort_code, 0x76)) break;
+      if (!pair_wait(smem_u32(&bar_acc_full[buf]), ph, &abort_code, 0x74)) break;
       tc_fence_after();
-      for (int c0 = 0; ok && c0 < width; c0 += 32) {
+      const uint32_t acc_empty = map_rank(smem_u32(&bar_acc_empty[buf]), 0);
+      if (first >= width) {
+        if (lane == 0) mbar_arrive_cluster(acc_empty);
+      }
+      for (int c0 = first; c0 < width; c0 += 64) {
         uint32_t r[32], u[32];
         tmem_ld32(taddr + buf * 256 + c0, r);
         if (kGated) tmem_ld32(taddr + buf * 256 + half + c0, u);
         tmem_wait_ld();
-        if (c0 + 32 >= width) {       // the accumulator has been read: the pair's next tile but one may overwrite it
+        if (c0 + 64 >= width) {       // read for the last time: the pair's next tile but one may overwrite it
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(map_rank(smem_u32(&bar_acc_empty[buf]), 0));
+          if (lane == 0) mbar_arrive_cluster(acc_empty);
         }
         const float* ws = scale_s[buf] + c0;
         const float* bs = bias_s[buf] + c0;
@@ -681,56 +701,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
           else if (p.bias) v = __fadd_rn(v, bs[j]);
           r[j] = __float_as_uint(v);
         }
-        // A thread has 32 neighbouring results of its own row; they leave through shared memory so that whole pieces of
-        // rows are written: by one TMA store a warp, or, for rows it cannot address, 32 columns a warp store.
+        // A thread has 32 neighbouring results of its own row, 64 or 128 whole bytes, and stores them itself where 16-byte
+        // stores can.  (Through shared memory and TMA stores: the same time within 3 % from K = 1024 on.)
         const int col = tw * width + c0;
-        const uint32_t at = stage + (p.out_f32 ? 0u : static_cast<uint32_t>((c0 >> 5) & 1) * 2048u);
-        if (lane == 0) {
-          if (p.out_f32) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        }
-        __syncwarp();
-        if (p.out_f32) {
+        if (p.out_vec && col + 32 <= p.N) {
+          if (t < p.T) {
+            const int64_t o = static_cast<int64_t>(t) * p.out_stride + col;
+            if (p.out_f32) {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + o);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            st_shared_v4(at + lane * 128 + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-        } else {
+              for (int j = 0; j < 8; ++j) dst[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t w[4];
+              for (int j = 0; j < 4; ++j) {
+                uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
-            st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
-          }
-        }
-        if (q.tma_out) {
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) {
-            if (row0 < p.T && col < p.N) tma_2d_s2g(&q.omap, at, col, row0);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-        } else {
-          __syncwarp();
-          if (col + lane < p.N)
-            for (int i = 0; i < 32 && row0 + i < p.T; ++i) {
-              const int64_t o = static_cast<int64_t>(row0 + i) * p.out_stride + col + lane;
-              if (p.out_f32) {
-                uint32_t v;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4));
-                static_cast<float*>(p.out)[o] = __uint_as_float(v);
-              } else {
-                uint16_t v;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at + i * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2));
-                static_cast<uint16_t*>(p.out)[o] = v;
+                for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
+                dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
               }
             }
-          __syncwarp();
+          }
+        } else {
+          // rows off the 16-byte grid, or the last columns: through shared memory, so that a warp stores neighbours of a row
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 1 && !p.out_f32) break;
+            if (p.out_f32) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), r[16 * h + 4 * j], r[16 * h + 4 * j + 1], r[16 * h + 4 * j + 2], r[16 * h + 4 * j + 3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
+                st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
+              }
+            }
+            __syncwarp();
+            if (p.out_f32) {       // 16 columns of two rows a step
+              const int cc = col + 16 * h + (lane & 15);
+#pragma unroll 4
+              for (int i = lane >> 4; i < 32; i += 2) {
+                uint32_t v;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at + i * 64 + ((((lane & 15) >> 2) ^ ((i >> 1) & 3)) << 4) + (lane & 3) * 4));
+                if (cc < p.N && row0 + i < p.T) static_cast<float*>(p.out)[static_cast<int64_t>(row0 + i) * p.out_stride + cc] = __uint_as_float(v);
+              }
+            } else {
+              const int cc = col + lane;
+#pragma unroll 8
+              for (int i = 0; i < 32; ++i) {
+                uint16_t v;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at + i * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2));
+                if (cc < p.N && row0 + i < p.T) static_cast<uint16_t*>(p.out)[static_cast<int64_t>(row0 + i) * p.out_stride + cc] = v;
+              }
+            }
+            __syncwarp();
+          }
         }
+        __syncwarp();      // the next load from tensor memory is one of the whole warp
       }
+      if (lane == 0) mbar_arrive(smem_u32(&bar_sc_empty[buf]));
+      buf ^= 1;
+      if (buf == 0) ph ^= 1;
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-    __syncwarp();
   }
   tc_fence_before();
   cg::this_cluster().sync();     // no CTA frees its tensor memory or leaves while the pair's MMAs and arrivals may touch it
@@ -749,20 +784,20 @@ cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStre
   q.n_kb = (p.K + kKb - 1) / kKb;
   q.tiles_t = (p.T + 255) / 256;
   const int64_t cols = static_cast<int64_t>(gated ? 2 : 1) * p.N;
-  // The tile width that leaves the least work in the last round of the 74 pairs.
+  // The tile width with the least work in whole rounds of the 74 pairs.  A round of tiles bn wide takes a time in proportion
+  // to bn + 120 (K = 7168, bn 64 / 96 / 128 / 160 / 192 / 224 / 256: 11.1 / 11.4 / 12.4 / 14.1 / 15.0 / 18.1 / 18.9 us): the
+  // token rows of a tile are copied whatever its width.  Narrow tiles win where wide ones leave pairs without work.
   q.bn = 256;
   long long best = -1;
-  for (int bn = 256; bn >= 128; bn -= gated ? 64 : 32) {
+  for (int bn = 256; bn >= 64; bn -= gated ? 64 : 32) {
     const long long tn = (cols + bn - 1) / bn;
-    const long long cost = ((tn * q.tiles_t + 73) / 74) * (bn + 16);
+    const long long cost = ((tn * q.tiles_t + 73) / 74) * (bn + 120);
     if (best < 0 || cost < best) { best = cost; q.bn = bn; q.tiles_n = static_cast<int>(tn); }
   }
   if (gated) q.tiles_n = (p.N + q.bn / 2 - 1) / (q.bn / 2);
   if (!encode_bytes_map(&q.xmap, p.x, p.T, p.K, p.x_stride, 128) ||
       !encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(cols), p.K, p.w_stride, q.bn / 2))
     return cudaErrorInvalidValue;
-  q.tma_out = p.out_vec;
-  if (q.tma_out && !encode_out_map(&q.omap, p.out, p.T, p.N, p.out_stride, p.out_f32 != 0)) return cudaErrorInvalidValue;
   const long long tiles = static_cast<long long>(q.tiles_t) * q.tiles_n;
   const int grid = static_cast<int>(tiles < 74 ? 2 * tiles : 148);
   auto kernel = gated ? okc_int8_many<true> : okc_int8_many<false>;

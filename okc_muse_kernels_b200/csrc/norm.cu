@@ -13,6 +13,8 @@
 
 namespace okc {
 
+__device__ int32_t g_norm_status;      // code of the first wait that ran out since the last read
+
 // most threads of a CTA: with 32 values of each tensor in registers a thread needs up to 128 registers
 constexpr int row_threads(int chunks) { return chunks == 4 ? 512 : 1024; }
 
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_block_norm(const Blo
     const RowScale s = row_scale(cta_max(amax, red_max));
     int8_t* dst = static_cast<int8_t*>(p.out) + row * p.out_stride;
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j) store_chunk_q<kVec>(dst, j, tid, nt, H, r[j], s.inv);
+    for (int j = 0; j < kChunks; ++j) store_chunk_q<kVec>(dst, j, tid, nt, H, r[j], s);
     if (tid == 0) p.out_scale[row] = s.scale;
   } else {
     const bool f32 = p.out_kind == kRowsF32;
@@ -111,6 +113,152 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_block_norm(const Blo
                     : static_cast<void*>(static_cast<uint16_t*>(p.out) + row * p.out_stride);
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) store_chunk<kVec>(dst, f32, j, tid, nt, H, r[j]);
+  }
+}
+
+// The same for many rows that 16-byte accesses can reach: persistent CTAs, each with a ring of rows in shared memory that
+// bulk copies fill ahead of it, so that HBM does not wait for the two dependent sums of a row.  The gains are copied
+// once.  4096 x 5120, everything bf16, a gate per element: NORM_US us (NORM_TB TB/s); a CTA per row 65.1 us (3.2 TB/s).
+constexpr int kStreamStages = 8;
+template <int kChunks>
+__global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream(const BlockNormParams p, int rows, int stages, int row_bytes) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ uint64_t bar_full[kStreamStages];
+  __shared__ int abort_code;
+  __shared__ float red_post[2][32], red_pre[2][32];
+  __shared__ uint32_t red_max[2][32];
+  const int tid = threadIdx.x, nt = blockDim.x, H = p.H;
+  const uint32_t res_bytes = static_cast<uint32_t>(H) * (p.res_f32 ? 4 : 2), blk_bytes = static_cast<uint32_t>(H) * (p.blk_f32 ? 4 : 2);
+  const bool gate_rows = p.gate && p.gate_col_stride != 0 && p.gate_stride != 0, gate_cols = p.gate && p.gate_col_stride != 0 && p.gate_stride == 0;
+  const uint32_t gate_bytes = gate_rows || gate_cols ? static_cast<uint32_t>(H) * (p.gate_f32 ? 4 : 2) : 0;
+  const uint32_t gain_bytes = static_cast<uint32_t>(H) * 4;
+  // shared memory: post gain, pre gain, channel gate (each if there), then the ring
+  uint8_t* const post_s = smem;
+  uint8_t* const pre_s = post_s + (p.post_gain ? gain_bytes : 0);
+  uint8_t* const chan_s = pre_s + (p.pre_gain ? gain_bytes : 0);
+  uint8_t* const ring = chan_s + (gate_cols ? gate_bytes : 0);
+  auto fetch = [&](int row, int st) {
+    const uint32_t bar = smem_u32(&bar_full[st]);
+    uint32_t dst = smem_u32(ring) + st * row_bytes;
+    mbar_expect_tx(bar, res_bytes + blk_bytes + (gate_rows ? gate_bytes : 0));
+    bulk_g2s(dst, static_cast<const uint8_t*>(p.res) + row * p.res_stride * (p.res_f32 ? 4 : 2), res_bytes, bar);
+    bulk_g2s(dst + res_bytes, static_cast<const uint8_t*>(p.blk) + row * p.blk_stride * (p.blk_f32 ? 4 : 2), blk_bytes, bar);
+    if (gate_rows) bulk_g2s(dst + res_bytes + blk_bytes, static_cast<const uint8_t*>(p.gate) + row * p.gate_stride * (p.gate_f32 ? 4 : 2), gate_bytes, bar);
+  };
+  if (tid == 0) {
+    for (int i = 0; i < stages; ++i) mbar_init(smem_u32(&bar_full[i]), 1);
+    abort_code = 0;
+    mbar_fence_init();
+    for (int i = 0; i < stages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
+  }
+  for (int i = tid * 4; i < H; i += nt * 4) {
+    if (p.post_gain) *reinterpret_cast<float4*>(post_s + i * 4) = *reinterpret_cast<const float4*>(p.post_gain + i);
+    if (p.pre_gain) *reinterpret_cast<float4*>(pre_s + i * 4) = *reinterpret_cast<const float4*>(p.pre_gain + i);
+  }
+  if (gate_cols)
+    for (uint32_t i = tid * 16; i < gate_bytes; i += nt * 16)
+      *reinterpret_cast<uint4*>(chan_s + i) = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.gate) + i);
+  __syncthreads();
+  int st = 0, n = 0;
+  uint32_t ph = 0;
+  for (int row = blockIdx.x; row < rows; row += gridDim.x, ++n) {
+    // a wait that runs out does not leave the loop (the other threads count on this one's barriers): the row's result is
+    // then undefined and the status word says so
+    mbar_wait(smem_u32(&bar_full[st]), ph, &abort_code, 0x81);
+    const uint8_t* const src = ring + st * row_bytes;
+    float mul = p.blk_scale;
+    if (p.gate && p.gate_col_stride == 0) {
+      const int64_t o = row * p.gate_stride;
+      float g = p.gate_f32 ? static_cast<const float*>(p.gate)[o]
+                           : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p.gate)[o]) << 16);
+      if (p.gate_sigmoid) g = 1.f / (1.f + __expf(-g));
+      mul *= g;
+    }
+    float r[kChunks][8];
+    {
+      float y[kChunks][8];
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j) load_chunk<true>(src + res_bytes, p.blk_f32, j, tid, nt, H, y[j]);
+      if (p.post_gain) {
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss = fmaf(y[j][e], y[j][e], ss);
+        const float rstd = rsqrtf(cta_sum(ss, red_post[n & 1]) / static_cast<float>(H) + p.eps);
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+          float g[8];
+          load_chunk<true>(post_s, true, j, tid, nt, H, g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[j][e] = y[j][e] * rstd * g[e];
+        }
+      }
+      if (p.gate && p.gate_col_stride != 0) {
+        const uint8_t* gsrc = gate_rows ? src + res_bytes + blk_bytes : chan_s;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+          float g[8];
+          load_chunk<true>(gsrc, p.gate_f32, j, tid, nt, H, g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[j][e] *= p.gate_sigmoid ? 1.f / (1.f + __expf(-g[e])) : g[e];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j) {
+        load_chunk<true>(src, p.res_f32, j, tid, nt, H, r[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[j][e] = p.res_scale * r[j][e] + mul * y[j][e];
+      }
+    }
+    void* rdst = p.res_f32 ? static_cast<void*>(static_cast<float*>(p.res_out) + row * p.res_out_stride)
+                           : static_cast<void*>(static_cast<uint16_t*>(p.res_out) + row * p.res_out_stride);
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      store_chunk<true>(rdst, p.res_f32, j, tid, nt, H, r[j]);
+      if (row_col<true>(j, 0, tid, nt) < H)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(r[j][e], r[j][e], ss);
+    }
+    float rstd = 0.f;
+    if (p.pre_gain) rstd = rsqrtf(cta_sum(ss, red_pre[n & 1]) / static_cast<float>(H) + p.eps);
+    // every thread has read its part of the slot once it is past that sum's barrier
+    if (!p.pre_gain || nt == 32) __syncthreads();
+    if (tid == 0 && row + static_cast<int64_t>(stages) * gridDim.x < rows) fetch(row + stages * gridDim.x, st);
+    if (p.pre_gain) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j) {
+        float g[8];
+        load_chunk<true>(pre_s, true, j, tid, nt, H, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[j][e] = r[j][e] * rstd * g[e];
+        if (row_col<true>(j, 0, tid, nt) < H)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) amax = max(amax, abs_bits(r[j][e]));
+      }
+      if (p.out_kind == kRowsInt8) {
+        const RowScale s = row_scale(cta_max(amax, red_max[n & 1]));
+        int8_t* dst = static_cast<int8_t*>(p.out) + row * p.out_stride;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) store_chunk_q<true>(dst, j, tid, nt, H, r[j], s);
+        if (tid == 0) p.out_scale[row] = s.scale;
+      } else {
+        const bool f32 = p.out_kind == kRowsF32;
+        void* dst = f32 ? static_cast<void*>(static_cast<float*>(p.out) + row * p.out_stride)
+                        : static_cast<void*>(static_cast<uint16_t*>(p.out) + row * p.out_stride);
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) store_chunk<true>(dst, f32, j, tid, nt, H, r[j]);
+      }
+    }
+    if (++st == stages) { st = 0; ph ^= 1; }
+  }
+  __syncthreads();
+  if (tid == 0 && abort_code != 0) {
+    atomicCAS(&g_norm_status, 0, abort_code);
+    const long long c0 = clock64();      // copies that are late get some time before the CTA's memory is another's
+    while (clock64() - c0 < kWaitLimitCycles / 100) {}
   }
 }
 
@@ -142,8 +290,40 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_quantize_rows(const 
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
       if (passes > 1) load_chunk<kVec>(src, p.x_f32, s * kChunks + j, tid, nt, p.cols, v[j]);
-      store_chunk_q<kVec>(dst, s * kChunks + j, tid, nt, p.cols, v[j], rs.inv);
+      store_chunk_q<kVec>(dst, s * kChunks + j, tid, nt, p.cols, v[j], rs);
     }
+  }
+}
+
+// The same for many rows of bf16: a warp per row, which it holds in registers as it is (up to 8192 columns in 128 of them).
+// Nothing waits on other warps, and a dozen warps an SM have their whole rows on the way at once.  4096 x 7168: the
+// kernel above, a CTA per row, 27.7 us; this one QUANT_US us (88 MB: QUANT_TB TB/s).
+template <int kVecs>
+__global__ void __launch_bounds__(128) okc_quantize_rows_warp(const QuantizeParams p, int64_t rows) {
+  griddep_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + row * p.x_stride);
+  const int units = p.cols / 8;
+  uint4 v[kVecs];
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    v[j] = make_uint4(0, 0, 0, 0);
+    if (j * 32 + lane < units) v[j] = __ldg(src + j * 32 + lane);
+  }
+  uint32_t m = 0;      // two running maxima of the magnitudes' bits, 16 bits each
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j)
+    m = __vmaxu2(__vmaxu2(__vmaxu2(m, v[j].x & 0x7FFF7FFFu), v[j].y & 0x7FFF7FFFu), __vmaxu2(v[j].z & 0x7FFF7FFFu, v[j].w & 0x7FFF7FFFu));
+  const RowScale s = row_scale(__reduce_max_sync(0xffffffffu, max(m & 0xFFFF0000u, m << 16)));
+  if (lane == 0) p.scale[row] = s.scale;
+  uint2* dst = reinterpret_cast<uint2*>(p.q + row * p.q_stride);
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    float f[8];
+    unpack_bf16x8(v[j], f);
+    if (j * 32 + lane < units) dst[j * 32 + lane] = make_uint2(quant8x4(f[0], f[1], f[2], f[3], s), quant8x4(f[4], f[5], f[6], f[7], s));
   }
 }
 
@@ -157,7 +337,36 @@ static void row_shape(int64_t rows, int cols, int& threads, int& chunks) {
   if (threads > row_threads(chunks)) threads = row_threads(chunks);
 }
 
+// The streaming kernel, if the rows are many and a ring of at least two fits; false: not launched.
+static bool try_stream(const BlockNormParams& p, int64_t rows, cudaStream_t stream, cudaError_t& e) {
+  if (!p.blk || rows < 4 * 148 || rows > INT32_MAX / 2) return false;
+  const int units = p.H / 8;
+  const int chunks = units > 1024 ? 4 : units > 256 ? 2 : 1;
+  const int threads = ((units + chunks - 1) / chunks + 31) / 32 * 32;
+  const bool rows_gate = p.gate && p.gate_col_stride != 0 && p.gate_stride != 0, cols_gate = p.gate && p.gate_col_stride != 0 && p.gate_stride == 0;
+  const int row_bytes = p.H * ((p.res_f32 ? 4 : 2) + (p.blk_f32 ? 4 : 2) + (rows_gate ? (p.gate_f32 ? 4 : 2) : 0));
+  const int fixed = p.H * ((p.post_gain ? 4 : 0) + (p.pre_gain ? 4 : 0) + (cols_gate ? (p.gate_f32 ? 4 : 2) : 0));
+  int per_sm = chunks == 4 ? 1 : 65536 / (threads * 64);      // CTAs an SM: by registers, then by shared memory
+  if (per_sm > 4) per_sm = 4;
+  int stages = 0;
+  for (; per_sm >= 1; --per_sm) {
+    stages = (216 * 1024 / per_sm - fixed - 2048) / row_bytes;
+    if (stages >= 2) break;
+  }
+  if (per_sm < 1) return false;
+  if (stages > kStreamStages) stages = kStreamStages;
+  const size_t smem = fixed + static_cast<size_t>(stages) * row_bytes;
+  const int64_t most = 148LL * per_sm;
+  const dim3 grid(static_cast<unsigned>(rows < most ? rows : most)), block(threads);
+  auto kernel = chunks == 1 ? okc_block_norm_stream<1> : chunks == 2 ? okc_block_norm_stream<2> : okc_block_norm_stream<4>;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e == cudaSuccess) e = launch_kernel(kernel, grid, block, smem, stream, false, p, static_cast<int>(rows), stages, row_bytes);
+  return true;
+}
+
 cudaError_t launch_block_norm(const BlockNormParams& p, int64_t rows, bool vec, cudaStream_t stream) {
+  cudaError_t e;
+  if (vec && try_stream(p, rows, stream, e)) return e;
   int threads, chunks;
   row_shape(rows, p.H, threads, chunks);
   const dim3 grid(static_cast<unsigned>(rows)), block(threads);
@@ -167,12 +376,30 @@ cudaError_t launch_block_norm(const BlockNormParams& p, int64_t rows, bool vec, 
 }
 
 cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool vec, cudaStream_t stream) {
+  if (vec && !p.x_f32 && p.cols <= 8192 && rows >= 4 * 148) {
+    const dim3 grid(static_cast<unsigned>((rows + 3) / 4)), block(128);
+    if (p.cols <= 1024) return launch_kernel(okc_quantize_rows_warp<4>, grid, block, 0, stream, false, p, rows);
+    if (p.cols <= 2048) return launch_kernel(okc_quantize_rows_warp<8>, grid, block, 0, stream, false, p, rows);
+    if (p.cols <= 4096) return launch_kernel(okc_quantize_rows_warp<16>, grid, block, 0, stream, false, p, rows);
+    return launch_kernel(okc_quantize_rows_warp<32>, grid, block, 0, stream, false, p, rows);
+  }
   int threads, chunks;
   row_shape(rows, p.cols, threads, chunks);
   const dim3 grid(static_cast<unsigned>(rows)), block(threads);
   if (chunks == 1) return vec ? launch_kernel(okc_quantize_rows<1, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_quantize_rows<1, false>, grid, block, 0, stream, false, p);
   if (chunks == 2) return vec ? launch_kernel(okc_quantize_rows<2, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_quantize_rows<2, false>, grid, block, 0, stream, false, p);
   return vec ? launch_kernel(okc_quantize_rows<4, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_quantize_rows<4, false>, grid, block, 0, stream, false, p);
+}
+
+__global__ void okc_norm_clear_status() { g_norm_status = 0; }
+
+cudaError_t norm_read_status(cudaStream_t stream, int32_t* code) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(code, g_norm_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, stream);
+  if (e != cudaSuccess) return e;
+  okc_norm_clear_status<<<1, 1, 0, stream>>>();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return cudaStreamSynchronize(stream);
 }
 
 }  // namespace okc

@@ -16,20 +16,26 @@ namespace okc {
 // is NaN instead of a number made from part of it.
 struct RowScale {
   float scale, inv;
+  uint32_t keep;      // all ones, or zero for a row that is not finite
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
   RowScale s;
   const float a = __uint_as_float(amax_bits);
-  if (amax_bits >= 0x7F800000u) { s.scale = __uint_as_float(0x7FC00000u); s.inv = 0.f; }
-  else if (a < 7.52316385e-37f) { s.scale = 0.f; s.inv = 0.f; }
-  else { s.scale = __fdiv_rn(a, 127.f); s.inv = __fdiv_rn(127.f, a); }
+  const bool zero = a < 7.52316385e-37f;                        // 2^-120
+  s.keep = amax_bits < 0x7F800000u ? 0xFFFFFFFFu : 0u;
+  s.scale = zero ? 0.f : s.keep ? __fdiv_rn(a, 127.f) : __uint_as_float(0x7FC00000u);
+  s.inv = zero || !s.keep ? 0.f : __fdiv_rn(127.f, a);
   return s;
 }
-// x * inv is within 127 * (1 + 2^-23) of zero, so the rounded value needs no clamp.  A row that is not finite has
-// inv = 0: infinity * 0 is NaN, which the conversion to an integer makes 0.
-__device__ __forceinline__ uint32_t quant8(float x, float inv) { return static_cast<uint32_t>(__float2int_rn(__fmul_rn(x, inv))) & 0xFFu; }
-__device__ __forceinline__ uint32_t quant8x4(float a, float b, float c, float d, float inv) {
-  return quant8(a, inv) | (quant8(b, inv) << 8) | (quant8(c, inv) << 16) | (quant8(d, inv) << 24);
+// rint(x * inv) as a byte.  Below 2^22 in magnitude, v + 1.5 * 2^23 rounds v to an integer, halves to even, which then is
+// the low end of the sum's bits: one addition instead of a conversion, which runs at a quarter of its rate or less.
+// |x * inv| is at most 127 * (1 + 2^-23), so the value needs no clamp; a row that is not finite has its bytes cleared.
+__device__ __forceinline__ uint32_t quant_bits(float x, float inv) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.f)); }
+__device__ __forceinline__ uint32_t quant8(float x, const RowScale& s) { return quant_bits(x, s.inv) & s.keep & 0xFFu; }
+__device__ __forceinline__ uint32_t quant8x4(float a, float b, float c, float d, const RowScale& s) {
+  const uint32_t lo = __byte_perm(quant_bits(a, s.inv), quant_bits(b, s.inv), 0x0040);
+  const uint32_t hi = __byte_perm(quant_bits(c, s.inv), quant_bits(d, s.inv), 0x0040);
+  return __byte_perm(lo, hi, 0x5410) & s.keep;
 }
 // Bits of |x|: compared as integers a NaN is above every number, so a maximum of these never loses one.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
@@ -104,15 +110,15 @@ __device__ __forceinline__ void store_chunk(void* row, bool f32, int chunk, int 
   }
 }
 template <bool kVec>
-__device__ __forceinline__ void store_chunk_q(int8_t* row, int chunk, int tid, int nt, int cols, const float (&v)[8], float inv) {
+__device__ __forceinline__ void store_chunk_q(int8_t* row, int chunk, int tid, int nt, int cols, const float (&v)[8], const RowScale& s) {
   if (kVec) {
     const int c = row_col<true>(chunk, 0, tid, nt);
-    if (c < cols) *reinterpret_cast<uint2*>(row + c) = make_uint2(quant8x4(v[0], v[1], v[2], v[3], inv), quant8x4(v[4], v[5], v[6], v[7], inv));
+    if (c < cols) *reinterpret_cast<uint2*>(row + c) = make_uint2(quant8x4(v[0], v[1], v[2], v[3], s), quant8x4(v[4], v[5], v[6], v[7], s));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int c = row_col<false>(chunk, e, tid, nt);
-      if (c < cols) row[c] = static_cast<int8_t>(quant8(v[e], inv));
+      if (c < cols) row[c] = static_cast<int8_t>(quant8(v[e], s));
     }
   }
 }

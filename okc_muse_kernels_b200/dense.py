@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["QuantRows", "quantize_rows", "int8_rows", "int8_linear", "int8_gated", "int8_ffn", "block_norm", "int8_status"]
+__all__ = ["QuantRows", "quantize_rows", "int8_rows", "int8_linear", "int8_gated", "int8_ffn", "block_norm", "dense_status"]
 
 BLOCK_NORM_MAX_HIDDEN = 16384
 INT8_MAX_K = 131071           # the integer sums stay in 32 bits
@@ -49,11 +49,13 @@ def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream     # the current stream of a device as an integer
+_current_device = torch._C._cuda_getDevice           # (a CUDA tensor is at hand: CUDA is initialised)
+_empty = torch.empty_strided                         # the cheapest of torch's ways to uninitialised memory
 
 
 def _call(fn, name: str, dev: int, *args) -> None:
     """The C entry on the tensors' device (made current for the call if it is not) and its current stream."""
-    if torch.cuda.current_device() == dev:
+    if _current_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -85,13 +87,12 @@ def _vector(t: torch.Tensor | None, n: int, what: str) -> torch.Tensor | None:
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the memory from a's first to its last element touches b's."""
-    if a.numel() == 0 or b.numel() == 0:
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    gap = b.data_ptr() - a.data_ptr()
+    if gap >= a.untyped_storage().nbytes() or not a.numel() or not b.numel():
         return False
-    def span(t):
-        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (n + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    return gap < (1 + sum((n - 1) * st for n, st in zip(a.shape, a.stride()))) * a.element_size()
 
 
 def _check_out(out: torch.Tensor, R: int, cols: int, dtype: torch.dtype, what: str, inputs) -> int:
@@ -110,7 +111,7 @@ def _check_out(out: torch.Tensor, R: int, cols: int, dtype: torch.dtype, what: s
 # ------------------------------------------------------------------------------------------------ int8 rows
 def _empty_rows(like: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
     pad = (cols + 15) // 16 * 16
-    q = like.new_empty((rows, pad), dtype=_I8)
+    q = _empty((rows, pad), (pad, 1), dtype=_I8, device=like.device)
     return q if pad == cols else q[:, :cols]
 
 
@@ -124,7 +125,7 @@ def quantize_rows(x: torch.Tensor) -> QuantRows:
         raise ValueError(f"rows of 1 to {INT8_MAX_K} columns, got {cols}")
     dev = _device(x)
     q = _empty_rows(x, R, cols)
-    scale = x.new_empty(R, dtype=_F32)
+    scale = _empty((R,), (1,), dtype=_F32, device=x.device)
     if R:
         _call(_lib.lib().okc_moe_quantize_rows, "okc_moe_quantize_rows", dev, x.data_ptr(), _ROWS_KIND[x.dtype],
               stride, R, cols, q.data_ptr(), max(q.stride(0), cols), scale.data_ptr())
@@ -161,29 +162,30 @@ def _product(name: str, x, weight, bias, out_f32: bool, out, halves: int) -> tor
     if N < halves or N % halves:
         raise ValueError("a gated weight holds the gate rows and then as many up rows" if halves == 2 else "weight has no rows")
     N //= halves
-    x_scale = None
     if isinstance(x, tuple):
         x, x_scale, T, cols, x_stride = _check_quant(x, "x")
+        xs_ptr, scratch = x_scale.data_ptr(), 0
     else:
         x, T, cols, x_stride = _rows(x, "x")
+        x_scale, xs_ptr, scratch = None, 0, T > INT8_FEW_TOKENS
     if cols != K or K < 1 or K > INT8_MAX_K:
         raise ValueError(f"x has {cols} columns and weight {K}; 1 to {INT8_MAX_K}, and as many in both")
     dev = _device(x, x_scale, w, w_scale, bias, out)
     bias = _vector(bias, N, "bias")
-    dtype = _F32 if out_f32 else _BF16
     if out is None:
-        out, out_stride = x.new_empty((T, N), dtype=dtype), N
+        out, out_stride = _empty((T, N), (N, 1), dtype=_F32 if out_f32 else _BF16, device=x.device), N
     else:
-        out_stride = _check_out(out, T, N, dtype, "out", (x, x_scale, w, w_scale, bias))
+        out_stride = _check_out(out, T, N, _F32 if out_f32 else _BF16, "out", (x, x_scale, w, w_scale, bias))
     if T == 0:
         return out
-    lib = _lib.lib()
-    scratch = None
-    if x_scale is None and T > INT8_FEW_TOKENS:
-        scratch = x.new_empty(lib.okc_moe_int8_scratch_bytes(0, T, K), dtype=_I8)
-    _call(getattr(lib, name), name, dev, _lib.pack_int8(
-        x.data_ptr(), 0 if x_scale is None else x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
-        0 if bias is None else bias.data_ptr(), out.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+    if scratch:      # int8 rows and scales of the tokens: okc_moe_int8_scratch_bytes
+        n = T * ((K + 15) // 16 * 16 + 4)
+        scratch = _empty((n,), (1,), dtype=_I8, device=x.device)
+        xs = scratch.data_ptr()
+    else:
+        xs = 0
+    _call(getattr(_lib.lib(), name), name, dev, _lib.pack_int8(
+        x.data_ptr(), xs_ptr, w.data_ptr(), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), xs,
         x_stride, w_stride, out_stride, _ROWS_KIND[x.dtype], out_f32, T, K, N))
     return out
 
@@ -213,11 +215,11 @@ def int8_ffn(x, w13, w2, *, bias: torch.Tensor | None = None, out_f32: bool = Fa
     return int8_linear(int8_gated(x, w13), w2, bias=bias, out_f32=out_f32, out=out)
 
 
-def int8_status() -> tuple[int, int]:
-    """(status, detail) of the int8 products on the current device since the last call: (0, 0), or (OKC_ERR_TIMEOUT, code)
+def dense_status() -> tuple[int, int]:
+    """(status, detail) of this module's operators on the current device since the last call: (0, 0), or (OKC_ERR_TIMEOUT, code)
     when a bounded device wait ran out.  Synchronises the current stream."""
     detail = C.c_int32(0)
-    rc = _lib.lib().okc_moe_int8_status(torch.cuda.current_stream().cuda_stream, C.byref(detail))
+    rc = _lib.lib().okc_moe_dense_status(torch.cuda.current_stream().cuda_stream, C.byref(detail))
     return rc, detail.value
 
 
@@ -264,7 +266,7 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
             gate, kind, gate_stride = _gate(gate, T, H)
             gate_f32 = gate.dtype is _F32
         if residual_out is None:
-            new, new_stride = res.new_empty((T, H)), H
+            new, new_stride = _empty((T, H), (H, 1), dtype=dtype, device=res.device), H
         else:
             # a thread reads its elements of every tensor before it writes r': the same memory element for element is fine
             new, new_stride = residual_out, _check_out(residual_out, T, H, dtype, "residual_out", (
@@ -276,10 +278,10 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
     code, kind_of_x = _OUT[out]
     if pre_gain is not None:
         if code == 2:
-            x, scale = _empty_rows(res, T, H), res.new_empty(T, dtype=_F32)
+            x, scale = _empty_rows(res, T, H), _empty((T,), (1,), dtype=_F32, device=res.device)
             x_stride = max(x.stride(0), H)
         else:
-            x, x_stride = res.new_empty((T, H), dtype=kind_of_x), H
+            x, x_stride = _empty((T, H), (H, 1), dtype=kind_of_x, device=res.device), H
     if T:
         _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, _lib.pack_block_norm(
             res.data_ptr(), blk_ptr, gate.data_ptr() if kind else 0,

@@ -80,7 +80,8 @@ def _gated_ref(q, scale, w, dtype):
 
 
 # ------------------------------------------------------------------------------------------------ quantize_rows
-@pytest.mark.parametrize("R,cols", [(1, 1), (3, 7), (2, 16), (5, 1000), (33, 4096), (2, 16385), (400, 2880), (301, 9000), (2, 131071), (7, 131064)])
+@pytest.mark.parametrize("R,cols", [(1, 1), (3, 7), (2, 16), (5, 1000), (33, 4096), (2, 16385), (400, 2880), (301, 9000), (2, 131071), (7, 131064),
+                                    (593, 8), (595, 1016), (600, 2048), (700, 4088), (601, 8192), (599, 8200), (600, 1001)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_quantize_rows_is_exact(R, cols, dtype):
     x = _randn((R, cols), _gen(R * cols), dtype)
@@ -90,15 +91,16 @@ def test_quantize_rows_is_exact(R, cols, dtype):
     assert got.q.stride(0) % 16 == 0 or R == 1
 
 
-def test_quantize_rows_special_rows():
-    x = torch.randn((12, 40), device="cuda")
+@pytest.mark.parametrize("rows,dtype", [(12, torch.float32), (12, torch.bfloat16), (700, torch.bfloat16)])
+def test_quantize_rows_special_rows(rows, dtype):
+    x = torch.randn((rows, 40), device="cuda").to(dtype)
     x[1] = 0
     x[2, 5] = float("inf")
     x[3, 39] = float("-inf")
     x[4, 0] = float("nan")
     x[5] *= 2.0 ** -130 / x[5].abs().max()            # below 2^-120: zeros
     x[6] = x[6] / x[6].abs().max() * 2.0 ** -119      # above
-    x[7] = x[7] / x[7].abs().max() * 3.4e38           # largest f32 values
+    x[7] = x[7] / x[7].abs().max() * 3.3e38           # near the largest values
     x[8, :] = 254.0                                   # multiplier 1/2: halves ...
     x[8, 1:5] = torch.tensor([1.0, 3.0, 5.0, -7.0])   # ... go to the even neighbour
     x[9, 3] = float("nan")
@@ -106,7 +108,7 @@ def test_quantize_rows_special_rows():
     got = okc.quantize_rows(x)
     q, scale = _quant_ref(x)
     assert torch.equal(got.q, q)
-    assert torch.equal(got.scale.isnan(), scale.isnan()) and got.scale.isnan().tolist() == [i in (2, 3, 4, 9) for i in range(12)]
+    assert torch.equal(got.scale.isnan(), scale.isnan()) and got.scale.isnan().tolist() == [i in (2, 3, 4, 9) for i in range(rows)]
     assert torch.equal(got.scale.nan_to_num(), scale.nan_to_num())
     assert q[8, 1:5].tolist() == [0, 2, 2, -4] and not q[5].any() and q[6].any()
 
@@ -140,7 +142,7 @@ def test_int8_linear(T, K, N, dtype):
             assert y.dtype == (torch.float32 if out_f32 else torch.bfloat16)
             _close(y, *_linear_ref(q, scale, w, b, y.dtype), f"bias {b is not None} f32 {out_f32}")
             assert torch.equal(y, okc.int8_linear(okc.quantize_rows(x), w, bias=b, out_f32=out_f32)), "int8 tokens"
-    assert okc.int8_status() == (0, 0)
+    assert okc.dense_status() == (0, 0)
 
 
 @pytest.mark.parametrize("T,K,N", SHAPES)
@@ -153,7 +155,7 @@ def test_int8_gated(T, K, N):
         h = okc.int8_gated(x, w, out_f32=out_f32)
         _close(h, *_gated_ref(q, scale, w, h.dtype), f"f32 {out_f32}")
     assert torch.equal(h, okc.int8_gated(okc.quantize_rows(x), w, out_f32=True))
-    assert okc.int8_status() == (0, 0)
+    assert okc.dense_status() == (0, 0)
 
 
 def test_gated_far_tails():
@@ -340,7 +342,8 @@ def _check_norm(res, blk, out, **kw):
     return r, x
 
 
-@pytest.mark.parametrize("T,H", [(1, 1), (1, 4096), (2, 63), (7, 1000), (33, 5120), (3, 16384), (2, 16383), (300, 2048), (297, 2056), (310, 6500), (500, 8200), (298, 12289)])
+@pytest.mark.parametrize("T,H", [(1, 1), (1, 4096), (2, 63), (7, 1000), (33, 5120), (3, 16384), (2, 16383), (300, 2048), (297, 2056), (310, 6500), (500, 8200), (298, 12289),
+                                 (593, 8), (600, 2040), (700, 5120), (597, 8192), (599, 12296)])
 @pytest.mark.parametrize("res,blk", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)])
 def test_block_norm(T, H, res, blk):
     g = _gen(T * H + 1)
@@ -364,6 +367,15 @@ def test_block_norm_strides_in_place_and_unaligned():
         _check_norm(res, blk, "f32", post_gain=gain[:H], pre_gain=gain[1:], gate=wide[:T, -1:])
         _check_norm(res, blk, "int8", post_gain=gain[1:], pre_gain=gain[:H], gate=wide[2:, 5:5 + H])
     _check_norm(wide.t()[:H, :T], wide.t()[:H, 1:T + 1], "bf16", pre_gain=gain[:T].contiguous())
+    # many rows in place, each copied ahead of its turn: the same bits as out of place, twice over
+    for dtype in (torch.float32, torch.bfloat16):
+        many, blk = _randn((2000, H), g, dtype), _randn((2000, H), g, dtype)
+        first, x = okc.block_norm(many, blk, pre_gain=gain[:H], post_gain=gain[:H], gate=many, out="int8")
+        second, x2 = okc.block_norm(first, blk, pre_gain=gain[:H], post_gain=gain[:H], gate=first, out="int8")
+        store = many.clone()
+        for want, wx in ((first, x), (second, x2)):
+            _, y = okc.block_norm(store, blk, pre_gain=gain[:H], post_gain=gain[:H], gate=store, out="int8", residual_out=store)
+            assert torch.equal(store, want) and torch.equal(y.q, wx.q) and torch.equal(y.scale, wx.scale)
     # in place: the same bits as out of place (from the same addresses: the order of a row's sum goes by its alignment),
     # the columns and rows around them untouched
     store = wide.clone()
@@ -380,10 +392,11 @@ def test_block_norm_strides_in_place_and_unaligned():
     assert torch.equal(okc.block_norm(same, same, post_gain=gain[:H], residual_out=same)[0], okc.block_norm(blk, blk.clone(), post_gain=gain[:H])[0])
 
 
-def test_block_norm_special_rows():
+@pytest.mark.parametrize("T", [9, 640])
+def test_block_norm_special_rows(T):
     """Rows of zeros, the largest values, infinities and NaN: what the formula gives, each in its own row only."""
     g = _gen(10)
-    T, H = 9, 520
+    H = 520
     r, y = _randn((T, H), g), _randn((T, H), g)
     gain = torch.ones(H, device="cuda")
     r[0] = y[0] = 0
@@ -413,10 +426,10 @@ def _calls(seed):
     def run(r, T):
         r2, x = okc.block_norm(r[:T], r[:T].flip(0).contiguous(), post_gain=gain, pre_gain=gain, out="int8")
         return r2, x.q, x.scale, okc.int8_ffn(x, w13, w2), okc.int8_linear(r[:T], w13, out_f32=True)
-    return run, _randn((400, 192), g)
+    return run, _randn((900, 192), g)
 
 
-@pytest.mark.parametrize("T", [1, 30, 400])
+@pytest.mark.parametrize("T", [1, 30, 400, 900])
 def test_captured_graphs_replay_on_new_inputs_and_side_by_side(T):
     run, r = _calls(T)
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
@@ -443,7 +456,7 @@ def test_captured_graphs_replay_on_new_inputs_and_side_by_side(T):
             assert all(torch.equal(a, b) for a, b in zip(o, w))
 
 
-@pytest.mark.parametrize("T", [5, 100, 400])
+@pytest.mark.parametrize("T", [5, 100, 400, 900])
 def test_two_streams_at_once_and_back_to_back_calls(T):
     run, r = _calls(T + 1)
     others = [_randn(r.shape, _gen(k)) for k in range(8)]
@@ -457,7 +470,7 @@ def test_two_streams_at_once_and_back_to_back_calls(T):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
-    assert okc.int8_status() == (0, 0)
+    assert okc.dense_status() == (0, 0)
 
 
 def test_one_token_sequence_after_sequence_reuses_memory_safely():
