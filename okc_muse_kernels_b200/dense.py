@@ -17,6 +17,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
+from ._lib import pack_block_norm as _pack_block_norm, pack_int8 as _pack_int8
 
 __all__ = ["QuantRows", "quantize_rows", "int8_rows", "int8_linear", "int8_gated", "int8_ffn", "block_norm", "dense_status"]
 
@@ -53,20 +54,21 @@ _current_device = torch._C._cuda_getDevice           # (a CUDA tensor is at hand
 _empty = torch.empty_strided                         # the cheapest of torch's ways to uninitialised memory
 
 
-def _call(fn, name: str, dev: int, *args) -> None:
+def _call(fn, name: str, dev: int, args) -> None:
     """The C entry on the tensors' device (made current for the call if it is not) and its current stream."""
     if _current_device() == dev:
-        rc = fn(*args, _raw_stream(dev))
+        rc = fn(args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
+            rc = fn(args, _raw_stream(dev))
     if rc:
         _lib.check(rc, name)
 
 
 def _rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]:
     """bf16 or f32 rows with contiguous columns (a copy if need be): tensor, rows, columns, row stride."""
-    if t.dim() != 2 or (t.dtype is not _BF16 and t.dtype is not _F32):
+    dtype = t.dtype
+    if (dtype is not _BF16 and dtype is not _F32) or t.dim() != 2:
         raise ValueError(f"{what} must be bf16 or f32 [rows, columns]")
     R, cols = t.shape
     stride, one = t.stride()
@@ -127,8 +129,8 @@ def quantize_rows(x: torch.Tensor) -> QuantRows:
     q = _empty_rows(x, R, cols)
     scale = _empty((R,), (1,), dtype=_F32, device=x.device)
     if R:
-        _call(_lib.lib().okc_moe_quantize_rows, "okc_moe_quantize_rows", dev, x.data_ptr(), _ROWS_KIND[x.dtype],
-              stride, R, cols, q.data_ptr(), max(q.stride(0), cols), scale.data_ptr())
+        args = x.data_ptr(), _ROWS_KIND[x.dtype], stride, R, cols, q.data_ptr(), max(q.stride(0), cols), scale.data_ptr()
+        _call(lambda a, stream: _lib.lib().okc_moe_quantize_rows(*a, stream), "okc_moe_quantize_rows", dev, args)
     return QuantRows(q, scale)
 
 
@@ -143,50 +145,62 @@ def int8_rows(q: torch.Tensor, scale: torch.Tensor) -> QuantRows:
     return QuantRows(rows, scale.contiguous())
 
 
-def _check_quant(rows, what: str) -> tuple[torch.Tensor, torch.Tensor, int, int, int]:
-    """int8 tensor, scales, rows, columns and the row stride to pass on."""
+def _check_quant(rows, what: str) -> tuple:
+    """int8 tensor, its device, address, rows, columns and row stride to pass on, scales, their address."""
     q, scale = rows
-    if q.dtype is not _I8 or q.dim() != 2 or scale.dtype is not _F32 or scale.dim() != 1 or scale.shape[0] != q.shape[0]:
+    try:
+        R, cols = q.shape
+        n, = scale.shape
+        ok = n == R and q.dtype is _I8 and scale.dtype is _F32
+    except ValueError:
+        ok = False
+    if not ok:
         raise ValueError(f"{what} must be int8 [rows, columns] with f32 [rows] scales")
-    R, cols = q.shape
     stride, one = q.stride()
     if R <= 1:
-        stride = (cols + 15) // 16 * 16
-    if (one != 1 and cols > 1) or stride < cols or stride % 16 or q.data_ptr() % 16:
+        stride = cols + 15 & -16
+    ptr = q.data_ptr()
+    if (one != 1 and cols > 1) or stride < cols or (stride | ptr) & 15:
         raise ValueError(f"{what} needs rows that start on 16-byte boundaries: lay them out with int8_rows() once")
-    return q, scale if scale.is_contiguous() else scale.contiguous(), R, cols, stride
+    dev = q.get_device()
+    if scale.get_device() != dev:
+        raise ValueError(f"{what}: int8 values on {q.device} and scales on {scale.device}")
+    if not scale.is_contiguous():
+        scale = scale.contiguous()
+    return q, dev, ptr, R, cols, stride, scale, scale.data_ptr()
 
 
 def _product(name: str, x, weight, bias, out_f32: bool, out, halves: int) -> torch.Tensor:
-    w, w_scale, N, K, w_stride = _check_quant(weight, "weight")
+    w, dev, w_ptr, N, K, w_stride, w_scale, ws_ptr = _check_quant(weight, "weight")
     if N < halves or N % halves:
         raise ValueError("a gated weight holds the gate rows and then as many up rows" if halves == 2 else "weight has no rows")
     N //= halves
     if isinstance(x, tuple):
-        x, x_scale, T, cols, x_stride = _check_quant(x, "x")
-        xs_ptr, scratch = x_scale.data_ptr(), 0
+        x, x_dev, x_ptr, T, cols, x_stride, x_scale, xs_ptr = _check_quant(x, "x")
+        kind, scratch = 2, 0
     else:
         x, T, cols, x_stride = _rows(x, "x")
-        x_scale, xs_ptr, scratch = None, 0, T > INT8_FEW_TOKENS
+        x_dev, x_ptr, kind, x_scale, xs_ptr, scratch = x.get_device(), x.data_ptr(), _ROWS_KIND[x.dtype], None, 0, T > INT8_FEW_TOKENS
     if cols != K or K < 1 or K > INT8_MAX_K:
         raise ValueError(f"x has {cols} columns and weight {K}; 1 to {INT8_MAX_K}, and as many in both")
-    dev = _device(x, x_scale, w, w_scale, bias, out)
-    bias = _vector(bias, N, "bias")
+    if x_dev != dev or dev < 0 or bias is not None or out is not None:
+        _device(x, w, bias, out)
+    device, bias_ptr = x.device, 0
+    if bias is not None:
+        bias = _vector(bias, N, "bias")
+        bias_ptr = bias.data_ptr()
     if out is None:
-        out, out_stride = _empty((T, N), (N, 1), dtype=_F32 if out_f32 else _BF16, device=x.device), N
+        out, out_stride = _empty((T, N), (N, 1), dtype=_F32 if out_f32 else _BF16, device=device), N
     else:
         out_stride = _check_out(out, T, N, _F32 if out_f32 else _BF16, "out", (x, x_scale, w, w_scale, bias))
     if T == 0:
         return out
+    scratch_ptr = 0
     if scratch:      # int8 rows and scales of the tokens: okc_moe_int8_scratch_bytes
-        n = T * ((K + 15) // 16 * 16 + 4)
-        scratch = _empty((n,), (1,), dtype=_I8, device=x.device)
-        xs = scratch.data_ptr()
-    else:
-        xs = 0
-    _call(getattr(_lib.lib(), name), name, dev, _lib.pack_int8(
-        x.data_ptr(), xs_ptr, w.data_ptr(), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), xs,
-        x_stride, w_stride, out_stride, _ROWS_KIND[x.dtype], out_f32, T, K, N))
+        scratch = _empty((T * ((K + 15 & -16) + 4),), (1,), dtype=_I8, device=device)
+        scratch_ptr = scratch.data_ptr()
+    _call(getattr(_lib.lib(), name), name, dev, _pack_int8(
+        x_ptr, xs_ptr, w_ptr, ws_ptr, bias_ptr, out.data_ptr(), scratch_ptr, x_stride, w_stride, out_stride, kind, out_f32, T, K, N))
     return out
 
 
@@ -283,7 +297,7 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
         else:
             x, x_stride = _empty((T, H), (H, 1), dtype=kind_of_x, device=res.device), H
     if T:
-        _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, _lib.pack_block_norm(
+        _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, _pack_block_norm(
             res.data_ptr(), blk_ptr, gate.data_ptr() if kind else 0,
             0 if post_gain is None else post_gain.data_ptr(), 0 if pre_gain is None else pre_gain.data_ptr(),
             new.data_ptr() if blk_ptr else 0, 0 if x is None else x.data_ptr(), 0 if scale is None else scale.data_ptr(),
