@@ -325,8 +325,8 @@ int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t ro
  * out[t][n] = (sum_k x[t][k] * w[n][k]) * (x_scale[t] * w_scale[n]) + bias[n]              (okc_moe_int8_linear)
  * out[t][i] = g / (1 + exp(-g)) * u with g, u = that sum for rows i and n + i of w          (okc_moe_int8_gated)
  * w: int8, n rows (gated: 2 n, gate rows first), 16-byte aligned, w_stride a multiple of 16; the bytes between k and
- * w_stride are not used.  x: int8 rows aligned the same way with x_scale, or bf16 / f32 rows, which are quantised as
- * okc_moe_quantize_rows does, into `scratch` (okc_moe_int8_scratch_bytes; up to 8 tokens need none).  k <= 131071.
+ * w_stride are not used (those up to the next multiple of 16 may be read).  x: int8 rows aligned the same way with x_scale, or bf16 / f32 rows, which are quantised as
+ * okc_moe_quantize_rows does, into `scratch` (okc_moe_int8_scratch_bytes; one token with k <= 16384 needs none).  k <= 131071.
  * The result of a token does not depend on the tokens beside it, bit for bit.
  */
 typedef struct okc_int8_args {

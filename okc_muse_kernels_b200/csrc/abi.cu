@@ -686,7 +686,7 @@ int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t ro
 static uint64_t int8_row_bytes(int K) { return (static_cast<uint64_t>(K) + 15) / 16 * 16; }
 
 uint64_t okc_moe_int8_scratch_bytes(int x_kind, int32_t tokens, int32_t k) {
-  if (x_kind == kRowsInt8 || tokens <= kInt8FewTokens || k <= 0) return 0;
+  if (x_kind == kRowsInt8 || k <= 0 || (tokens == 1 && k <= kInt8OneMaxK)) return 0;
   return static_cast<uint64_t>(tokens) * (int8_row_bytes(k) + 4);
 }
 
@@ -699,8 +699,8 @@ static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_
   if (!a->x || !a->w || !a->w_scale || !a->out || (gated && a->bias)) return OKC_ERR_BAD_ARG;
   if (a->w_stride < K || (a->w_stride % 16) != 0 || !aligned(a->w, 16) || (T > 1 && (a->x_stride < K || a->out_stride < N))) return OKC_ERR_BAD_ARG;
   if (a->x_kind == kRowsInt8 && (!a->x_scale || !aligned(a->x, 16) || a->x_stride < K || (a->x_stride % 16) != 0)) return OKC_ERR_BAD_ARG;
-  const bool few = T <= kInt8FewTokens;
-  if (!few && a->x_kind != kRowsInt8 && (!a->scratch || !aligned(a->scratch, 16))) return OKC_ERR_BAD_ARG;
+  const bool one = T == 1 && K <= kInt8OneMaxK;
+  if (!one && a->x_kind != kRowsInt8 && (!a->scratch || !aligned(a->scratch, 16))) return OKC_ERR_BAD_ARG;
   if (!is_sm100()) return OKC_ERR_NO_DEVICE;
   Int8Params p;
   p.x = a->x; p.x_scale = a->x_scale; p.w = static_cast<const int8_t*>(a->w); p.w_scale = a->w_scale; p.bias = a->bias; p.out = a->out;
@@ -709,7 +709,7 @@ static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_
   p.out_f32 = a->out_f32 ? 1 : 0;
   p.out_vec = rows_vec(p.out, p.out_stride, T, p.out_f32 ? 4 : 2) ? 1 : 0;
   p.T = T; p.K = K; p.N = N;
-  if (few) return launch_int8_few(p, gated, stream) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
+  if (one) return launch_int8_one(p, gated, stream) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
   bool pdl = false;
   if (p.x_kind != kRowsInt8) {
     const int64_t q_stride = static_cast<int64_t>(int8_row_bytes(K));

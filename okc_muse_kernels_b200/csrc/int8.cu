@@ -5,8 +5,8 @@
 // below turns it into the result with the same f32 operations: a token's bits do not depend on the batch it is in.
 //
 // Three kernels, by what bounds the product:
-//   okc_int8_few   up to 8 tokens   the weights are read once by plain 16-byte loads and multiplied on the integer
-//                                   dot-product units; the token rows are quantised in the kernel (one launch)
+//   okc_int8_one   one token        the weights are read by plain 16-byte loads and multiplied on the integer dot-product
+//                                   units; the token is quantised in the kernel (one launch)
 //   okc_int8_mid   some hundred     the weights fill M of a tcgen05.mma (kind::i8), the tokens are N; K is split over a
 //                                   cluster of CTAs that add their integer sums through distributed shared memory
 //   okc_int8_many  beyond           CTA pairs (cta_group::2) on tiles of 256 tokens x up to 256 weight rows, persistent
@@ -25,163 +25,160 @@ __device__ int32_t g_int8_status;      // code of the first wait that ran out si
 __device__ __forceinline__ float int8_value(int acc, float sx, float sw) { return __fmul_rn(__int2float_rn(acc), __fmul_rn(sx, sw)); }
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fmul_rn(__fdividef(g, 1.f + __expf(-g)), u); }
 
-// ------------------------------------------------------------------ few tokens
-constexpr int kFewThreads = 1024;
-constexpr int kFewChunk = 512;         // K elements of one warp-wide 16-byte load
-constexpr int kFewRowsMax = 512;       // most weight rows a CTA owns (its integer sums live in shared memory)
+__device__ __forceinline__ void store_out(const Int8Params& p, int64_t o, float v) {
+  if (p.out_f32) static_cast<float*>(p.out)[o] = v;
+  else static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v);
+}
 
-// Sixteen values of a token row at column k (zeros past K), as f32.
-__device__ __forceinline__ void few_load_x(const Int8Params& p, int t, int k, float (&v)[16]) {
-  const int64_t o = t * p.x_stride + k;
-  if (p.x_vec && k + 16 <= p.K) {
+// ------------------------------------------------------------------ one token
+constexpr int kOneThreads = 512;
+constexpr int kOneChunk = 512;         // K elements of one warp-wide 16-byte load
+constexpr int kOneRowsMax = 1024;      // most weight rows a CTA owns (its integer sums live in shared memory, with the token)
+
+// Eight values of the token at column i (zeros past K), as f32.
+__device__ __forceinline__ void one_load_x(const Int8Params& p, int i, float (&v)[8]) {
+  if (p.x_vec && i + 8 <= p.K) {
     if (p.x_kind == kRowsF32) {
-      const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + o);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) { const float4 a = s[j]; v[4 * j] = a.x; v[4 * j + 1] = a.y; v[4 * j + 2] = a.z; v[4 * j + 3] = a.w; }
+      const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p.x) + i);
+      const float4 a = s[0], b = s[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
-      const uint4* s = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + o);
-      float a[8], b[8];
-      unpack_bf16x8(s[0], a); unpack_bf16x8(s[1], b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) { v[j] = a[j]; v[8 + j] = b[j]; }
+      unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + i), v);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 8; ++j) {
       v[j] = 0.f;
-      if (k + j < p.K)
-        v[j] = p.x_kind == kRowsF32 ? static_cast<const float*>(p.x)[o + j]
-                                    : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p.x)[o + j]) << 16);
+      if (i + j < p.K)
+        v[j] = p.x_kind == kRowsF32 ? static_cast<const float*>(p.x)[i + j]
+                                    : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(p.x)[i + j]) << 16);
     }
   }
 }
-// Sixteen int8 values at column k of an aligned row, zeros past K (the bytes behind a row's end are never used).
-__device__ __forceinline__ uint4 load_q16(const int8_t* row, int k, int K) {
-  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (k + j < K) w[j >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + j])) << (8 * (j & 3));
-  return make_uint4(w[0], w[1], w[2], w[3]);
+// 16 bytes that are read once: past L1.
+__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
 }
 
-// A CTA owns `rows_per_cta` neighbouring outputs and all of K.  A warp keeps one 512-wide chunk of K: its 16 bytes of
-// every token row stay in registers (quantised there), and it walks over the CTA's weight rows with one 16-byte load a
-// lane and row; `kTok` integer dot products, a warp sum each, and one shared-memory add.  With all 32 warps loading
-// four rows ahead an SM has 64 KB in flight, above what the HBM rate needs.
-template <int kTok, bool kGated>
-__global__ void __launch_bounds__(kFewThreads) okc_int8_few(const Int8Params p, int rows_per_cta) {
-  extern __shared__ int few_acc[];      // [rows][kTok]
-  __shared__ uint32_t amax_s[kTok];
+// A CTA owns `rows_per_cta` neighbouring outputs and all of K.  Its threads quantise the token into shared memory (every
+// CTA the whole row: a few KB from L2, where another launch would take longer); a warp then keeps one 512-wide chunk of K,
+// its 16 bytes of the token in registers, and walks over the CTA's weight rows with one 16-byte load a lane and row, four
+// integer dot products, a warp sum, and one shared-memory add for eight rows.  Sixteen rows a warp are on their way at any
+// time (128 KB an SM), the first ones before the token has been looked at.  The 16 bytes at a row's end may reach past K,
+// never past the row's next 16-byte boundary; the token's bytes are zero there.
+// bf16 token, weights of three layers in turn: K = 4096, N = 4096 5.7 us (the quantiser and okc_int8_mid: 7.4), gated,
+// K = 7168, 2 x 2048 rows 8.2 (8.7); a token of 128 columns alone takes 4.5: launch, three dependent trips to memory.
+template <bool kGated>
+__global__ void __launch_bounds__(kOneThreads) okc_int8_one(const Int8Params p, int rows_per_cta) {
+  extern __shared__ __align__(16) uint8_t one_smem[];
+  constexpr int kWarps = kOneThreads / 32, kAhead = 8;
+  __shared__ uint32_t amax_s[kWarps];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kpad = (p.K + 15) & ~15;
+  uint8_t* const xq_s = one_smem;                            // [kpad] int8
+  int* const acc_s = reinterpret_cast<int*>(one_smem + kpad);     // [rows]
   const int n0 = blockIdx.x * rows_per_cta;
   const int nr = min(rows_per_cta, p.N - n0);
   const int rows = kGated ? 2 * nr : nr;
-  const int chunks = (p.K + kFewChunk - 1) / kFewChunk;
-  const int groups = chunks >= 32 ? 1 : 32 / chunks;
-  const int group = chunks >= 32 ? 0 : warp / chunks;
-  for (int i = tid; i < rows * kTok; i += kFewThreads) few_acc[i] = 0;
-  if (tid < kTok) amax_s[tid] = 0;
-  __syncthreads();
+  const int chunks = (p.K + kOneChunk - 1) / kOneChunk;
+  const int step = min(chunks, kWarps);            // chunks under way at once
+  const int groups = kWarps / step;                // warps that share a chunk and take turns at its rows
+  const int group = warp / step;
+  int c = group < groups ? warp % step : chunks;
+  int k = c * kOneChunk + lane * 16;
+  auto load = [&](uint4 (&w)[kAhead], int r0) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int r = r0 + u * groups;
+      w[u] = make_uint4(0, 0, 0, 0);
+      if (r < rows && k < p.K) w[u] = ldg_stream(p.w + (!kGated || r < nr ? n0 + r : p.N + n0 + r - nr) * p.w_stride + k);
+    }
+  };
+  uint4 wa[kAhead], wb[kAhead];
+  load(wa, group);
+  load(wb, group + kAhead * groups);
+  // scales of the output this thread finishes first (most CTAs have no more outputs than threads)
+  const int n_mine = n0 + tid % nr;
+  const float sw_mine = p.w_scale[n_mine], su_mine = kGated ? p.w_scale[p.N + n_mine] : 0.f;
 
-  const bool raw = p.x_kind != kRowsInt8;
-  if (raw) {
-    if (group == 0)
-      for (int c = warp; c < chunks; c += 32) {
-        const int k = c * kFewChunk + lane * 16;
+  RowScale rs;
+  if (p.x_kind != kRowsInt8) {
+    uint32_t m = 0;
+    for (int i = tid * 8; i < p.K; i += kOneThreads * 8) {
+      float v[8];
+      one_load_x(p, i, v);
 #pragma unroll
-        for (int t = 0; t < kTok; ++t) {
-          uint32_t m = 0;
-          if (t < p.T && k < p.K) {
-            float v[16];
-            few_load_x(p, t, k, v);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) m = max(m, abs_bits(v[j]));
-          }
-          m = __reduce_max_sync(0xffffffffu, m);
-          if (lane == 0) atomicMax(&amax_s[t], m);
-        }
-      }
+      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) amax_s[warp] = m;
     __syncthreads();
+    rs = row_scale(__reduce_max_sync(0xffffffffu, amax_s[lane % kWarps]));
+    for (int i = tid * 8; i < kpad; i += kOneThreads * 8) {
+      float v[8];
+      one_load_x(p, i, v);
+      *reinterpret_cast<uint2*>(xq_s + i) = make_uint2(quant8x4(v[0], v[1], v[2], v[3], rs), quant8x4(v[4], v[5], v[6], v[7], rs));
+    }
+  } else {
+    rs.scale = p.x_scale[0];
+    for (int i = tid * 4; i < kpad; i += kOneThreads * 4) {
+      uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const int8_t*>(p.x) + i);
+      if (i + 4 > p.K) w = i < p.K ? w & ((1u << (8 * (p.K - i))) - 1u) : 0u;
+      *reinterpret_cast<uint32_t*>(xq_s + i) = w;
+    }
   }
-  if (group < groups) {
-    for (int c = chunks >= 32 ? warp : warp % chunks; c < chunks; c += chunks >= 32 ? 32 : chunks) {
-      const int k = c * kFewChunk + lane * 16;
-      uint4 xq[kTok];
+  for (int i = tid; i < rows; i += kOneThreads) acc_s[i] = 0;
+  __syncthreads();
+  for (; c < chunks; c += step) {
+    const uint4 xq = k < p.K ? *reinterpret_cast<const uint4*>(xq_s + k) : make_uint4(0, 0, 0, 0);
+    auto use = [&](const uint4 (&w)[kAhead], int r0) {
+      if (r0 >= rows) return;
+      int mine = 0;
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        xq[t] = make_uint4(0, 0, 0, 0);
-        if (t < p.T && k < p.K) {
-          if (raw) {
-            float v[16];
-            few_load_x(p, t, k, v);
-            const RowScale rs = row_scale(amax_s[t]);
-            xq[t].x = quant8x4(v[0], v[1], v[2], v[3], rs);
-            xq[t].y = quant8x4(v[4], v[5], v[6], v[7], rs);
-            xq[t].z = quant8x4(v[8], v[9], v[10], v[11], rs);
-            xq[t].w = quant8x4(v[12], v[13], v[14], v[15], rs);
-          } else {
-            xq[t] = load_q16(static_cast<const int8_t*>(p.x) + t * p.x_stride, k, p.K);
-          }
-        }
+      for (int u = 0; u < kAhead; ++u) {
+        int d = __dp4a(static_cast<int>(w[u].x), static_cast<int>(xq.x), 0);
+        d = __dp4a(static_cast<int>(w[u].y), static_cast<int>(xq.y), d);
+        d = __dp4a(static_cast<int>(w[u].z), static_cast<int>(xq.z), d);
+        d = __dp4a(static_cast<int>(w[u].w), static_cast<int>(xq.w), d);
+        d = __reduce_add_sync(0xffffffffu, d);
+        if (lane == u) mine = d;
       }
-      for (int r0 = group; r0 < rows; r0 += 4 * groups) {
-        uint4 w[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = r0 + u * groups;
-          w[u] = make_uint4(0, 0, 0, 0);
-          if (r < rows && k < p.K) {
-            const int n = kGated ? (r < nr ? n0 + r : p.N + n0 + r - nr) : n0 + r;
-            w[u] = load_q16(p.w + n * p.w_stride, k, p.K);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = r0 + u * groups;
-          if (r >= rows) break;
-          int mine = 0;
-#pragma unroll
-          for (int t = 0; t < kTok; ++t) {
-            int d = __dp4a(static_cast<int>(w[u].x), static_cast<int>(xq[t].x), 0);
-            d = __dp4a(static_cast<int>(w[u].y), static_cast<int>(xq[t].y), d);
-            d = __dp4a(static_cast<int>(w[u].z), static_cast<int>(xq[t].z), d);
-            d = __dp4a(static_cast<int>(w[u].w), static_cast<int>(xq[t].w), d);
-            d = __reduce_add_sync(0xffffffffu, d);
-            if (lane == t) mine = d;
-          }
-          if (lane < kTok) atomicAdd(&few_acc[r * kTok + lane], mine);
-        }
-      }
+      const int r = r0 + lane * groups;
+      if (lane < kAhead && r < rows) atomicAdd(&acc_s[r], mine);
+    };
+    for (int r0 = group; r0 < rows; r0 += 2 * kAhead * groups) {
+      use(wa, r0);
+      load(wa, r0 + 2 * kAhead * groups);
+      use(wb, r0 + kAhead * groups);
+      load(wb, r0 + 3 * kAhead * groups);
+    }
+    k += step * kOneChunk;                                   // the next chunk of K, if this warp has one
+    if (c + step < chunks) {
+      load(wa, group);
+      load(wb, group + kAhead * groups);
     }
   }
   __syncthreads();
-  for (int i = tid; i < nr * p.T; i += kFewThreads) {
-    const int t = i / nr, j = i - t * nr, n = n0 + j;
-    const float sx = raw ? row_scale(amax_s[t]).scale : p.x_scale[t];
-    float v = int8_value(few_acc[j * kTok + t], sx, p.w_scale[n]);
-    if (kGated) v = silu_mul(v, int8_value(few_acc[(nr + j) * kTok + t], sx, p.w_scale[p.N + n]));
+  for (int j = tid; j < nr; j += kOneThreads) {
+    const int n = n0 + j;
+    const bool first = j == tid;       // (n_mine is this output's column then)
+    float v = int8_value(acc_s[j], rs.scale, first ? sw_mine : p.w_scale[n]);
+    if (kGated) v = silu_mul(v, int8_value(acc_s[nr + j], rs.scale, first ? su_mine : p.w_scale[p.N + n]));
     else if (p.bias) v = __fadd_rn(v, p.bias[n]);
-    if (p.out_f32) static_cast<float*>(p.out)[t * p.out_stride + n] = v;
-    else static_cast<__nv_bfloat16*>(p.out)[t * p.out_stride + n] = __float2bfloat16_rn(v);
+    store_out(p, n, v);
   }
 }
 
-static int few_tok(int T) { return T <= 1 ? 1 : T <= 2 ? 2 : T <= 4 ? 4 : 8; }
-
-cudaError_t launch_int8_few(const Int8Params& p, bool gated, cudaStream_t stream) {
+cudaError_t launch_int8_one(const Int8Params& p, bool gated, cudaStream_t stream) {
   int rpc = (p.N + 147) / 148;
-  const int most = gated ? kFewRowsMax / 2 : kFewRowsMax;
+  const int most = gated ? kOneRowsMax / 2 : kOneRowsMax;
   if (rpc > most) rpc = most;
-  const int tok = few_tok(p.T);
-  const size_t smem = static_cast<size_t>(gated ? 2 : 1) * rpc * tok * sizeof(int);
-  const dim3 grid((p.N + rpc - 1) / rpc), block(kFewThreads);
-#define OKC_FEW(TOK) return gated ? launch_kernel(okc_int8_few<TOK, true>, grid, block, smem, stream, false, p, rpc) : launch_kernel(okc_int8_few<TOK, false>, grid, block, smem, stream, false, p, rpc)
-  if (tok == 1) OKC_FEW(1);
-  if (tok == 2) OKC_FEW(2);
-  if (tok == 4) OKC_FEW(4);
-  OKC_FEW(8);
-#undef OKC_FEW
+  const size_t smem = static_cast<size_t>(gated ? 2 : 1) * rpc * sizeof(int) + static_cast<size_t>((p.K + 15) & ~15);     // at most 20 KB
+  const dim3 grid((p.N + rpc - 1) / rpc), block(kOneThreads);
+  return gated ? launch_kernel(okc_int8_one<true>, grid, block, smem, stream, false, p, rpc)
+               : launch_kernel(okc_int8_one<false>, grid, block, smem, stream, false, p, rpc);
 }
 
 // ------------------------------------------------------------------ tcgen05 pieces shared by the two tiled kernels
@@ -225,11 +222,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void store_out(const Int8Params& p, int64_t o, float v) {
-  if (p.out_f32) static_cast<float*>(p.out)[o] = v;
-  else static_cast<__nv_bfloat16*>(p.out)[o] = __float2bfloat16_rn(v);
-}
-
 // ------------------------------------------------------------------ some hundred tokens
 constexpr int kMidThreads = 256;       // warps 0..3 read the accumulator, 4 TMA producer, 5 MMA issuer; all finish the rows
 constexpr int kMidMaxStages = 8;

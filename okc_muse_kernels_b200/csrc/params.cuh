@@ -159,7 +159,7 @@ cudaError_t norm_read_status(cudaStream_t stream, int32_t* code);
 
 // The int8 products (int8.cu).
 struct Int8Params {
-  const void* x;              // token rows: int8 with x_scale, or (few tokens only) bf16 / f32 rows quantised in the kernel
+  const void* x;              // token rows: int8 with x_scale, or (one token only) bf16 / f32 rows quantised in the kernel
   const float* x_scale;
   const int8_t* w;            // weight rows, K int8 values each
   const float* w_scale;       // f32, one per weight row
@@ -171,9 +171,9 @@ struct Int8Params {
   int out_f32, out_vec;       // out_vec: 16-byte stores of an output row are possible from any column that is a multiple of 8
   int T, K, N;                // N = outputs: weight rows, or half of them for the gated product
 };
-constexpr int kInt8FewTokens = 8;
+constexpr int kInt8OneMaxK = 16384;         // up to here the product of one token quantises it itself
 constexpr int kInt8MaxK = 131071;          // 128 * 128 * K stays below 2^31
-cudaError_t launch_int8_few(const Int8Params& p, bool gated, cudaStream_t stream);
+cudaError_t launch_int8_one(const Int8Params& p, bool gated, cudaStream_t stream);
 cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream);
 cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream);
 bool int8_use_many(int T, int K, int N, bool gated);

@@ -23,7 +23,7 @@ __all__ = ["QuantRows", "quantize_rows", "int8_rows", "int8_linear", "int8_gated
 
 BLOCK_NORM_MAX_HIDDEN = 16384
 INT8_MAX_K = 131071           # the integer sums stay in 32 bits
-INT8_FEW_TOKENS = 8           # up to here a product quantises its tokens itself and needs no scratch
+INT8_ONE_MAX_K = 16384        # up to here the product of one token quantises it itself and needs no scratch
 _BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
 _ROWS_KIND = {_BF16: 0, _F32: 1, _I8: 2}
 _OUT = {"bf16": (0, _BF16), "f32": (1, _F32), "int8": (2, _I8)}
@@ -180,7 +180,7 @@ def _product(name: str, x, weight, bias, out_f32: bool, out, halves: int) -> tor
         kind, scratch = 2, 0
     else:
         x, T, cols, x_stride = _rows(x, "x")
-        x_dev, x_ptr, kind, x_scale, xs_ptr, scratch = x.get_device(), x.data_ptr(), _ROWS_KIND[x.dtype], None, 0, T > INT8_FEW_TOKENS
+        x_dev, x_ptr, kind, x_scale, xs_ptr, scratch = x.get_device(), x.data_ptr(), _ROWS_KIND[x.dtype], None, 0, T > 1 or K > INT8_ONE_MAX_K
     if cols != K or K < 1 or K > INT8_MAX_K:
         raise ValueError(f"x has {cols} columns and weight {K}; 1 to {INT8_MAX_K}, and as many in both")
     if x_dev != dev or dev < 0 or bias is not None or out is not None:

@@ -122,8 +122,9 @@ def test_quantize_rows_abi_checks_and_scratch():
     assert q(rows=0) == OK and q(rows=-1) == BAD and q(cols=0) == BAD and q(cols=131072) == LARGE
     assert q(xs=63) == BAD and q(qs=63) == BAD and q(x=None) == BAD
     assert lib.okc_moe_block_norm(None, None) == BAD and lib.okc_moe_int8_linear(None, None) == BAD
-    assert lib.okc_moe_int8_scratch_bytes(0, 8, 4096) == 0 and lib.okc_moe_int8_scratch_bytes(2, 4096, 4096) == 0
-    assert lib.okc_moe_int8_scratch_bytes(1, 9, 1000) == 9 * (1008 + 4)
+    assert lib.okc_moe_int8_scratch_bytes(0, 1, 4096) == 0 and lib.okc_moe_int8_scratch_bytes(2, 4096, 4096) == 0
+    assert lib.okc_moe_int8_scratch_bytes(0, 1, dense.INT8_ONE_MAX_K) == 0 and lib.okc_moe_int8_scratch_bytes(0, 1, dense.INT8_ONE_MAX_K + 1) == 16400 + 4
+    assert lib.okc_moe_int8_scratch_bytes(1, 2, 1000) == 2 * (1008 + 4)
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="a GPU is there")

@@ -124,7 +124,7 @@ def test_quantize_rows_strided_and_unaligned_input():
 
 
 # ------------------------------------------------------------------------------------------------ products
-SHAPES = [(1, 1, 1), (1, 16, 5), (2, 511, 130), (3, 513, 7), (5, 1000, 301), (8, 4100, 149), (1, 20000, 33), (4, 16400, 64),
+SHAPES = [(1, 1, 1), (1, 16384, 40), (1, 16385, 9), (1, 9001, 1200), (1, 520, 3001), (1, 64, 160000), (2, 520, 3001), (1, 16, 5), (2, 511, 130), (3, 513, 7), (5, 1000, 301), (8, 4100, 149), (1, 20000, 33), (4, 16400, 64),
           (9, 1, 1), (9, 128, 128), (16, 129, 127), (17, 1000, 301), (40, 4096, 640), (65, 333, 1000), (130, 2048, 257), (256, 520, 384),
           (257, 17, 3), (257, 128, 256), (300, 1000, 301), (513, 2047, 129), (1025, 640, 2050)]
 
@@ -170,7 +170,7 @@ def test_gated_far_tails():
         assert torch.isfinite(h).all() and (h[1::2] == 0).all() and (h[0::2] > 1e6).all()
 
 
-@pytest.mark.parametrize("T", [3, 40, 300])
+@pytest.mark.parametrize("T", [1, 3, 40, 300])
 def test_longest_sums_stay_in_32_bits(T):
     """Every product 127 * 127 (and -128 * -128 of rows made elsewhere) over the longest K."""
     K = 131071
