@@ -117,12 +117,13 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_block_norm(const Blo
 }
 
 // The same for many rows that 16-byte accesses can reach: persistent CTAs, each with a ring of rows in shared memory that
-// bulk copies fill ahead of it, so that HBM does not wait for the two dependent sums of a row.  The gains are copied
-// once.  4096 x 5120, everything bf16, a gate per element: NORM_US us (NORM_TB TB/s); a CTA per row 65.1 us (3.2 TB/s).
-constexpr int kStreamStages = 8;
-template <int kChunks>
+// bulk copies fill ahead of it, so that HBM does not wait for the two dependent sums of a row.  What is left is issue
+// slots: pairs of f32 an instruction, and as many CTAs an SM as registers allow (the gains stay in L1, not in shared
+// memory, for that).  4096 x 5120, everything bf16, a gate per element: NORM_US us (NORM_TB TB/s); a CTA per row 65.1 us.
+constexpr int kStreamStages = 4;
+template <int kChunks, bool kInt8>
 __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream(const BlockNormParams p, int rows, int stages, int row_bytes) {
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t bar_full[kStreamStages];
   __shared__ int abort_code;
   __shared__ float red_post[2][32], red_pre[2][32];
@@ -130,17 +131,11 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
   const int tid = threadIdx.x, nt = blockDim.x, H = p.H;
   const uint32_t res_bytes = static_cast<uint32_t>(H) * (p.res_f32 ? 4 : 2), blk_bytes = static_cast<uint32_t>(H) * (p.blk_f32 ? 4 : 2);
   const bool gate_rows = p.gate && p.gate_col_stride != 0 && p.gate_stride != 0, gate_cols = p.gate && p.gate_col_stride != 0 && p.gate_stride == 0;
-  const uint32_t gate_bytes = gate_rows || gate_cols ? static_cast<uint32_t>(H) * (p.gate_f32 ? 4 : 2) : 0;
-  const uint32_t gain_bytes = static_cast<uint32_t>(H) * 4;
-  // shared memory: post gain, pre gain, channel gate (each if there), then the ring
-  uint8_t* const post_s = smem;
-  uint8_t* const pre_s = post_s + (p.post_gain ? gain_bytes : 0);
-  uint8_t* const chan_s = pre_s + (p.pre_gain ? gain_bytes : 0);
-  uint8_t* const ring = chan_s + (gate_cols ? gate_bytes : 0);
+  const uint32_t gate_bytes = gate_rows ? static_cast<uint32_t>(H) * (p.gate_f32 ? 4 : 2) : 0;
   auto fetch = [&](int row, int st) {
     const uint32_t bar = smem_u32(&bar_full[st]);
-    uint32_t dst = smem_u32(ring) + st * row_bytes;
-    mbar_expect_tx(bar, res_bytes + blk_bytes + (gate_rows ? gate_bytes : 0));
+    const uint32_t dst = smem_u32(ring) + st * row_bytes;
+    mbar_expect_tx(bar, res_bytes + blk_bytes + gate_bytes);
     bulk_g2s(dst, static_cast<const uint8_t*>(p.res) + row * p.res_stride * (p.res_f32 ? 4 : 2), res_bytes, bar);
     bulk_g2s(dst + res_bytes, static_cast<const uint8_t*>(p.blk) + row * p.blk_stride * (p.blk_f32 ? 4 : 2), blk_bytes, bar);
     if (gate_rows) bulk_g2s(dst + res_bytes + blk_bytes, static_cast<const uint8_t*>(p.gate) + row * p.gate_stride * (p.gate_f32 ? 4 : 2), gate_bytes, bar);
@@ -151,21 +146,12 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     mbar_fence_init();
     for (int i = 0; i < stages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
   }
-  for (int i = tid * 4; i < H; i += nt * 4) {
-    if (p.post_gain) *reinterpret_cast<float4*>(post_s + i * 4) = *reinterpret_cast<const float4*>(p.post_gain + i);
-    if (p.pre_gain) *reinterpret_cast<float4*>(pre_s + i * 4) = *reinterpret_cast<const float4*>(p.pre_gain + i);
-  }
-  if (gate_cols)
-    for (uint32_t i = tid * 16; i < gate_bytes; i += nt * 16)
-      *reinterpret_cast<uint4*>(chan_s + i) = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.gate) + i);
   __syncthreads();
+  const float over_h = 1.f / static_cast<float>(H);
+  const F2 res_scale = f2_pack(p.res_scale, p.res_scale);
   int st = 0, n = 0;
   uint32_t ph = 0;
   for (int row = blockIdx.x; row < rows; row += gridDim.x, ++n) {
-    // a wait that runs out does not leave the loop (the other threads count on this one's barriers): the row's result is
-    // then undefined and the status word says so
-    mbar_wait(smem_u32(&bar_full[st]), ph, &abort_code, 0x81);
-    const uint8_t* const src = ring + st * row_bytes;
     float mul = p.blk_scale;
     if (p.gate && p.gate_col_stride == 0) {
       const int64_t o = row * p.gate_stride;
@@ -174,82 +160,129 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
       if (p.gate_sigmoid) g = 1.f / (1.f + __expf(-g));
       mul *= g;
     }
-    float r[kChunks][8];
+    // a wait that runs out does not leave the loop (the other threads count on this one's barriers): the row's result is
+    // then undefined and the status word says so
+    mbar_wait(smem_u32(&bar_full[st]), ph, &abort_code, 0x81);
+    const uint8_t* const src = ring + st * row_bytes;
+    F2 r[kChunks][4];
     {
-      float y[kChunks][8];
+      F2 y[kChunks][4];
 #pragma unroll
-      for (int j = 0; j < kChunks; ++j) load_chunk<true>(src + res_bytes, p.blk_f32, j, tid, nt, H, y[j]);
+      for (int j = 0; j < kChunks; ++j) {
+        const int c = (j * nt + tid) * 8;
+        y[j][0] = y[j][1] = y[j][2] = y[j][3] = 0ull;
+        if (c < H) load8_f2(src + res_bytes, p.blk_f32, c, y[j]);
+      }
       if (p.post_gain) {
-        float ss = 0.f;
+        F2 sum = 0ull;
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(y[j][e], y[j][e], ss);
-        const float rstd = rsqrtf(cta_sum(ss, red_post[n & 1]) / static_cast<float>(H) + p.eps);
+          for (int e = 0; e < 4; ++e) sum = f2_fma(y[j][e], y[j][e], sum);
+        float lo, hi;
+        f2_unpack(sum, lo, hi);
+        const float rstd = rsqrtf(cta_sum(lo + hi, red_post[n & 1]) * over_h + p.eps);
+        const F2 rstd2 = f2_pack(rstd, rstd);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
-          float g[8];
-          load_chunk<true>(post_s, true, j, tid, nt, H, g);
+          const int c = (j * nt + tid) * 8;
+          if (c < H) {
+            F2 g[4];
+            load8_f2(p.post_gain, true, c, g);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[j][e] = y[j][e] * rstd * g[e];
+            for (int e = 0; e < 4; ++e) y[j][e] = f2_mul(f2_mul(y[j][e], rstd2), g[e]);
+          }
         }
       }
-      if (p.gate && p.gate_col_stride != 0) {
-        const uint8_t* gsrc = gate_rows ? src + res_bytes + blk_bytes : chan_s;
+      if (gate_rows || gate_cols) {
+        const void* gsrc = gate_rows ? static_cast<const void*>(src + res_bytes + blk_bytes) : p.gate;
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
-          float g[8];
-          load_chunk<true>(gsrc, p.gate_f32, j, tid, nt, H, g);
+          const int c = (j * nt + tid) * 8;
+          if (c < H) {
+            F2 g[4];
+            load8_f2(gsrc, p.gate_f32, c, g);
+            if (p.gate_sigmoid) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[j][e] *= p.gate_sigmoid ? 1.f / (1.f + __expf(-g[e])) : g[e];
+              for (int e = 0; e < 4; ++e) {
+                float lo, hi;
+                f2_unpack(g[e], lo, hi);
+                g[e] = f2_pack(1.f / (1.f + __expf(-lo)), 1.f / (1.f + __expf(-hi)));
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[j][e] = f2_mul(y[j][e], g[e]);
+          }
         }
       }
+      const F2 mul2 = f2_pack(mul, mul);
 #pragma unroll
       for (int j = 0; j < kChunks; ++j) {
-        load_chunk<true>(src, p.res_f32, j, tid, nt, H, r[j]);
+        const int c = (j * nt + tid) * 8;
+        r[j][0] = r[j][1] = r[j][2] = r[j][3] = 0ull;
+        if (c < H) {
+          load8_f2(src, p.res_f32, c, r[j]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[j][e] = p.res_scale * r[j][e] + mul * y[j][e];
+          for (int e = 0; e < 4; ++e) r[j][e] = f2_fma(r[j][e], res_scale, f2_mul(y[j][e], mul2));
+        }
       }
     }
     void* rdst = p.res_f32 ? static_cast<void*>(static_cast<float*>(p.res_out) + row * p.res_out_stride)
                            : static_cast<void*>(static_cast<uint16_t*>(p.res_out) + row * p.res_out_stride);
-    float ss = 0.f;
+    F2 sum = 0ull;
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-      store_chunk<true>(rdst, p.res_f32, j, tid, nt, H, r[j]);
-      if (row_col<true>(j, 0, tid, nt) < H)
+      const int c = (j * nt + tid) * 8;
+      if (c < H) store8_f2(rdst, p.res_f32, c, r[j]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(r[j][e], r[j][e], ss);
+      for (int e = 0; e < 4; ++e) sum = f2_fma(r[j][e], r[j][e], sum);
     }
     float rstd = 0.f;
-    if (p.pre_gain) rstd = rsqrtf(cta_sum(ss, red_pre[n & 1]) / static_cast<float>(H) + p.eps);
+    if (p.pre_gain) {
+      float lo, hi;
+      f2_unpack(sum, lo, hi);
+      rstd = rsqrtf(cta_sum(lo + hi, red_pre[n & 1]) * over_h + p.eps);
+    }
     // every thread has read its part of the slot once it is past that sum's barrier
     if (!p.pre_gain || nt == 32) __syncthreads();
     if (tid == 0 && row + static_cast<int64_t>(stages) * gridDim.x < rows) fetch(row + stages * gridDim.x, st);
     if (p.pre_gain) {
+      const F2 rstd2 = f2_pack(rstd, rstd);
       uint32_t amax = 0;
 #pragma unroll
       for (int j = 0; j < kChunks; ++j) {
-        float g[8];
-        load_chunk<true>(pre_s, true, j, tid, nt, H, g);
+        const int c = (j * nt + tid) * 8;
+        if (c < H) {
+          F2 g[4];
+          load8_f2(p.pre_gain, true, c, g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[j][e] = r[j][e] * rstd * g[e];
-        if (row_col<true>(j, 0, tid, nt) < H)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) amax = max(amax, abs_bits(r[j][e]));
+          for (int e = 0; e < 4; ++e) {
+            r[j][e] = f2_mul(f2_mul(r[j][e], rstd2), g[e]);
+            if (kInt8) {
+              float lo, hi;
+              f2_unpack(r[j][e], lo, hi);
+              amax = max(amax, max(abs_bits(lo), abs_bits(hi)));
+            }
+          }
+          if (!kInt8) {
+            const bool f32 = p.out_kind == kRowsF32;
+            store8_f2(f32 ? static_cast<void*>(static_cast<float*>(p.out) + row * p.out_stride)
+                          : static_cast<void*>(static_cast<uint16_t*>(p.out) + row * p.out_stride), f32, c, r[j]);
+          }
+        }
       }
-      if (p.out_kind == kRowsInt8) {
+      if (kInt8) {
         const RowScale s = row_scale(cta_max(amax, red_max[n & 1]));
         int8_t* dst = static_cast<int8_t*>(p.out) + row * p.out_stride;
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) store_chunk_q<true>(dst, j, tid, nt, H, r[j], s);
-        if (tid == 0) p.out_scale[row] = s.scale;
-      } else {
-        const bool f32 = p.out_kind == kRowsF32;
-        void* dst = f32 ? static_cast<void*>(static_cast<float*>(p.out) + row * p.out_stride)
-                        : static_cast<void*>(static_cast<uint16_t*>(p.out) + row * p.out_stride);
+        for (int j = 0; j < kChunks; ++j) {
+          const int c = (j * nt + tid) * 8;
+          float f[8];
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) store_chunk<true>(dst, f32, j, tid, nt, H, r[j]);
+          for (int e = 0; e < 4; ++e) f2_unpack(r[j][e], f[2 * e], f[2 * e + 1]);
+          if (c < H) *reinterpret_cast<uint2*>(dst + c) = make_uint2(quant8x4(f[0], f[1], f[2], f[3], s), quant8x4(f[4], f[5], f[6], f[7], s));
+        }
+        if (tid == 0) p.out_scale[row] = s.scale;
       }
     }
     if (++st == stages) { st = 0; ph ^= 1; }
@@ -343,22 +376,21 @@ static bool try_stream(const BlockNormParams& p, int64_t rows, cudaStream_t stre
   const int units = p.H / 8;
   const int chunks = units > 1024 ? 4 : units > 256 ? 2 : 1;
   const int threads = ((units + chunks - 1) / chunks + 31) / 32 * 32;
-  const bool rows_gate = p.gate && p.gate_col_stride != 0 && p.gate_stride != 0, cols_gate = p.gate && p.gate_col_stride != 0 && p.gate_stride == 0;
+  const bool rows_gate = p.gate && p.gate_col_stride != 0 && p.gate_stride != 0;
   const int row_bytes = p.H * ((p.res_f32 ? 4 : 2) + (p.blk_f32 ? 4 : 2) + (rows_gate ? (p.gate_f32 ? 4 : 2) : 0));
-  const int fixed = p.H * ((p.post_gain ? 4 : 0) + (p.pre_gain ? 4 : 0) + (cols_gate ? (p.gate_f32 ? 4 : 2) : 0));
-  int per_sm = chunks == 4 ? 1 : 65536 / (threads * 64);      // CTAs an SM: by registers, then by shared memory
-  if (per_sm > 4) per_sm = 4;
-  int stages = 0;
-  for (; per_sm >= 1; --per_sm) {
-    stages = (216 * 1024 / per_sm - fixed - 2048) / row_bytes;
-    if (stages >= 2) break;
-  }
-  if (per_sm < 1) return false;
-  if (stages > kStreamStages) stages = kStreamStages;
-  const size_t smem = fixed + static_cast<size_t>(stages) * row_bytes;
+  // CTAs an SM by registers, then by shared memory; a ring of two, more do not help (4096 x 4096: 2 / 3 / 8 rows 37.8 /
+  // 38.7 / 39.4 us), and L1 keeps some room for the gains
+  int per_sm = 65536 / (threads * (chunks == 4 ? 128 : 64));
+  if (per_sm > 8) per_sm = 8;
+  while (per_sm > 1 && 2 * row_bytes * per_sm > 184 * 1024) --per_sm;
+  const int stages = 2;
+  const size_t smem = static_cast<size_t>(stages) * row_bytes;
+  if (smem > 200 * 1024) return false;
   const int64_t most = 148LL * per_sm;
   const dim3 grid(static_cast<unsigned>(rows < most ? rows : most)), block(threads);
-  auto kernel = chunks == 1 ? okc_block_norm_stream<1> : chunks == 2 ? okc_block_norm_stream<2> : okc_block_norm_stream<4>;
+  const bool q = p.pre_gain && p.out_kind == kRowsInt8;
+  auto kernel = q ? (chunks == 1 ? okc_block_norm_stream<1, true> : chunks == 2 ? okc_block_norm_stream<2, true> : okc_block_norm_stream<4, true>)
+                  : (chunks == 1 ? okc_block_norm_stream<1, false> : chunks == 2 ? okc_block_norm_stream<2, false> : okc_block_norm_stream<4, false>);
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e == cudaSuccess) e = launch_kernel(kernel, grid, block, smem, stream, false, p, static_cast<int>(rows), stages, row_bytes);
   return true;

@@ -53,6 +53,51 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// Two f32 in one 64-bit register: sm_100 multiplies and adds such pairs in one instruction, each half rounded as usual.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2_pack(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void f2_unpack(F2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// Eight neighbouring values at column c of an aligned row, as four pairs.
+__device__ __forceinline__ void load8_f2(const void* row, bool f32, int c, F2 (&v)[4]) {
+  if (f32) {
+    const float4 a = reinterpret_cast<const float4*>(static_cast<const float*>(row) + c)[0];
+    const float4 b = reinterpret_cast<const float4*>(static_cast<const float*>(row) + c)[1];
+    v[0] = f2_pack(a.x, a.y); v[1] = f2_pack(a.z, a.w); v[2] = f2_pack(b.x, b.y); v[3] = f2_pack(b.z, b.w);
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = f2_pack(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+  }
+}
+__device__ __forceinline__ void store8_f2(void* row, bool f32, int c, const F2 (&v)[4]) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f2_unpack(v[j], f[2 * j], f[2 * j + 1]);
+  if (f32) {
+    float4* d = reinterpret_cast<float4*>(static_cast<float*>(row) + c);
+    d[0] = make_float4(f[0], f[1], f[2], f[3]);
+    d[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + c) =
+        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+}
+
 // The columns of a row belong to threads in chunks of eight.  With kVec a chunk is eight neighbours (16- and 32-byte
 // accesses; the host checks that the width and every stride and address allow them); without, neighbouring threads
 // take neighbouring columns, so that single-element accesses still coalesce.
