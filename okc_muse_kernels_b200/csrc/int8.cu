@@ -474,9 +474,10 @@ constexpr int kManySmem = 1024 + kManyStages * kManyStageBytes + kManyEpilogueWa
 struct Int8ManyParams {
   CUtensorMap xmap;      // int8 token rows, box 128 x 128 rows
   CUtensorMap wmap;      // int8 weight rows, box 128 x bn / 2 rows
+  CUtensorMap omap;      // bf16 result rows, box 32 columns x 32 rows (only with tma_out)
   Int8Params p;
   int bn;                // weight rows of a pair's tile (columns of its accumulator): a multiple of 32 (gated: 64), at most 256
-  int n_kb, tiles_t, tiles_n;
+  int n_kb, tiles_t, tiles_n, tma_out;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -537,6 +538,22 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// 2-D tiled tensor store shared -> global; elements outside the tensor are not written.
+__device__ __forceinline__ void tma_2d_s2g(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(c0), "r"(c1), "r"(src)
+               : "memory");
+}
+// 32 bf16 results of a thread's row into its warp's staging: rows of 64 bytes, 16-byte pieces in the 64-byte swizzle.
+__device__ __forceinline__ void stage_bf16_row(uint32_t at, int lane, const uint32_t (&r)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
+    st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
+  }
+}
+
 template <bool kGated>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_int8_many(const __grid_constant__ Int8ManyParams q) {
   extern __shared__ uint8_t smem_raw[];
@@ -693,26 +710,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
           else if (p.bias) v = __fadd_rn(v, bs[j]);
           r[j] = __float_as_uint(v);
         }
-        // A thread has 32 neighbouring results of its own row, 64 or 128 whole bytes, and stores them itself where 16-byte
-        // stores can.  (Through shared memory and TMA stores: the same time within 3 % from K = 1024 on.)
+        // A thread has 32 neighbouring results of its own row.  As bf16 they leave through shared memory and a TMA store a
+        // warp, whole sectors at a time (stored by the threads themselves, 16 bytes each, 4096x1024x4096 takes 28.6 us for
+        // 25.3); as f32 the thread has whole sectors.
         const int col = tw * width + c0;
-        if (p.out_vec && col + 32 <= p.N) {
+        if (q.tma_out) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
+          stage_bf16_row(at, lane, r);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            if (row0 < p.T && col < p.N) tma_2d_s2g(&q.omap, at, col, row0);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else if (p.out_f32 && p.out_vec && col + 32 <= p.N) {
           if (t < p.T) {
-            const int64_t o = static_cast<int64_t>(t) * p.out_stride + col;
-            if (p.out_f32) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + o);
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + static_cast<int64_t>(t) * p.out_stride + col);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) dst[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-            } else {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + o);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
-                dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
-              }
-            }
+            for (int j = 0; j < 8; ++j) dst[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
           }
         } else {
           // rows off the 16-byte grid, or the last columns: through shared memory, so that a warp stores neighbours of a row
@@ -723,13 +739,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
 #pragma unroll
               for (int j = 0; j < 4; ++j) st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), r[16 * h + 4 * j], r[16 * h + 4 * j + 1], r[16 * h + 4 * j + 2], r[16 * h + 4 * j + 3]);
             } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(__uint_as_float(r[8 * j + 2 * i]), __uint_as_float(r[8 * j + 2 * i + 1]));
-                st_shared_v4(at + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
-              }
+              stage_bf16_row(at, lane, r);
             }
             __syncwarp();
             if (p.out_f32) {       // 16 columns of two rows a step
@@ -758,6 +768,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
       buf ^= 1;
       if (buf == 0) ph ^= 1;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
   tc_fence_before();
   cg::this_cluster().sync();     // no CTA frees its tensor memory or leaves while the pair's MMAs and arrivals may touch it
@@ -790,6 +802,8 @@ cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStre
   if (!encode_bytes_map(&q.xmap, p.x, p.T, p.K, p.x_stride, 128) ||
       !encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(cols), p.K, p.w_stride, q.bn / 2))
     return cudaErrorInvalidValue;
+  q.tma_out = p.out_vec && !p.out_f32;
+  if (q.tma_out && !encode_bf16_out_map(&q.omap, p.out, p.T, p.N, p.out_stride)) return cudaErrorInvalidValue;
   const long long tiles = static_cast<long long>(q.tiles_t) * q.tiles_n;
   const int grid = static_cast<int>(tiles < 74 ? 2 * tiles : 148);
   auto kernel = gated ? okc_int8_many<true> : okc_int8_many<false>;
