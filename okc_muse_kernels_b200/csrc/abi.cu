@@ -721,16 +721,16 @@ static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_
   p.out_vec = rows_vec(p.out, p.out_stride, T, p.out_f32 ? 4 : 2) ? 1 : 0;
   p.T = T; p.K = K; p.N = N;
   if (one) return launch_int8_one(p, gated, stream) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
-  bool pdl = false;
+  bool quantised_here = false;
   if (p.x_kind != kRowsInt8) {
     const int64_t q_stride = static_cast<int64_t>(int8_row_bytes(K));
     float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(a->scratch) + static_cast<size_t>(T) * q_stride);
     const int rc = okc_moe_quantize_rows(p.x, p.x_kind == kRowsF32, p.x_stride, T, K, a->scratch, q_stride, scale, stream_);
     if (rc != OKC_OK) return rc;
     p.x = a->scratch; p.x_scale = scale; p.x_stride = q_stride; p.x_kind = kRowsInt8;
-    pdl = true;
+    quantised_here = true;
   }
-  const cudaError_t e = int8_use_many(T, K, N, gated) ? launch_int8_many(p, gated, pdl, stream) : launch_int8_mid(p, gated, pdl, stream);
+  const cudaError_t e = int8_use_many(T, K, N, gated) ? launch_int8_many(p, gated, quantised_here, stream) : launch_int8_mid(p, gated, quantised_here, stream);
   return e == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
 }
 

@@ -96,6 +96,8 @@ __global__ void __launch_bounds__(kOneThreads) okc_int8_one(const Int8Params p, 
       if (r < rows && k < p.K) w[u] = ldg_stream(p.w + (!kGated || r < nr ? n0 + r : p.N + n0 + r - nr) * p.w_stride + k);
     }
   };
+  griddep_wait();
+  griddep_launch_dependents();
   uint4 wa[kAhead], wb[kAhead];
   load(wa, group);
   load(wb, group + kAhead * groups);
@@ -177,8 +179,8 @@ cudaError_t launch_int8_one(const Int8Params& p, bool gated, cudaStream_t stream
   if (rpc > most) rpc = most;
   const size_t smem = static_cast<size_t>(gated ? 2 : 1) * rpc * sizeof(int) + static_cast<size_t>((p.K + 15) & ~15);     // at most 20 KB
   const dim3 grid((p.N + rpc - 1) / rpc), block(kOneThreads);
-  return gated ? launch_kernel(okc_int8_one<true>, grid, block, smem, stream, false, p, rpc)
-               : launch_kernel(okc_int8_one<false>, grid, block, smem, stream, false, p, rpc);
+  return gated ? launch_kernel(okc_int8_one<true>, grid, block, smem, stream, true, p, rpc)
+               : launch_kernel(okc_int8_one<false>, grid, block, smem, stream, true, p, rpc);
 }
 
 // ------------------------------------------------------------------ tcgen05 pieces shared by the two tiled kernels
@@ -233,6 +235,7 @@ struct Int8MidParams {
   CUtensorMap xmap;      // int8 token rows, box 128 x tn
   Int8Params p;
   int tn, stages, n_kb, tmem_cols;
+  int early_w;           // the kernel before this one is the quantiser of its tokens: the weights may be read at once
 };
 
 // The producer and the issuer run as whole warps with one elected lane acting: in code that only one thread runs, every
@@ -277,6 +280,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   constexpr int kQuads = kGated ? kTileW / 8 : kTileW / 4;
   const int o4 = (tid % kQuads) * 4, n = w0 + o4;
   float sw[4], su[4] = {}, sb[4] = {};
+  if (!q.early_w) griddep_wait();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const bool in = n + j < p.N;
@@ -297,10 +301,10 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     auto load_x = [&](int i, uint32_t st) {
       if (elect_one()) tma_2d_g2s(smem0 + st * stage_bytes + kTileW * kKb, &q.xmap, (kb0 + i) * kKb, t0, full0 + 8 * st);
     };
-    // the weights of the first stages do not depend on the kernel before this one, the token rows may
     const int first = min(nkb, q.stages);
     for (int i = 0; i < first; ++i) load_w(i, i);
     griddep_wait();
+    griddep_launch_dependents();
     for (int i = 0; i < first; ++i) load_x(i, i);
     int i = first;
     uint32_t st = 0, ph = 0;
@@ -415,9 +419,10 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
 
 static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
 
-cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream) {
+cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream) {
   Int8MidParams q;
   q.p = p;
+  q.early_w = quantised_here ? 1 : 0;
   const int per_tile = gated ? kTileW / 2 : kTileW;
   const int tiles = (p.N + per_tile - 1) / per_tile;
   const int ttiles = (p.T + 255) / 256;
@@ -449,17 +454,12 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStrea
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  int n = 0;
-  attr[n].id = cudaLaunchAttributeClusterDimension;
-  attr[n].val.clusterDim.x = splits; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
-  ++n;
-  if (pdl) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = n;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, q);
 }
 
@@ -478,6 +478,7 @@ struct Int8ManyParams {
   Int8Params p;
   int bn;                // weight rows of a pair's tile (columns of its accumulator): a multiple of 32 (gated: 64), at most 256
   int n_kb, tiles_t, tiles_n, tma_out;
+  int early_w;           // as in Int8MidParams
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -585,9 +586,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
   cg::this_cluster().sync();
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
+  if (!q.early_w) griddep_wait();
 
   if (warp == 0) {
     griddep_wait();
+    griddep_launch_dependents();
     const uint32_t half_bytes = 128u * kKb + static_cast<uint32_t>(q.bn / 2) * kKb;
     const uint32_t full0 = map_rank(smem_u32(&bar_full[0]), 0);      // the bytes of both CTAs count on the leader's barriers
     const uint32_t empty0 = smem_u32(&bar_empty[0]);
@@ -782,9 +785,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
 
 bool int8_use_many(int T, int K, int N, bool gated) { (void)K; (void)N; (void)gated; return T > 256; }
 
-cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream) {
+cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream) {
   Int8ManyParams q;
   q.p = p;
+  q.early_w = quantised_here ? 1 : 0;
   q.n_kb = (p.K + kKb - 1) / kKb;
   q.tiles_t = (p.T + 255) / 256;
   const int64_t cols = static_cast<int64_t>(gated ? 2 : 1) * p.N;
@@ -809,7 +813,7 @@ cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStre
   auto kernel = gated ? okc_int8_many<true> : okc_int8_many<false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(grid), dim3(kManyThreads), kManySmem, stream, pdl, q);
+  return launch_kernel(kernel, dim3(grid), dim3(kManyThreads), kManySmem, stream, true, q);
 }
 
 __global__ void okc_int8_clear_status() { g_int8_status = 0; }

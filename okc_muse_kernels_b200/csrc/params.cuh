@@ -174,8 +174,9 @@ struct Int8Params {
 constexpr int kInt8OneMaxK = 16384;         // up to here the product of one token quantises it itself
 constexpr int kInt8MaxK = 131071;          // 128 * 128 * K stays below 2^31
 cudaError_t launch_int8_one(const Int8Params& p, bool gated, cudaStream_t stream);
-cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream);
-cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool pdl, cudaStream_t stream);
+// quantised_here: launched right behind the kernel that quantised its tokens
+cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream);
+cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream);
 bool int8_use_many(int T, int K, int N, bool gated);
 cudaError_t int8_read_status(cudaStream_t stream, int32_t* code);
 // Tensor map of int8 rows (abi.cu): box = 128 bytes x box_rows, 128-byte swizzle, zero fill outside.
