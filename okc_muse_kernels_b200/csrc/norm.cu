@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_block_norm(const Blo
 // bulk copies fill ahead of it, so that HBM does not wait for the two dependent sums of a row.  What is left is issue
 // slots: pairs of f32 an instruction, and as many CTAs an SM as registers allow (the gains stay in L1, not in shared
 // memory, for that).  4096 x 5120, everything bf16, a gate per element: NORM_US us (NORM_TB TB/s); a CTA per row 65.1 us.
-constexpr int kStreamStages = 4;
+constexpr int kStreamStages = 4, kStreamSmem = 200 * 1024;      // an SM's shared memory for rings
 template <int kChunks, bool kInt8>
 __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream(const BlockNormParams p, int rows, int stages, int row_bytes) {
   extern __shared__ __align__(16) uint8_t ring[];
@@ -391,12 +391,12 @@ static bool try_stream(const BlockNormParams& p, int64_t rows, cudaStream_t stre
   const int row_bytes = p.H * ((p.res_f32 ? 4 : 2) + (p.blk_f32 ? 4 : 2) + (rows_gate ? (p.gate_f32 ? 4 : 2) : 0));
   // CTAs an SM by registers, then by shared memory; a ring of two, more do not help (4096 x 4096: 2 / 3 / 8 rows 37.8 /
   // 38.7 / 39.4 us), and L1 keeps some room for the gains
-  int per_sm = 65536 / (threads * (chunks == 4 ? 128 : 64));
-  if (per_sm > 8) per_sm = 8;
-  while (per_sm > 1 && 2 * row_bytes * per_sm > 184 * 1024) --per_sm;
+  int per_sm = 65536 / (threads * (chunks == 4 ? 96 : chunks == 2 ? 56 : 40));
+  if (per_sm > 16) per_sm = 16;
+  while (per_sm > 1 && 2 * row_bytes * per_sm > kStreamSmem) --per_sm;
   const int stages = 2;
   const size_t smem = static_cast<size_t>(stages) * row_bytes;
-  if (smem > 200 * 1024) return false;
+  if (smem > kStreamSmem) return false;
   const int64_t most = 148LL * per_sm;
   const dim3 grid(static_cast<unsigned>(rows < most ? rows : most)), block(threads);
   const bool q = p.pre_gain && p.out_kind == kRowsInt8;
