@@ -317,7 +317,8 @@ int okc_moe_block_norm(const okc_block_norm_args* args, okc_stream_t stream);
 
 /* Rows of bf16 / f32 -> int8 rows and their scales.  With a = max|x| of a row: scale = f32(a / 127),
  * q = rint(f32(x * f32(127 / a))); a < 2^-120: zeros and scale 0; a row with an infinity or a NaN: zeros and scale NaN.
- * cols <= 131071. */
+ * cols <= 131071.  q: rows x q_stride bytes; where q and q_stride are multiples of 16, the bytes between cols and the next
+ * multiple of 8 may be written (with zeros). */
 int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t rows, int32_t cols, void* q,
                           int64_t q_stride, float* scale, okc_stream_t stream);
 

@@ -659,6 +659,10 @@ int okc_moe_block_norm(const okc_block_norm_args* a, okc_stream_t stream) {
   }
   if ((a->gate != nullptr) != (a->gate_kind != 0)) return OKC_ERR_BAD_ARG;
   if (a->gate_kind == 3 && many_rows && a->gate_stride < H) return OKC_ERR_BAD_ARG;
+  if (!aligned(a->residual, a->residual_f32 ? 4 : 2) || !aligned(a->residual_out, a->residual_f32 ? 4 : 2) || !aligned(a->block, a->block_f32 ? 4 : 2) ||
+      !aligned(a->gate, a->gate_f32 ? 4 : 2) || !aligned(a->out, a->out_kind == kRowsF32 ? 4 : a->out_kind == kRowsInt8 ? 1 : 2) ||
+      !aligned(a->post_gain, 4) || !aligned(a->pre_gain, 4) || !aligned(a->out_scale, 4))
+    return OKC_ERR_BAD_ARG;
   if (a->pre_gain && (!a->out || (many_rows && a->out_stride < H) || (a->out_kind == kRowsInt8 && !a->out_scale))) return OKC_ERR_BAD_ARG;
   if (!is_sm100()) return OKC_ERR_NO_DEVICE;
   BlockNormParams p;
@@ -686,11 +690,11 @@ int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t ro
   if (cols > kInt8MaxK) return OKC_ERR_TOO_LARGE;
   if (rows == 0) return OKC_OK;
   if (!x || !q || !scale || (rows > 1 && (x_stride < cols || q_stride < cols))) return OKC_ERR_BAD_ARG;
+  if (!aligned(x, x_f32 ? 4 : 2) || !aligned(scale, 4)) return OKC_ERR_BAD_ARG;
   if (!is_sm100()) return OKC_ERR_NO_DEVICE;
   QuantizeParams p;
   p.x = x; p.q = static_cast<int8_t*>(q); p.scale = scale; p.x_stride = x_stride; p.q_stride = q_stride; p.cols = cols; p.x_f32 = x_f32 ? 1 : 0;
-  const bool vec = (cols % 8) == 0 && rows_vec(x, x_stride, rows, x_f32 ? 4 : 2) && rows_vec(q, q_stride, rows, 1);
-  return launch_quantize_rows(p, rows, vec, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
+  return launch_quantize_rows(p, rows, rows_vec(x, x_stride, rows, x_f32 ? 4 : 2), rows_vec(q, q_stride, rows, 1), reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
 }
 
 // Scratch of a product on bf16 / f32 tokens: their int8 rows, then the scales.
@@ -709,6 +713,9 @@ static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_
   const int T = a->tokens, K = a->k, N = a->n;
   if (!a->x || !a->w || !a->w_scale || !a->out || (gated && a->bias)) return OKC_ERR_BAD_ARG;
   if (a->w_stride < K || (a->w_stride % 16) != 0 || !aligned(a->w, 16) || (T > 1 && (a->x_stride < K || a->out_stride < N))) return OKC_ERR_BAD_ARG;
+  if (!aligned(a->x, a->x_kind == kRowsF32 ? 4 : a->x_kind == kRowsBf16 ? 2 : 16) || !aligned(a->out, a->out_f32 ? 4 : 2) || !aligned(a->w_scale, 4) ||
+      !aligned(a->x_scale, 4) || !aligned(a->bias, 4))
+    return OKC_ERR_BAD_ARG;
   if (a->x_kind == kRowsInt8 && (!a->x_scale || !aligned(a->x, 16) || a->x_stride < K || (a->x_stride % 16) != 0)) return OKC_ERR_BAD_ARG;
   const bool one = T == 1 && K <= kInt8OneMaxK;
   if (!one && a->x_kind != kRowsInt8 && (!a->scratch || !aligned(a->scratch, 16))) return OKC_ERR_BAD_ARG;

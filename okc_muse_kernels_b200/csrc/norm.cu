@@ -304,6 +304,148 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
   }
 }
 
+// The same ring for rows of any width and alignment: a copy takes the 16-byte pieces that a row lies in (never past the
+// row's last piece, so never out of its allocation), and the threads find the row behind the bytes in front of it.
+// Neighbouring threads take neighbouring columns.  4096 x 5121, bf16, a gate per element: ANY_US us, a CTA per row with
+// plain loads 138.5.
+template <int kChunks>
+__global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream_any(const BlockNormParams p, int rows, int stages, int row_bytes) {
+  extern __shared__ __align__(16) uint8_t ring[];
+  constexpr int kVals = kChunks * 8;
+  __shared__ uint64_t bar_full[kStreamStages];
+  __shared__ int abort_code;
+  __shared__ float red_post[2][32], red_pre[2][32];
+  __shared__ uint32_t red_max[2][32];
+  const int tid = threadIdx.x, nt = blockDim.x, H = p.H;
+  const bool gate_rows = p.gate && p.gate_col_stride != 0 && p.gate_stride != 0, gate_cols = p.gate && p.gate_col_stride != 0 && p.gate_stride == 0;
+  const int res_size = p.res_f32 ? 4 : 2, blk_size = p.blk_f32 ? 4 : 2, gate_size = p.gate_f32 ? 4 : 2;
+  const int res_room = (H * res_size + 30) & ~15, blk_room = (H * blk_size + 30) & ~15;      // any row's pieces fit
+  auto pieces = [&](const uint8_t* row, int bytes) {     // length of the pieces that a row lies in
+    return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15) + bytes + 15) & ~15u;
+  };
+  auto aligned_down = [](const uint8_t* row) { return reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(row) & ~static_cast<uintptr_t>(15)); };
+  auto head = [](const uint8_t* row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15); };
+  auto res_row = [&](int row) { return static_cast<const uint8_t*>(p.res) + row * p.res_stride * res_size; };
+  auto blk_row = [&](int row) { return static_cast<const uint8_t*>(p.blk) + row * p.blk_stride * blk_size; };
+  auto gate_row = [&](int row) { return static_cast<const uint8_t*>(p.gate) + row * p.gate_stride * gate_size; };
+  auto fetch = [&](int row, int st) {
+    const uint32_t bar = smem_u32(&bar_full[st]);
+    const uint32_t dst = smem_u32(ring) + st * row_bytes;
+    const uint32_t a = pieces(res_row(row), H * res_size), b = pieces(blk_row(row), H * blk_size), c = gate_rows ? pieces(gate_row(row), H * gate_size) : 0;
+    mbar_expect_tx(bar, a + b + c);
+    bulk_g2s(dst, aligned_down(res_row(row)), a, bar);
+    bulk_g2s(dst + res_room, aligned_down(blk_row(row)), b, bar);
+    if (gate_rows) bulk_g2s(dst + res_room + blk_room, aligned_down(gate_row(row)), c, bar);
+  };
+  // this thread's values of a row; the type is asked once
+  auto take = [&](const void* row, bool f32, float (&v)[kVals]) {
+    if (f32) {
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) { const int c = e * nt + tid; v[e] = c < H ? static_cast<const float*>(row)[c] : 0.f; }
+    } else {
+      uint32_t u[kVals];
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) { const int c = e * nt + tid; u[e] = c < H ? static_cast<const uint16_t*>(row)[c] : 0u; }
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) v[e] = __uint_as_float(u[e] << 16);
+    }
+  };
+  auto put = [&](void* row, bool f32, const float (&v)[kVals]) {
+    if (f32) {
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) { const int c = e * nt + tid; if (c < H) static_cast<float*>(row)[c] = v[e]; }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) { const int c = e * nt + tid; if (c < H) static_cast<__nv_bfloat16*>(row)[c] = __float2bfloat16_rn(v[e]); }
+    }
+  };
+  if (tid == 0) {
+    for (int i = 0; i < stages; ++i) mbar_init(smem_u32(&bar_full[i]), 1);
+    abort_code = 0;
+    mbar_fence_init();
+    griddep_wait();
+    for (int i = 0; i < stages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  __syncthreads();
+  const float over_h = 1.f / static_cast<float>(H);
+  int st = 0, n = 0;
+  uint32_t ph = 0;
+  for (int row = blockIdx.x; row < rows; row += gridDim.x, ++n) {
+    float mul = p.blk_scale;
+    if (p.gate && p.gate_col_stride == 0) {
+      float g;
+      if (p.gate_f32) g = *reinterpret_cast<const float*>(gate_row(row));
+      else g = __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(gate_row(row))) << 16);
+      if (p.gate_sigmoid) g = 1.f / (1.f + __expf(-g));
+      mul *= g;
+    }
+    mbar_wait(smem_u32(&bar_full[st]), ph, &abort_code, 0x82);     // (as in the kernel above: no thread leaves the loop)
+    const uint8_t* const src = ring + st * row_bytes;
+    float r[kVals], y[kVals];
+    take(src + res_room + head(blk_row(row)), p.blk_f32, y);
+    if (p.post_gain) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) ss = fmaf(y[e], y[e], ss);
+      const float rstd = rsqrtf(cta_sum(ss, red_post[n & 1]) * over_h + p.eps);
+      take(p.post_gain, true, r);
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) y[e] = y[e] * rstd * r[e];
+    }
+    if (gate_rows || gate_cols) {
+      take(gate_rows ? src + res_room + blk_room + head(gate_row(row)) : static_cast<const uint8_t*>(p.gate), p.gate_f32, r);
+      if (p.gate_sigmoid) {
+#pragma unroll
+        for (int e = 0; e < kVals; ++e) r[e] = 1.f / (1.f + __expf(-r[e]));
+      }
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) y[e] *= r[e];
+    }
+    take(src + head(res_row(row)), p.res_f32, r);
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < kVals; ++e) {
+      r[e] = p.res_scale * r[e] + mul * y[e];
+      if (e * nt + tid < H) ss = fmaf(r[e], r[e], ss);
+    }
+    put(p.res_f32 ? static_cast<void*>(static_cast<float*>(p.res_out) + row * p.res_out_stride)
+                  : static_cast<void*>(static_cast<uint16_t*>(p.res_out) + row * p.res_out_stride), p.res_f32, r);
+    float rstd = 0.f;
+    if (p.pre_gain) rstd = rsqrtf(cta_sum(ss, red_pre[n & 1]) * over_h + p.eps);
+    if (!p.pre_gain || nt == 32) __syncthreads();
+    if (tid == 0 && row + static_cast<int64_t>(stages) * gridDim.x < rows) fetch(row + stages * gridDim.x, st);
+    if (p.pre_gain) {
+      take(p.pre_gain, true, y);
+#pragma unroll
+      for (int e = 0; e < kVals; ++e) r[e] = r[e] * rstd * y[e];
+      if (p.out_kind == kRowsInt8) {
+        uint32_t amax = 0;
+#pragma unroll
+        for (int e = 0; e < kVals; ++e)
+          if (e * nt + tid < H) amax = max(amax, abs_bits(r[e]));
+        const RowScale s = row_scale(cta_max(amax, red_max[n & 1]));
+        int8_t* dst = static_cast<int8_t*>(p.out) + row * p.out_stride;
+#pragma unroll
+        for (int e = 0; e < kVals; ++e) { const int c = e * nt + tid; if (c < H) dst[c] = static_cast<int8_t>(quant8(r[e], s)); }
+        if (tid == 0) p.out_scale[row] = s.scale;
+      } else {
+        const bool f32 = p.out_kind == kRowsF32;
+        put(f32 ? static_cast<void*>(static_cast<float*>(p.out) + row * p.out_stride)
+                : static_cast<void*>(static_cast<uint16_t*>(p.out) + row * p.out_stride), f32, r);
+      }
+    }
+    if (++st == stages) { st = 0; ph ^= 1; }
+  }
+  __syncthreads();
+  if (tid == 0 && abort_code != 0) {
+    atomicCAS(&g_norm_status, 0, abort_code);
+    const long long c0 = clock64();
+    while (clock64() - c0 < kWaitLimitCycles / 100) {}
+  }
+}
+
 // Rows -> int8 values and a scale per row.  A CTA per row; a row that fits the CTA's registers is read once, a longer
 // one (more than 16384 columns) a second time, from L2.
 template <int kChunks, bool kVec>
@@ -339,8 +481,10 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_quantize_rows(const 
 }
 
 // The same for many rows of bf16: a warp per row, which it holds in registers as it is (up to 8192 columns in 128 of them).
-// Nothing waits on other warps, and a dozen warps an SM have their whole rows on the way at once.  4096 x 7168: the
-// kernel above, a CTA per row, 27.7 us; this one QUANT_US us (88 MB: QUANT_TB TB/s).
+// Nothing waits on other warps, and a dozen warps an SM have their whole rows on the way at once.  A row may start
+// anywhere: the loads are those of the 16-byte pieces that it lies in (with up to 7 values before and behind it, which
+// count as zeros), and the int8 values move down by as many lanes' bytes before they are stored eight at a time.
+// 4096 x 7168: a CTA per row 27.7 us, this kernel 16.7 (88 MB: 5.3 TB/s).
 template <int kVecs>
 __global__ void __launch_bounds__(128) okc_quantize_rows_warp(const QuantizeParams p, int64_t rows) {
   griddep_wait();
@@ -348,13 +492,29 @@ __global__ void __launch_bounds__(128) okc_quantize_rows_warp(const QuantizePara
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + row * p.x_stride);
-  const int units = p.cols / 8;
+  const uintptr_t start = reinterpret_cast<uintptr_t>(static_cast<const uint16_t*>(p.x) + row * p.x_stride);
+  const int head = static_cast<int>(start & 15) >> 1;         // values in front of the row in its first piece
+  const uint4* src = reinterpret_cast<const uint4*>(start & ~static_cast<uintptr_t>(15));
+  const int end = head + p.cols, units = (end + 7) / 8;
   uint4 v[kVecs];
 #pragma unroll
   for (int j = 0; j < kVecs; ++j) {
     v[j] = make_uint4(0, 0, 0, 0);
     if (j * 32 + lane < units) v[j] = __ldg(src + j * 32 + lane);
+  }
+  const bool ragged = (head | (end & 7)) != 0;
+  if (ragged) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const int u = j * 32 + lane;
+      if (u == 0 || u == units - 1) {
+        uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (u * 8 + i < head || u * 8 + i >= end) w[i >> 1] &= (i & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+        v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
   }
   uint32_t m = 0;      // two running maxima of the magnitudes' bits, 16 bits each
 #pragma unroll
@@ -363,11 +523,29 @@ __global__ void __launch_bounds__(128) okc_quantize_rows_warp(const QuantizePara
   const RowScale s = row_scale(__reduce_max_sync(0xffffffffu, max(m & 0xFFFF0000u, m << 16)));
   if (lane == 0) p.scale[row] = s.scale;
   uint2* dst = reinterpret_cast<uint2*>(p.q + row * p.q_stride);
-#pragma unroll
-  for (int j = 0; j < kVecs; ++j) {
+  auto quantised = [&](int j) {
     float f[8];
     unpack_bf16x8(v[j], f);
-    if (j * 32 + lane < units) dst[j * 32 + lane] = make_uint2(quant8x4(f[0], f[1], f[2], f[3], s), quant8x4(f[4], f[5], f[6], f[7], s));
+    return make_uint2(quant8x4(f[0], f[1], f[2], f[3], s), quant8x4(f[4], f[5], f[6], f[7], s));
+  };
+  const int out_units = (p.cols + 7) / 8;
+  if (head == 0) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j)
+      if (j * 32 + lane < out_units) dst[j * 32 + lane] = quantised(j);
+  } else {
+    uint2 cur = quantised(0);
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+      const uint2 next = j + 1 < kVecs ? quantised(j + 1) : make_uint2(0, 0);
+      // the eight values behind this lane's: the next lane's, or the first lane's of the next step
+      const uint2 give = lane == 0 ? next : cur;
+      const uint2 from = make_uint2(__shfl_sync(0xffffffffu, give.x, (lane + 1) & 31), __shfl_sync(0xffffffffu, give.y, (lane + 1) & 31));
+      const uint64_t lo = cur.x | (static_cast<uint64_t>(cur.y) << 32), hi = from.x | (static_cast<uint64_t>(from.y) << 32);
+      const uint64_t out = (lo >> (8 * head)) | (hi << (64 - 8 * head));
+      if (j * 32 + lane < out_units) dst[j * 32 + lane] = make_uint2(static_cast<uint32_t>(out), static_cast<uint32_t>(out >> 32));
+      cur = next;
+    }
   }
 }
 
@@ -381,18 +559,21 @@ static void row_shape(int64_t rows, int cols, int& threads, int& chunks) {
   if (threads > row_threads(chunks)) threads = row_threads(chunks);
 }
 
-// The streaming kernel, if the rows are many and a ring of at least two fits; false: not launched.
-static bool try_stream(const BlockNormParams& p, int64_t rows, cudaStream_t stream, cudaError_t& e) {
+// The streaming kernels, if the rows are many and a ring of two fits; false: not launched.
+static bool try_stream(const BlockNormParams& p, int64_t rows, bool vec, cudaStream_t stream, cudaError_t& e) {
   if (!p.blk || rows < 4 * 148 || rows > INT32_MAX / 2) return false;
-  const int units = p.H / 8;
+  const int units = (p.H + 7) / 8;
   const int chunks = units > 1024 ? 4 : units > 256 ? 2 : 1;
   const int threads = ((units + chunks - 1) / chunks + 31) / 32 * 32;
   const bool rows_gate = p.gate && p.gate_col_stride != 0 && p.gate_stride != 0;
-  const int row_bytes = p.H * ((p.res_f32 ? 4 : 2) + (p.blk_f32 ? 4 : 2) + (rows_gate ? (p.gate_f32 ? 4 : 2) : 0));
+  auto room = [&](int f32) { return vec ? p.H * (f32 ? 4 : 2) : (p.H * (f32 ? 4 : 2) + 30) & ~15; };
+  const int row_bytes = room(p.res_f32) + room(p.blk_f32) + (rows_gate ? room(p.gate_f32) : 0);
   // CTAs an SM by registers, then by shared memory; a ring of two, more do not help (4096 x 4096: 2 / 3 / 8 rows 37.8 /
   // 38.7 / 39.4 us), and L1 keeps some room for the gains
-  int per_sm = 65536 / (threads * (chunks == 4 ? 96 : chunks == 2 ? 56 : 40));
+  const int regs = vec ? (chunks == 4 ? 96 : chunks == 2 ? 56 : 40) : (chunks == 4 ? 128 : 64);
+  int per_sm = 65536 / (threads * regs);
   if (per_sm > 16) per_sm = 16;
+  if (per_sm < 1) per_sm = 1;
   while (per_sm > 1 && 2 * row_bytes * per_sm > kStreamSmem) --per_sm;
   const int stages = 2;
   const size_t smem = static_cast<size_t>(stages) * row_bytes;
@@ -400,7 +581,8 @@ static bool try_stream(const BlockNormParams& p, int64_t rows, cudaStream_t stre
   const int64_t most = 148LL * per_sm;
   const dim3 grid(static_cast<unsigned>(rows < most ? rows : most)), block(threads);
   const bool q = p.pre_gain && p.out_kind == kRowsInt8;
-  auto kernel = q ? (chunks == 1 ? okc_block_norm_stream<1, true> : chunks == 2 ? okc_block_norm_stream<2, true> : okc_block_norm_stream<4, true>)
+  auto kernel = !vec ? (chunks == 1 ? okc_block_norm_stream_any<1> : chunks == 2 ? okc_block_norm_stream_any<2> : okc_block_norm_stream_any<4>)
+              : q ? (chunks == 1 ? okc_block_norm_stream<1, true> : chunks == 2 ? okc_block_norm_stream<2, true> : okc_block_norm_stream<4, true>)
                   : (chunks == 1 ? okc_block_norm_stream<1, false> : chunks == 2 ? okc_block_norm_stream<2, false> : okc_block_norm_stream<4, false>);
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e == cudaSuccess) e = launch_kernel(kernel, grid, block, smem, stream, true, p, static_cast<int>(rows), stages, row_bytes);
@@ -409,7 +591,7 @@ static bool try_stream(const BlockNormParams& p, int64_t rows, cudaStream_t stre
 
 cudaError_t launch_block_norm(const BlockNormParams& p, int64_t rows, bool vec, cudaStream_t stream) {
   cudaError_t e;
-  if (vec && try_stream(p, rows, stream, e)) return e;
+  if (try_stream(p, rows, vec, stream, e)) return e;
   int threads, chunks;
   row_shape(rows, p.H, threads, chunks);
   const dim3 grid(static_cast<unsigned>(rows)), block(threads);
@@ -418,12 +600,14 @@ cudaError_t launch_block_norm(const BlockNormParams& p, int64_t rows, bool vec, 
   return vec ? launch_kernel(okc_block_norm<4, true>, grid, block, 0, stream, true, p) : launch_kernel(okc_block_norm<4, false>, grid, block, 0, stream, true, p);
 }
 
-cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool vec, cudaStream_t stream) {
-  if (vec && !p.x_f32 && p.cols <= 8192 && rows >= 4 * 148) {
+cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool x_vec, bool q_vec, cudaStream_t stream) {
+  const bool vec = x_vec && q_vec && (p.cols % 8) == 0;
+  const int span = vec ? p.cols : p.cols + 7;
+  if (q_vec && !p.x_f32 && span <= 8192 && rows >= 4 * 148) {
     const dim3 grid(static_cast<unsigned>((rows + 3) / 4)), block(128);
-    if (p.cols <= 1024) return launch_kernel(okc_quantize_rows_warp<4>, grid, block, 0, stream, true, p, rows);
-    if (p.cols <= 2048) return launch_kernel(okc_quantize_rows_warp<8>, grid, block, 0, stream, true, p, rows);
-    if (p.cols <= 4096) return launch_kernel(okc_quantize_rows_warp<16>, grid, block, 0, stream, true, p, rows);
+    if (span <= 1024) return launch_kernel(okc_quantize_rows_warp<4>, grid, block, 0, stream, true, p, rows);
+    if (span <= 2048) return launch_kernel(okc_quantize_rows_warp<8>, grid, block, 0, stream, true, p, rows);
+    if (span <= 4096) return launch_kernel(okc_quantize_rows_warp<16>, grid, block, 0, stream, true, p, rows);
     return launch_kernel(okc_quantize_rows_warp<32>, grid, block, 0, stream, true, p, rows);
   }
   int threads, chunks;

@@ -154,7 +154,7 @@ struct QuantizeParams {
   int64_t x_stride, q_stride;
   int cols, x_f32;
 };
-cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool vec, cudaStream_t stream);
+cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool x_vec, bool q_vec, cudaStream_t stream);
 cudaError_t norm_read_status(cudaStream_t stream, int32_t* code);
 
 // The int8 products (int8.cu).

@@ -122,11 +122,22 @@ __device__ __forceinline__ void load_chunk(const void* row, bool f32, int chunk,
       for (int e = 0; e < 8; ++e) v[e] = 0.f;
     }
   } else {
+    // (the type is asked once, not for every value: the eight loads have to be under way together)
+    if (f32) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = row_col<false>(chunk, e, tid, nt);
-      v[e] = 0.f;
-      if (c < cols) v[e] = f32 ? static_cast<const float*>(row)[c] : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(row)[c]) << 16);
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_col<false>(chunk, e, tid, nt);
+        v[e] = c < cols ? static_cast<const float*>(row)[c] : 0.f;
+      }
+    } else {
+      uint32_t u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_col<false>(chunk, e, tid, nt);
+        u[e] = c < cols ? static_cast<const uint16_t*>(row)[c] : 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(u[e] << 16);
     }
   }
 }
@@ -144,12 +155,17 @@ __device__ __forceinline__ void store_chunk(void* row, bool f32, int chunk, int 
           make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
     }
   } else {
+    if (f32) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = row_col<false>(chunk, e, tid, nt);
-      if (c < cols) {
-        if (f32) static_cast<float*>(row)[c] = v[e];
-        else static_cast<__nv_bfloat16*>(row)[c] = __float2bfloat16_rn(v[e]);
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_col<false>(chunk, e, tid, nt);
+        if (c < cols) static_cast<float*>(row)[c] = v[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = row_col<false>(chunk, e, tid, nt);
+        if (c < cols) static_cast<__nv_bfloat16*>(row)[c] = __float2bfloat16_rn(v[e]);
       }
     }
   }

@@ -92,6 +92,8 @@ def _norm_args(**kw):
     (dict(residual_out_stride=10), BAD), (dict(out=None), BAD), (dict(out_stride=1), BAD), (dict(out_kind=3), BAD),
     (dict(out_kind=2), BAD), (dict(eps=-1e-3), BAD), (dict(gate=0x7000), BAD), (dict(gate_kind=1), BAD),
     (dict(gate=0x7000, gate_kind=3, gate_stride=63), BAD), (dict(block=None), BAD), (dict(block=None, post_gain=None, pre_gain=None), BAD),
+    (dict(residual=0x1001), BAD), (dict(residual=0x1002, residual_f32=1), BAD), (dict(block=0x2001), BAD), (dict(out=0x4002, out_kind=1), BAD),
+    (dict(pre_gain=0x5002), BAD), (dict(gate=0x7001, gate_kind=1), BAD),
 ])
 def test_block_norm_abi_checks(kw, rc):
     assert _lib.lib().okc_moe_block_norm(C.byref(_norm_args(**kw)), None) == rc
@@ -107,7 +109,8 @@ def _int8_args(**kw):
     (dict(tokens=0), OK), (dict(tokens=-1), BAD), (dict(k=0), BAD), (dict(n=0), BAD), (dict(k=131072, x_stride=131072, w_stride=131072), LARGE),
     (dict(x=None), BAD), (dict(w=None), BAD), (dict(w_scale=None), BAD), (dict(out=None), BAD), (dict(scratch=None), BAD),
     (dict(w=0x2008), BAD), (dict(w_stride=72), BAD), (dict(w_stride=48), BAD), (dict(x_stride=63), BAD), (dict(out_stride=31), BAD),
-    (dict(x_kind=3), BAD), (dict(x_kind=2), BAD), (dict(x_kind=2, x_scale=0x6000, x=0x1004), BAD), (dict(x_kind=2, x_scale=0x6000, x_stride=72), BAD),
+    (dict(x=0x1001), BAD), (dict(x=0x1002, x_kind=1), BAD), (dict(out=0x4001), BAD), (dict(out=0x4002, out_f32=1), BAD), (dict(w_scale=0x3002), BAD),
+    (dict(bias=0x7002), BAD), (dict(x_kind=3), BAD), (dict(x_kind=2), BAD), (dict(x_kind=2, x_scale=0x6000, x=0x1004), BAD), (dict(x_kind=2, x_scale=0x6000, x_stride=72), BAD),
 ])
 def test_int8_product_abi_checks(kw, rc):
     lib = _lib.lib()

@@ -81,7 +81,7 @@ def _gated_ref(q, scale, w, dtype):
 
 # ------------------------------------------------------------------------------------------------ quantize_rows
 @pytest.mark.parametrize("R,cols", [(1, 1), (3, 7), (2, 16), (5, 1000), (33, 4096), (2, 16385), (400, 2880), (301, 9000), (2, 131071), (7, 131064),
-                                    (593, 8), (595, 1016), (600, 2048), (700, 4088), (601, 8192), (599, 8200), (600, 1001)])
+                                    (593, 8), (595, 1016), (600, 2048), (700, 4088), (601, 8192), (599, 8200), (600, 1001), (640, 8185), (640, 8186), (700, 3), (600, 4089), (593, 250), (601, 257)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_quantize_rows_is_exact(R, cols, dtype):
     x = _randn((R, cols), _gen(R * cols), dtype)
@@ -115,8 +115,9 @@ def test_quantize_rows_special_rows(rows, dtype):
 
 def test_quantize_rows_strided_and_unaligned_input():
     g = _gen(5)
+    many = _randn((700, 301), g, torch.bfloat16)
     wide = _randn((6, 301), g)
-    for x in (wide[:, 3:200], wide[::2, :100], wide.t(), wide[1:, 1:2], wide.bfloat16()[:, 8:136], wide[0:1, 5:]):
+    for x in (many, many[:, 3:200], many[1:, 1:], many[::1, 8:136], many[5:, 7:8], many[:, :296], wide[:, 3:200], wide[::2, :100], wide.t(), wide[1:, 1:2], wide.bfloat16()[:, 8:136], wide[0:1, 5:]):
         got = okc.quantize_rows(x)
         q, scale = _quant_ref(x)
         assert torch.equal(got.q, q) and torch.equal(got.scale, scale)
@@ -343,7 +344,8 @@ def _check_norm(res, blk, out, **kw):
 
 
 @pytest.mark.parametrize("T,H", [(1, 1), (1, 4096), (2, 63), (7, 1000), (33, 5120), (3, 16384), (2, 16383), (300, 2048), (297, 2056), (310, 6500), (500, 8200), (298, 12289),
-                                 (593, 8), (600, 2040), (700, 5120), (597, 8192), (599, 12296)])
+                                 (593, 8), (600, 2040), (700, 5120), (597, 8192), (599, 12296),
+                                 (593, 1), (600, 2051), (650, 5121), (593, 16383), (700, 1001)])
 @pytest.mark.parametrize("res,blk", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)])
 def test_block_norm(T, H, res, blk):
     g = _gen(T * H + 1)
@@ -367,8 +369,17 @@ def test_block_norm_strides_in_place_and_unaligned():
         _check_norm(res, blk, "f32", post_gain=gain[:H], pre_gain=gain[1:], gate=wide[:T, -1:])
         _check_norm(res, blk, "int8", post_gain=gain[1:], pre_gain=gain[:H], gate=wide[2:, 5:5 + H])
     _check_norm(wide.t()[:H, :T], wide.t()[:H, 1:T + 1], "bf16", pre_gain=gain[:T].contiguous())
+    # many rows of all starts, each copied ahead of its turn
+    many = _randn((800, 3 * H + 1), g, torch.bfloat16)
+    for lo in (0, 1, 2, 3):
+        res, blk = many[:700, lo:lo + H - 1], many[100:, H + lo:2 * H - 1 + lo]
+        _check_norm(res, blk, "f32", post_gain=gain[1:H], pre_gain=gain[2:], gate=many[3:703, 2 * H:3 * H - 1])
+        _check_norm(res, blk.float(), "int8", post_gain=gain[1:H], pre_gain=gain[:H - 1], gate=many[0, 5:H + 4], gate_sigmoid=True)
+        _check_norm(res.float(), blk, "bf16", pre_gain=gain[:H - 1], gate=many[3:703, -1:], gate_sigmoid=True)
+        _check_norm(res, blk, "bf16", post_gain=gain[1:H])
     # many rows in place, each copied ahead of its turn: the same bits as out of place, twice over
-    for dtype in (torch.float32, torch.bfloat16):
+    for dtype, width in ((torch.float32, H), (torch.bfloat16, H), (torch.float32, H - 3), (torch.bfloat16, H - 3)):
+        H = width
         many, blk = _randn((2000, H), g, dtype), _randn((2000, H), g, dtype)
         first, x = okc.block_norm(many, blk, pre_gain=gain[:H], post_gain=gain[:H], gate=many, out="int8")
         second, x2 = okc.block_norm(first, blk, pre_gain=gain[:H], post_gain=gain[:H], gate=first, out="int8")
@@ -376,6 +387,7 @@ def test_block_norm_strides_in_place_and_unaligned():
         for want, wx in ((first, x), (second, x2)):
             _, y = okc.block_norm(store, blk, pre_gain=gain[:H], post_gain=gain[:H], gate=store, out="int8", residual_out=store)
             assert torch.equal(store, want) and torch.equal(y.q, wx.q) and torch.equal(y.scale, wx.scale)
+    H = 136
     # in place: the same bits as out of place (from the same addresses: the order of a row's sum goes by its alignment),
     # the columns and rows around them untouched
     store = wide.clone()
