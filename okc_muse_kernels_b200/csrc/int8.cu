@@ -7,7 +7,7 @@
 // Three kernels, by what bounds the product:
 //   okc_int8_one   one token        the weights are read by plain 16-byte loads and multiplied on the integer dot-product
 //                                   units; the token is quantised in the kernel (one launch)
-//   okc_int8_mid   some hundred     the weights fill M of a tcgen05.mma (kind::i8), the tokens are N; K is split over a
+//   okc_int8_mid   to some hundred  the weights fill M of a tcgen05.mma (kind::i8), the tokens are N; K is split over a
 //                                   cluster of CTAs that add their integer sums through distributed shared memory
 //   okc_int8_many  beyond           CTA pairs (cta_group::2) on tiles of 256 tokens x up to 256 weight rows, persistent
 // Every wait on a barrier is bounded; one that runs out is reported through a status word (okc_moe_dense_status).
@@ -419,21 +419,64 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
 
 static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
 
+// How the two tiled kernels would cut a product, and what each is expected to take.  The estimates are a start-up time, a
+// time for the end of a tile, and a time for each stage: what a CTA needs for it alone, or, with all SMs busy, what its
+// bytes take at the 90 KB/us that an SM takes in then.  Of 196 measured shapes (3 to 512 tokens, K 300 to 7168, N 300 to
+// 7168, plain and gated), where the two differ by up to 2 either way, the choice costs 0.14 % of the better one's time on
+// average and 13 % at worst.
+struct TileShape {
+  int tokens;        // mid: tokens of a tile
+  int t_tiles, tiles, splits;
+  int bn;            // many: weight rows of a tile
+  double us;
+};
+static double stage_us(double alone, double kbytes, double ctas) {
+  const double busy = kbytes / 90.0 * (ctas < 148 ? ctas / 148.0 : 1.0);
+  return busy > alone ? busy : alone;
+}
+static TileShape mid_shape(int T, int K, int N, bool gated) {
+  TileShape s = {};
+  const int per_tile = gated ? kTileW / 2 : kTileW, n_kb = (K + kKb - 1) / kKb;
+  s.tiles = (N + per_tile - 1) / per_tile;
+  s.t_tiles = (T + 255) / 256;
+  s.tokens = ((T + s.t_tiles - 1) / s.t_tiles + 15) & ~15;
+  // As many CTAs a cluster as one round of them fits the SMs (a cluster lives in one group of 16 to 20 SMs: 33 clusters of
+  // 4 and 15 of 8 fit at once).  K = 4096, N = 4096, 16 tokens (32 tiles), 1 / 2 / 4 / 8 CTAs a cluster: 10.5 / 7.8 / 6.6 /
+  // 13.9 us; gated, K = 7168, 2 x 2048 rows, 128 tokens: 18.4 / 12.9 / 10.6 / 26.0 us.
+  const int64_t clusters = static_cast<int64_t>(s.tiles) * s.t_tiles;
+  s.splits = clusters <= 14 ? 8 : clusters <= 32 ? 4 : clusters <= 74 ? 2 : 1;
+  while (s.splits > n_kb) s.splits /= 2;
+  const double ctas = static_cast<double>(clusters) * s.splits, rounds = static_cast<double>((clusters * s.splits + 147) / 148);
+  s.us = 3.0 + rounds * (0.021 * s.tokens + (n_kb + s.splits - 1) / s.splits * stage_us(0.21, 16 + s.tokens / 8.0, ctas));
+  return s;
+}
+static TileShape many_shape(int T, int K, int N, bool gated) {
+  TileShape s = {};
+  const int n_kb = (K + kKb - 1) / kKb;
+  const int64_t cols = static_cast<int64_t>(gated ? 2 : 1) * N;
+  s.t_tiles = (T + 255) / 256;
+  // The tile width with the least work in whole rounds of the 74 pairs.  A round of tiles bn wide takes a time in proportion
+  // to bn + 120 (K = 7168, bn 64 / 96 / 128 / 160 / 192 / 224 / 256: 11.1 / 11.4 / 12.4 / 14.1 / 15.0 / 18.1 / 18.9 us): the
+  // token rows of a tile are copied whatever its width.  Narrow tiles win where wide ones leave pairs without work.
+  long long best = -1, rounds = 0;
+  for (int bn = 256; bn >= 64; bn -= gated ? 64 : 32) {
+    const long long n = (cols + bn - 1) / bn, r = (n * s.t_tiles + 73) / 74;
+    if (best < 0 || r * (bn + 120) < best) { best = r * (bn + 120); rounds = r; s.bn = bn; s.tiles = static_cast<int>(n); }
+  }
+  const double ctas = 2.0 * s.tiles * s.t_tiles;
+  const double alone = s.bn <= 96 ? 0.19 : 0.00088 * (s.bn + 120);
+  s.us = 3.0 + rounds * (0.02 * s.bn + n_kb * stage_us(alone, 16 + s.bn / 16.0, ctas));
+  return s;
+}
+
 cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream) {
   Int8MidParams q;
   q.p = p;
   q.early_w = quantised_here ? 1 : 0;
-  const int per_tile = gated ? kTileW / 2 : kTileW;
-  const int tiles = (p.N + per_tile - 1) / per_tile;
-  const int ttiles = (p.T + 255) / 256;
-  q.tn = ((p.T + ttiles - 1) / ttiles + 15) & ~15;
+  const TileShape shape = mid_shape(p.T, p.K, p.N, gated);
+  const int per_tile = gated ? kTileW / 2 : kTileW, tiles = shape.tiles, ttiles = shape.t_tiles, splits = shape.splits;
+  q.tn = shape.tokens;
   q.n_kb = (p.K + kKb - 1) / kKb;
-  // As many CTAs a cluster as one round of them fits the SMs (a cluster lives in one group of 16 to 20 SMs: 33 clusters of
-  // 4 and 15 of 8 fit at once).  K = 4096, N = 4096, 16 tokens (32 tiles), 1 / 2 / 4 / 8 CTAs a cluster: 10.5 / 7.8 / 6.6 /
-  // 13.9 us; gated, K = 7168, 2 x 2048 rows, 128 tokens: 18.4 / 12.9 / 10.6 / 26.0 us.
-  const int64_t clusters = static_cast<int64_t>(tiles) * ttiles;
-  int splits = clusters <= 14 ? 8 : clusters <= 32 ? 4 : clusters <= 74 ? 2 : 1;
-  while (splits > q.n_kb) splits /= 2;
   const int stage = kTileW * kKb + q.tn * kKb;
   q.stages = 216 * 1024 / stage;
   if (q.stages > kMidMaxStages) q.stages = kMidMaxStages;
@@ -783,26 +826,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
   if (tid == 0 && abort_code != 0) atomicCAS(&g_int8_status, 0, abort_code);
 }
 
-bool int8_use_many(int T, int K, int N, bool gated) { (void)K; (void)N; (void)gated; return T > 256; }
+bool int8_use_many(int T, int K, int N, bool gated) { return T > 512 || many_shape(T, K, N, gated).us < mid_shape(T, K, N, gated).us; }
 
 cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream) {
   Int8ManyParams q;
   q.p = p;
   q.early_w = quantised_here ? 1 : 0;
   q.n_kb = (p.K + kKb - 1) / kKb;
-  q.tiles_t = (p.T + 255) / 256;
+  const TileShape shape = many_shape(p.T, p.K, p.N, gated);
   const int64_t cols = static_cast<int64_t>(gated ? 2 : 1) * p.N;
-  // The tile width with the least work in whole rounds of the 74 pairs.  A round of tiles bn wide takes a time in proportion
-  // to bn + 120 (K = 7168, bn 64 / 96 / 128 / 160 / 192 / 224 / 256: 11.1 / 11.4 / 12.4 / 14.1 / 15.0 / 18.1 / 18.9 us): the
-  // token rows of a tile are copied whatever its width.  Narrow tiles win where wide ones leave pairs without work.
-  q.bn = 256;
-  long long best = -1;
-  for (int bn = 256; bn >= 64; bn -= gated ? 64 : 32) {
-    const long long tn = (cols + bn - 1) / bn;
-    const long long cost = ((tn * q.tiles_t + 73) / 74) * (bn + 120);
-    if (best < 0 || cost < best) { best = cost; q.bn = bn; q.tiles_n = static_cast<int>(tn); }
-  }
-  if (gated) q.tiles_n = (p.N + q.bn / 2 - 1) / (q.bn / 2);
+  q.tiles_t = shape.t_tiles;
+  q.bn = shape.bn;
+  q.tiles_n = shape.tiles;      // (of a gated product: n tiles of bn / 2 outputs cover as many as n tiles of bn rows)
   if (!encode_bytes_map(&q.xmap, p.x, p.T, p.K, p.x_stride, 128) ||
       !encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(cols), p.K, p.w_stride, q.bn / 2))
     return cudaErrorInvalidValue;
