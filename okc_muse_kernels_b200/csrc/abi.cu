@@ -684,8 +684,8 @@ int okc_moe_block_norm(const okc_block_norm_args* a, okc_stream_t stream) {
   return launch_block_norm(p, rows, vec, reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
 }
 
-int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t rows, int32_t cols, void* q, int64_t q_stride,
-                          float* scale, okc_stream_t stream) {
+static int quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t rows, int32_t cols, void* q, int64_t q_stride,
+                         float* scale, bool product_follows, okc_stream_t stream) {
   if (rows < 0 || rows > INT32_MAX || cols <= 0) return OKC_ERR_BAD_ARG;
   if (cols > kInt8MaxK) return OKC_ERR_TOO_LARGE;
   if (rows == 0) return OKC_OK;
@@ -694,7 +694,13 @@ int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t ro
   if (!is_sm100()) return OKC_ERR_NO_DEVICE;
   QuantizeParams p;
   p.x = x; p.q = static_cast<int8_t*>(q); p.scale = scale; p.x_stride = x_stride; p.q_stride = q_stride; p.cols = cols; p.x_f32 = x_f32 ? 1 : 0;
+  p.product_follows = product_follows ? 1 : 0;
   return launch_quantize_rows(p, rows, rows_vec(x, x_stride, rows, x_f32 ? 4 : 2), rows_vec(q, q_stride, rows, 1), reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
+}
+
+int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t rows, int32_t cols, void* q, int64_t q_stride,
+                          float* scale, okc_stream_t stream) {
+  return quantize_rows(x, x_f32, x_stride, rows, cols, q, q_stride, scale, false, stream);
 }
 
 // Scratch of a product on bf16 / f32 tokens: their int8 rows, then the scales.
@@ -732,7 +738,7 @@ static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_
   if (p.x_kind != kRowsInt8) {
     const int64_t q_stride = static_cast<int64_t>(int8_row_bytes(K));
     float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(a->scratch) + static_cast<size_t>(T) * q_stride);
-    const int rc = okc_moe_quantize_rows(p.x, p.x_kind == kRowsF32, p.x_stride, T, K, a->scratch, q_stride, scale, stream_);
+    const int rc = quantize_rows(p.x, p.x_kind == kRowsF32, p.x_stride, T, K, a->scratch, q_stride, scale, true, stream_);
     if (rc != OKC_OK) return rc;
     p.x = a->scratch; p.x_scale = scale; p.x_stride = q_stride; p.x_kind = kRowsInt8;
     quantised_here = true;

@@ -10,6 +10,8 @@
 //   okc_int8_mid   to some hundred  the weights fill M of a tcgen05.mma (kind::i8), the tokens are N; K is split over a
 //                                   cluster of CTAs that add their integer sums through distributed shared memory
 //   okc_int8_many  beyond           CTA pairs (cta_group::2) on tiles of 256 tokens x up to 256 weight rows, persistent
+// The tiled kernels start early (programmatic launch) behind the quantiser of their own tokens and only there: it is
+// launched plainly, so everything before it, the weights too, is complete, and all its CTAs are on their SMs by then.
 // Every wait on a barrier is bounded; one that runs out is reported through a status word (okc_moe_dense_status).
 #include <cooperative_groups.h>
 
@@ -96,8 +98,6 @@ __global__ void __launch_bounds__(kOneThreads) okc_int8_one(const Int8Params p, 
       if (r < rows && k < p.K) w[u] = ldg_stream(p.w + (!kGated || r < nr ? n0 + r : p.N + n0 + r - nr) * p.w_stride + k);
     }
   };
-  griddep_wait();
-  griddep_launch_dependents();
   uint4 wa[kAhead], wb[kAhead];
   load(wa, group);
   load(wb, group + kAhead * groups);
@@ -179,8 +179,8 @@ cudaError_t launch_int8_one(const Int8Params& p, bool gated, cudaStream_t stream
   if (rpc > most) rpc = most;
   const size_t smem = static_cast<size_t>(gated ? 2 : 1) * rpc * sizeof(int) + static_cast<size_t>((p.K + 15) & ~15);     // at most 20 KB
   const dim3 grid((p.N + rpc - 1) / rpc), block(kOneThreads);
-  return gated ? launch_kernel(okc_int8_one<true>, grid, block, smem, stream, true, p, rpc)
-               : launch_kernel(okc_int8_one<false>, grid, block, smem, stream, true, p, rpc);
+  return gated ? launch_kernel(okc_int8_one<true>, grid, block, smem, stream, false, p, rpc)
+               : launch_kernel(okc_int8_one<false>, grid, block, smem, stream, false, p, rpc);
 }
 
 // ------------------------------------------------------------------ tcgen05 pieces shared by the two tiled kernels
@@ -235,7 +235,6 @@ struct Int8MidParams {
   CUtensorMap xmap;      // int8 token rows, box 128 x tn
   Int8Params p;
   int tn, stages, n_kb, tmem_cols;
-  int early_w;           // the kernel before this one is the quantiser of its tokens: the weights may be read at once
 };
 
 // The producer and the issuer run as whole warps with one elected lane acting: in code that only one thread runs, every
@@ -280,7 +279,6 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   constexpr int kQuads = kGated ? kTileW / 8 : kTileW / 4;
   const int o4 = (tid % kQuads) * 4, n = w0 + o4;
   float sw[4], su[4] = {}, sb[4] = {};
-  if (!q.early_w) griddep_wait();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const bool in = n + j < p.N;
@@ -301,10 +299,10 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     auto load_x = [&](int i, uint32_t st) {
       if (elect_one()) tma_2d_g2s(smem0 + st * stage_bytes + kTileW * kKb, &q.xmap, (kb0 + i) * kKb, t0, full0 + 8 * st);
     };
+    // the weights of the first stages do not depend on the kernel before this one, the token rows may
     const int first = min(nkb, q.stages);
     for (int i = 0; i < first; ++i) load_w(i, i);
     griddep_wait();
-    griddep_launch_dependents();
     for (int i = 0; i < first; ++i) load_x(i, i);
     int i = first;
     uint32_t st = 0, ph = 0;
@@ -472,7 +470,6 @@ static TileShape many_shape(int T, int K, int N, bool gated) {
 cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream) {
   Int8MidParams q;
   q.p = p;
-  q.early_w = quantised_here ? 1 : 0;
   const TileShape shape = mid_shape(p.T, p.K, p.N, gated);
   const int per_tile = gated ? kTileW / 2 : kTileW, tiles = shape.tiles, ttiles = shape.t_tiles, splits = shape.splits;
   q.tn = shape.tokens;
@@ -502,7 +499,7 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = quantised_here ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, q);
 }
 
@@ -521,7 +518,6 @@ struct Int8ManyParams {
   Int8Params p;
   int bn;                // weight rows of a pair's tile (columns of its accumulator): a multiple of 32 (gated: 64), at most 256
   int n_kb, tiles_t, tiles_n, tma_out;
-  int early_w;           // as in Int8MidParams
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -629,11 +625,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
   cg::this_cluster().sync();
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
-  if (!q.early_w) griddep_wait();
 
   if (warp == 0) {
     griddep_wait();
-    griddep_launch_dependents();
     const uint32_t half_bytes = 128u * kKb + static_cast<uint32_t>(q.bn / 2) * kKb;
     const uint32_t full0 = map_rank(smem_u32(&bar_full[0]), 0);      // the bytes of both CTAs count on the leader's barriers
     const uint32_t empty0 = smem_u32(&bar_empty[0]);
@@ -654,6 +648,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
         }
         if (++st == kManyStages) { st = 0; ph ^= 1; }
       }
+    }
+    // The issuer's last arrivals at this CTA's empty barriers come from the other CTA of the pair and nobody has waited for
+    // them yet: they have to land before this CTA's memory becomes another's.  (Empty barriers that were never used, or
+    // whose last arrival has been seen, pass at once.)
+    for (int i = 0; ok && i < kManyStages; ++i) {
+      ok = pair_wait(empty0 + 8 * st, ph, &abort_code, 0x77);
+      if (++st == kManyStages) { st = 0; ph ^= 1; }
     }
     // Every copy has landed once the epilogue has seen the last tile; a producer that gave up leaves them some time.
     if (!ok) {
@@ -831,7 +832,6 @@ bool int8_use_many(int T, int K, int N, bool gated) { return T > 512 || many_sha
 cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream) {
   Int8ManyParams q;
   q.p = p;
-  q.early_w = quantised_here ? 1 : 0;
   q.n_kb = (p.K + kKb - 1) / kKb;
   const TileShape shape = many_shape(p.T, p.K, p.N, gated);
   const int64_t cols = static_cast<int64_t>(gated ? 2 : 1) * p.N;
@@ -848,7 +848,7 @@ cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool quantised_her
   auto kernel = gated ? okc_int8_many<true> : okc_int8_many<false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kManySmem);
   if (e != cudaSuccess) return e;
-  return launch_kernel(kernel, dim3(grid), dim3(kManyThreads), kManySmem, stream, true, q);
+  return launch_kernel(kernel, dim3(grid), dim3(kManyThreads), kManySmem, stream, quantised_here, q);
 }
 
 __global__ void okc_int8_clear_status() { g_int8_status = 0; }

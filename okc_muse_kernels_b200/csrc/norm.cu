@@ -10,9 +10,9 @@
 // norms), the latency of one row's three dependent reductions for few.  A CTA per row: the thread count is chosen so
 // that a thread holds 8 values for few rows (short chains) and up to 32 for many (fewer barriers a byte).
 //
-// Every kernel here and in int8.cu is launched with the programmatic-serialization attribute, waits for the kernel before
-// it ahead of its first access to memory, and only then lets the kernel behind it start: a kernel that has started knows
-// that everything before its predecessor is complete.
+// These kernels are launched plainly: each starts when the one before it has completed.  Only the tiled int8 products
+// start early, behind the quantiser of their own tokens.  With every launch programmatic, CTAs of the next call that wait
+// hold registers that clusters of the product before them still need, and long queues of calls came to a stop.
 #include "rows.cuh"
 
 namespace okc {
@@ -28,8 +28,6 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_block_norm(const Blo
   __shared__ uint32_t red_max[32];
   const int tid = threadIdx.x, nt = blockDim.x, H = p.H;
   const int64_t row = blockIdx.x;
-  griddep_wait();
-  griddep_launch_dependents();
   float r[kChunks][8];
   {
     const void* src = p.res_f32 ? static_cast<const void*>(static_cast<const float*>(p.res) + row * p.res_stride)
@@ -150,11 +148,8 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     for (int i = 0; i < stages; ++i) mbar_init(smem_u32(&bar_full[i]), 1);
     abort_code = 0;
     mbar_fence_init();
-    griddep_wait();
     for (int i = 0; i < stages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
   }
-  griddep_wait();
-  griddep_launch_dependents();
   __syncthreads();
   const float over_h = 1.f / static_cast<float>(H);
   const F2 res_scale = f2_pack(p.res_scale, p.res_scale);
@@ -363,11 +358,8 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     for (int i = 0; i < stages; ++i) mbar_init(smem_u32(&bar_full[i]), 1);
     abort_code = 0;
     mbar_fence_init();
-    griddep_wait();
     for (int i = 0; i < stages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
   }
-  griddep_wait();
-  griddep_launch_dependents();
   __syncthreads();
   const float over_h = 1.f / static_cast<float>(H);
   int st = 0, n = 0;
@@ -451,8 +443,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
 template <int kChunks, bool kVec>
 __global__ void __launch_bounds__(row_threads(kChunks)) okc_quantize_rows(const QuantizeParams p) {
   __shared__ uint32_t red[32];
-  griddep_wait();
-  griddep_launch_dependents();
+  if (p.product_follows) griddep_launch_dependents();     // it may set itself up; it waits before it reads the rows
   const int tid = threadIdx.x, nt = blockDim.x;
   const int64_t row = blockIdx.x;
   const void* src = p.x_f32 ? static_cast<const void*>(static_cast<const float*>(p.x) + row * p.x_stride)
@@ -487,8 +478,7 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_quantize_rows(const 
 // 4096 x 7168: a CTA per row 27.7 us, this kernel 16.7 (88 MB: 5.3 TB/s).
 template <int kVecs>
 __global__ void __launch_bounds__(128) okc_quantize_rows_warp(const QuantizeParams p, int64_t rows) {
-  griddep_wait();
-  griddep_launch_dependents();
+  if (p.product_follows) griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
@@ -585,7 +575,7 @@ static bool try_stream(const BlockNormParams& p, int64_t rows, bool vec, cudaStr
               : q ? (chunks == 1 ? okc_block_norm_stream<1, true> : chunks == 2 ? okc_block_norm_stream<2, true> : okc_block_norm_stream<4, true>)
                   : (chunks == 1 ? okc_block_norm_stream<1, false> : chunks == 2 ? okc_block_norm_stream<2, false> : okc_block_norm_stream<4, false>);
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e == cudaSuccess) e = launch_kernel(kernel, grid, block, smem, stream, true, p, static_cast<int>(rows), stages, row_bytes);
+  if (e == cudaSuccess) e = launch_kernel(kernel, grid, block, smem, stream, false, p, static_cast<int>(rows), stages, row_bytes);
   return true;
 }
 
@@ -595,9 +585,9 @@ cudaError_t launch_block_norm(const BlockNormParams& p, int64_t rows, bool vec, 
   int threads, chunks;
   row_shape(rows, p.H, threads, chunks);
   const dim3 grid(static_cast<unsigned>(rows)), block(threads);
-  if (chunks == 1) return vec ? launch_kernel(okc_block_norm<1, true>, grid, block, 0, stream, true, p) : launch_kernel(okc_block_norm<1, false>, grid, block, 0, stream, true, p);
-  if (chunks == 2) return vec ? launch_kernel(okc_block_norm<2, true>, grid, block, 0, stream, true, p) : launch_kernel(okc_block_norm<2, false>, grid, block, 0, stream, true, p);
-  return vec ? launch_kernel(okc_block_norm<4, true>, grid, block, 0, stream, true, p) : launch_kernel(okc_block_norm<4, false>, grid, block, 0, stream, true, p);
+  if (chunks == 1) return vec ? launch_kernel(okc_block_norm<1, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_block_norm<1, false>, grid, block, 0, stream, false, p);
+  if (chunks == 2) return vec ? launch_kernel(okc_block_norm<2, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_block_norm<2, false>, grid, block, 0, stream, false, p);
+  return vec ? launch_kernel(okc_block_norm<4, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_block_norm<4, false>, grid, block, 0, stream, false, p);
 }
 
 cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool x_vec, bool q_vec, cudaStream_t stream) {
@@ -605,17 +595,17 @@ cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool x_v
   const int span = vec ? p.cols : p.cols + 7;
   if (q_vec && !p.x_f32 && span <= 8192 && rows >= 4 * 148) {
     const dim3 grid(static_cast<unsigned>((rows + 3) / 4)), block(128);
-    if (span <= 1024) return launch_kernel(okc_quantize_rows_warp<4>, grid, block, 0, stream, true, p, rows);
-    if (span <= 2048) return launch_kernel(okc_quantize_rows_warp<8>, grid, block, 0, stream, true, p, rows);
-    if (span <= 4096) return launch_kernel(okc_quantize_rows_warp<16>, grid, block, 0, stream, true, p, rows);
-    return launch_kernel(okc_quantize_rows_warp<32>, grid, block, 0, stream, true, p, rows);
+    if (span <= 1024) return launch_kernel(okc_quantize_rows_warp<4>, grid, block, 0, stream, false, p, rows);
+    if (span <= 2048) return launch_kernel(okc_quantize_rows_warp<8>, grid, block, 0, stream, false, p, rows);
+    if (span <= 4096) return launch_kernel(okc_quantize_rows_warp<16>, grid, block, 0, stream, false, p, rows);
+    return launch_kernel(okc_quantize_rows_warp<32>, grid, block, 0, stream, false, p, rows);
   }
   int threads, chunks;
   row_shape(rows, p.cols, threads, chunks);
   const dim3 grid(static_cast<unsigned>(rows)), block(threads);
-  if (chunks == 1) return vec ? launch_kernel(okc_quantize_rows<1, true>, grid, block, 0, stream, true, p) : launch_kernel(okc_quantize_rows<1, false>, grid, block, 0, stream, true, p);
-  if (chunks == 2) return vec ? launch_kernel(okc_quantize_rows<2, true>, grid, block, 0, stream, true, p) : launch_kernel(okc_quantize_rows<2, false>, grid, block, 0, stream, true, p);
-  return vec ? launch_kernel(okc_quantize_rows<4, true>, grid, block, 0, stream, true, p) : launch_kernel(okc_quantize_rows<4, false>, grid, block, 0, stream, true, p);
+  if (chunks == 1) return vec ? launch_kernel(okc_quantize_rows<1, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_quantize_rows<1, false>, grid, block, 0, stream, false, p);
+  if (chunks == 2) return vec ? launch_kernel(okc_quantize_rows<2, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_quantize_rows<2, false>, grid, block, 0, stream, false, p);
+  return vec ? launch_kernel(okc_quantize_rows<4, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_quantize_rows<4, false>, grid, block, 0, stream, false, p);
 }
 
 __global__ void okc_norm_clear_status() { g_norm_status = 0; }

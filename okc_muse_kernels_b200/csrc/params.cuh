@@ -153,6 +153,7 @@ struct QuantizeParams {
   float* scale;
   int64_t x_stride, q_stride;
   int cols, x_f32;
+  int product_follows;        // the next launch is the product of these rows: it may start early
 };
 cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool x_vec, bool q_vec, cudaStream_t stream);
 cudaError_t norm_read_status(cudaStream_t stream, int32_t* code);
