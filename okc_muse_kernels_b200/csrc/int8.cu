@@ -239,7 +239,9 @@ struct Int8MidParams {
 
 // The producer and the issuer run as whole warps with one elected lane acting: in code that only one thread runs, every
 // MMA costs it about 100 cycles (its operands go through vector registers), which with four MMAs and a commit a stage was
-// more than the stage's copy takes (K = 4096, N = 4096, 16 tokens, no split: 20.0 us).
+// more than the stage's copy takes (K = 4096, N = 4096, 16 tokens, no split: 20.0 us; as whole warps 10.4).
+// Bounded by the copies into the SMs for most sizes: 32 tokens, K = 4096, N = 7168 7.9 us (29.4 MB of weights), gated, 128
+// tokens, K = 7168, 2 x 2048 rows 10.3 us (29.4 MB), of which about 4 us are the launch and the sums' way through the cluster.
 template <bool kGated, int kSplits>
 __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constant__ Int8MidParams q) {
   extern __shared__ uint8_t smem_raw[];
@@ -504,6 +506,12 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here
 }
 
 // ------------------------------------------------------------------ many tokens
+// A pair of CTAs works on tiles of 256 tokens x bn weight rows: each CTA brings its 128 token rows and half of the weight
+// rows into shared memory, the leader issues the MMAs of both (cta_group::2), each keeps its rows of the sums in its own
+// tensor memory, two tiles side by side, so that the end of one tile runs under the next one's MMAs.  Half the operand
+// bytes a CTA against two single tiles is what the rate needs: 64 bytes a clock and SM at 256 x 256.
+// 4096 x 7168 x 7168: 127 us, 3.3e15 operations/s (twice the bf16 rate of the measured peaks is 3.25e15: bounded by the
+// tensor cores under the power limit); gated 4096 x 5120 x 2 x 2048 54 us, 3.2e15.
 constexpr int kManyThreads = 384;      // warps 0 TMA producer, 1 MMA issuer (leader CTA), 2 TMEM, 3 weight scales, 4..11 epilogue
 constexpr int kManyEpilogueWarps = 8;  // one warp a scheduler kept up with one instruction in five cycles only
 constexpr int kManyStages = 6;

@@ -123,10 +123,11 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_block_norm(const Blo
 // The same for many rows that 16-byte accesses can reach: persistent CTAs, each with a ring of rows in shared memory that
 // bulk copies fill ahead of it, so that HBM does not wait for the two dependent sums of a row.  What is left is issue
 // slots: pairs of f32 an instruction, and as many CTAs an SM as registers allow (the gains stay in L1, not in shared
-// memory, for that).  4096 x 5120, everything bf16, a gate per element: NORM_US us (NORM_TB TB/s); a CTA per row 65.1 us.
-constexpr int kStreamStages = 4, kStreamSmem = 200 * 1024;      // an SM's shared memory for rings
+// memory, for that).  4096 x 5120, everything bf16, a gate per element: 39.4 us (210 MB: 5.3 TB/s); a CTA per row 65.1 us.
+constexpr int kStreamStages = 2;                 // rows of a ring; more do not help (4096 x 4096: 2 / 3 / 8 rows 37.8 / 38.7 / 39.4 us)
+constexpr int kStreamSmem = 200 * 1024;          // an SM's shared memory for rings; L1 keeps the rest, for the gains
 template <int kChunks, bool kInt8>
-__global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream(const BlockNormParams p, int rows, int stages, int row_bytes) {
+__global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream(const BlockNormParams p, int rows, int row_bytes) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ uint64_t bar_full[kStreamStages];
   __shared__ int abort_code;
@@ -145,10 +146,10 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     if (gate_rows) bulk_g2s(dst + res_bytes + blk_bytes, static_cast<const uint8_t*>(p.gate) + row * p.gate_stride * (p.gate_f32 ? 4 : 2), gate_bytes, bar);
   };
   if (tid == 0) {
-    for (int i = 0; i < stages; ++i) mbar_init(smem_u32(&bar_full[i]), 1);
+    for (int i = 0; i < kStreamStages; ++i) mbar_init(smem_u32(&bar_full[i]), 1);
     abort_code = 0;
     mbar_fence_init();
-    for (int i = 0; i < stages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
+    for (int i = 0; i < kStreamStages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
   }
   __syncthreads();
   const float over_h = 1.f / static_cast<float>(H);
@@ -249,7 +250,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     }
     // every thread has read its part of the slot once it is past that sum's barrier
     if (!p.pre_gain || nt == 32) __syncthreads();
-    if (tid == 0 && row + static_cast<int64_t>(stages) * gridDim.x < rows) fetch(row + stages * gridDim.x, st);
+    if (tid == 0 && row + static_cast<int64_t>(kStreamStages) * gridDim.x < rows) fetch(row + kStreamStages * gridDim.x, st);
     if (p.pre_gain) {
       const F2 rstd2 = f2_pack(rstd, rstd);
       uint32_t amax = 0;
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
         if (tid == 0) p.out_scale[row] = s.scale;
       }
     }
-    if (++st == stages) { st = 0; ph ^= 1; }
+    if (++st == kStreamStages) { st = 0; ph ^= 1; }
   }
   __syncthreads();
   if (tid == 0 && abort_code != 0) {
@@ -301,10 +302,10 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
 
 // The same ring for rows of any width and alignment: a copy takes the 16-byte pieces that a row lies in (never past the
 // row's last piece, so never out of its allocation), and the threads find the row behind the bytes in front of it.
-// Neighbouring threads take neighbouring columns.  4096 x 5121, bf16, a gate per element: ANY_US us, a CTA per row with
+// Neighbouring threads take neighbouring columns.  4096 x 5121, bf16, a gate per element: 86.7 us, a CTA per row with
 // plain loads 138.5.
 template <int kChunks>
-__global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream_any(const BlockNormParams p, int rows, int stages, int row_bytes) {
+__global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream_any(const BlockNormParams p, int rows, int row_bytes) {
   extern __shared__ __align__(16) uint8_t ring[];
   constexpr int kVals = kChunks * 8;
   __shared__ uint64_t bar_full[kStreamStages];
@@ -355,10 +356,10 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     }
   };
   if (tid == 0) {
-    for (int i = 0; i < stages; ++i) mbar_init(smem_u32(&bar_full[i]), 1);
+    for (int i = 0; i < kStreamStages; ++i) mbar_init(smem_u32(&bar_full[i]), 1);
     abort_code = 0;
     mbar_fence_init();
-    for (int i = 0; i < stages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
+    for (int i = 0; i < kStreamStages && blockIdx.x + i * gridDim.x < static_cast<unsigned>(rows); ++i) fetch(blockIdx.x + i * gridDim.x, i);
   }
   __syncthreads();
   const float over_h = 1.f / static_cast<float>(H);
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     float rstd = 0.f;
     if (p.pre_gain) rstd = rsqrtf(cta_sum(ss, red_pre[n & 1]) * over_h + p.eps);
     if (!p.pre_gain || nt == 32) __syncthreads();
-    if (tid == 0 && row + static_cast<int64_t>(stages) * gridDim.x < rows) fetch(row + stages * gridDim.x, st);
+    if (tid == 0 && row + static_cast<int64_t>(kStreamStages) * gridDim.x < rows) fetch(row + kStreamStages * gridDim.x, st);
     if (p.pre_gain) {
       take(p.pre_gain, true, y);
 #pragma unroll
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
                 : static_cast<void*>(static_cast<uint16_t*>(p.out) + row * p.out_stride), f32, r);
       }
     }
-    if (++st == stages) { st = 0; ph ^= 1; }
+    if (++st == kStreamStages) { st = 0; ph ^= 1; }
   }
   __syncthreads();
   if (tid == 0 && abort_code != 0) {
@@ -549,7 +550,8 @@ static void row_shape(int64_t rows, int cols, int& threads, int& chunks) {
   if (threads > row_threads(chunks)) threads = row_threads(chunks);
 }
 
-// The streaming kernels, if the rows are many and a ring of two fits; false: not launched.
+// The streaming kernels, if the rows are many (4 an SM and more: bf16, a gate per channel, 500 / 600 rows of 4096 take 6.3 us
+// a CTA each and 7.2 streamed; at 4096 rows the streamed ones take 29.6 of 44) and a ring fits; false: not launched.
 static bool try_stream(const BlockNormParams& p, int64_t rows, bool vec, cudaStream_t stream, cudaError_t& e) {
   if (!p.blk || rows < 4 * 148 || rows > INT32_MAX / 2) return false;
   const int units = (p.H + 7) / 8;
@@ -558,15 +560,13 @@ static bool try_stream(const BlockNormParams& p, int64_t rows, bool vec, cudaStr
   const bool rows_gate = p.gate && p.gate_col_stride != 0 && p.gate_stride != 0;
   auto room = [&](int f32) { return vec ? p.H * (f32 ? 4 : 2) : (p.H * (f32 ? 4 : 2) + 30) & ~15; };
   const int row_bytes = room(p.res_f32) + room(p.blk_f32) + (rows_gate ? room(p.gate_f32) : 0);
-  // CTAs an SM by registers, then by shared memory; a ring of two, more do not help (4096 x 4096: 2 / 3 / 8 rows 37.8 /
-  // 38.7 / 39.4 us), and L1 keeps some room for the gains
+  // CTAs an SM by registers, then by shared memory
   const int regs = vec ? (chunks == 4 ? 96 : chunks == 2 ? 56 : 40) : (chunks == 4 ? 128 : 64);
   int per_sm = 65536 / (threads * regs);
   if (per_sm > 16) per_sm = 16;
   if (per_sm < 1) per_sm = 1;
-  while (per_sm > 1 && 2 * row_bytes * per_sm > kStreamSmem) --per_sm;
-  const int stages = 2;
-  const size_t smem = static_cast<size_t>(stages) * row_bytes;
+  while (per_sm > 1 && kStreamStages * row_bytes * per_sm > kStreamSmem) --per_sm;
+  const size_t smem = static_cast<size_t>(kStreamStages) * row_bytes;
   if (smem > kStreamSmem) return false;
   const int64_t most = 148LL * per_sm;
   const dim3 grid(static_cast<unsigned>(rows < most ? rows : most)), block(threads);
@@ -575,7 +575,7 @@ static bool try_stream(const BlockNormParams& p, int64_t rows, bool vec, cudaStr
               : q ? (chunks == 1 ? okc_block_norm_stream<1, true> : chunks == 2 ? okc_block_norm_stream<2, true> : okc_block_norm_stream<4, true>)
                   : (chunks == 1 ? okc_block_norm_stream<1, false> : chunks == 2 ? okc_block_norm_stream<2, false> : okc_block_norm_stream<4, false>);
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (e == cudaSuccess) e = launch_kernel(kernel, grid, block, smem, stream, false, p, static_cast<int>(rows), stages, row_bytes);
+  if (e == cudaSuccess) e = launch_kernel(kernel, grid, block, smem, stream, false, p, static_cast<int>(rows), row_bytes);
   return true;
 }
 
