@@ -5,7 +5,7 @@
 // below turns it into the result with the same f32 operations: a token's bits do not depend on the batch it is in.
 //
 // Three kernels, by what bounds the product:
-//   okc_int8_one   one token        the weights are read by plain 16-byte loads and multiplied on the integer dot-product
+//   okc_int8_one   one token        the weights stream through shared memory and are multiplied on the integer dot-product
 //                                   units; the token is quantised in the kernel (one launch)
 //   okc_int8_mid   to some hundred  the weights fill M of a tcgen05.mma (kind::i8), the tokens are N; K is split over a
 //                                   cluster of CTAs that add their integer sums through distributed shared memory
@@ -33,9 +33,11 @@ __device__ __forceinline__ void store_out(const Int8Params& p, int64_t o, float 
 }
 
 // ------------------------------------------------------------------ one token
-constexpr int kOneThreads = 512;
-constexpr int kOneChunk = 512;         // K elements of one warp-wide 16-byte load
-constexpr int kOneRowsMax = 1024;      // most weight rows a CTA owns (its integer sums live in shared memory, with the token)
+constexpr int kOneWarps = 16;          // that multiply; one more brings the weights
+constexpr int kOneThreads = 32 * kOneWarps + 32;
+constexpr int kOneOutMax = 1024;       // most outputs of a CTA
+constexpr int kOneSlots = 32;
+constexpr int kOneSmem = 208 * 1024;
 
 // Eight values of the token at column i (zeros past K), as f32.
 __device__ __forceinline__ void one_load_x(const Int8Params& p, int i, float (&v)[8]) {
@@ -57,130 +59,172 @@ __device__ __forceinline__ void one_load_x(const Int8Params& p, int i, float (&v
     }
   }
 }
-// 16 bytes that are read once: past L1.
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
 
-// A CTA owns `rows_per_cta` neighbouring outputs and all of K.  Its threads quantise the token into shared memory (every
-// CTA the whole row: a few KB from L2, where another launch would take longer); a warp then keeps one 512-wide chunk of K,
-// its 16 bytes of the token in registers, and walks over the CTA's weight rows with one 16-byte load a lane and row, four
-// integer dot products, a warp sum, and one shared-memory add for eight rows.  Sixteen rows a warp are on their way at any
-// time (128 KB an SM), the first ones before the token has been looked at.  The 16 bytes at a row's end may reach past K,
-// never past the row's next 16-byte boundary; the token's bytes are zero there.
-// bf16 token, weights of three layers in turn: K = 4096, N = 4096 5.7 us (the quantiser and okc_int8_mid: 7.4), gated,
-// K = 7168, 2 x 2048 rows 8.2 (8.7); a token of 128 columns alone takes 4.5: launch, three dependent trips to memory.
+struct OneShape {
+  int outs;          // neighbouring outputs of a CTA
+  int group;         // pairs of weight rows of a ring slot
+  int slots;
+};
+
+// A CTA owns `outs` neighbouring outputs and all of K.  One warp starts bulk copies of the weight rows into a ring that
+// takes as much of them as shared memory holds (28 rows of 7168 bytes are all of a CTA's of 4096 outputs): what is on its
+// way is not bounded by registers, and it starts before the token has been looked at.  Meanwhile the other warps quantise
+// the token into shared memory (every CTA the whole row: a few KB from L2, where another launch would take longer).  Then
+// a warp takes a slot: pairs of rows (two neighbours, or a gate row and its up row) against the token, 16 bytes a lane of
+// each, integer dot products, one warp sum a row, and the outputs leave from there.
+// The 16 bytes at a row's end may reach past K, never past the row's next 16-byte boundary; the token is zero there.
+// bf16 token, weights of three layers in turn: K = 4096, N = 4096 4.3 us (the quantiser and okc_int8_mid: 7.4; rows held in
+// registers, 16 a warp on their way: 5.7), gated, K = 7168, 2 x 2048 rows 6.6 (8.7; 8.2);
+// a token and one weight tile alone take 3.3.
 template <bool kGated>
-__global__ void __launch_bounds__(kOneThreads) okc_int8_one(const Int8Params p, int rows_per_cta) {
+__global__ void __launch_bounds__(kOneThreads) okc_int8_one(const Int8Params p, const OneShape q) {
   extern __shared__ __align__(16) uint8_t one_smem[];
-  constexpr int kWarps = kOneThreads / 32, kAhead = 8;
-  __shared__ uint32_t amax_s[kWarps];
+  __shared__ uint64_t bar_full[kOneSlots], bar_empty[kOneSlots];
+  __shared__ uint32_t amax_s[kOneWarps];
+  __shared__ int abort_code;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kpad = (p.K + 15) & ~15;
-  uint8_t* const xq_s = one_smem;                            // [kpad] int8
-  int* const acc_s = reinterpret_cast<int*>(one_smem + kpad);     // [rows]
-  const int n0 = blockIdx.x * rows_per_cta;
-  const int nr = min(rows_per_cta, p.N - n0);
-  const int rows = kGated ? 2 * nr : nr;
-  const int chunks = (p.K + kOneChunk - 1) / kOneChunk;
-  const int step = min(chunks, kWarps);            // chunks under way at once
-  const int groups = kWarps / step;                // warps that share a chunk and take turns at its rows
-  const int group = warp / step;
-  int c = group < groups ? warp % step : chunks;
-  int k = c * kOneChunk + lane * 16;
-  auto load = [&](uint4 (&w)[kAhead], int r0) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int r = r0 + u * groups;
-      w[u] = make_uint4(0, 0, 0, 0);
-      if (r < rows && k < p.K) w[u] = ldg_stream(p.w + (!kGated || r < nr ? n0 + r : p.N + n0 + r - nr) * p.w_stride + k);
-    }
-  };
-  uint4 wa[kAhead], wb[kAhead];
-  load(wa, group);
-  load(wb, group + kAhead * groups);
-  // scales of the output this thread finishes first (most CTAs have no more outputs than threads)
-  const int n_mine = n0 + tid % nr;
-  const float sw_mine = p.w_scale[n_mine], su_mine = kGated ? p.w_scale[p.N + n_mine] : 0.f;
+  const int n0 = blockIdx.x * q.outs, nr = min(q.outs, p.N - n0);
+  const int per_unit = kGated ? q.group : 2 * q.group;         // outputs of a slot
+  const int units = (nr + per_unit - 1) / per_unit;
+  const uint32_t slot_bytes = 2u * q.group * kpad;
+  uint8_t* const xq_s = one_smem;                              // [kpad] int8
+  uint8_t* const ring = xq_s + kpad;
+  float* const sw_s = reinterpret_cast<float*>(ring + static_cast<size_t>(q.slots) * slot_bytes);      // [outs] (gated: and [outs] of the up rows)
+  float* const sb_s = sw_s + q.outs;                           // bias or up rows' scales
+  const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
 
-  RowScale rs;
-  if (p.x_kind != kRowsInt8) {
-    uint32_t m = 0;
-    for (int i = tid * 8; i < p.K; i += kOneThreads * 8) {
-      float v[8];
-      one_load_x(p, i, v);
+  if (warp == kOneWarps) {
+    // unit u of weight rows into its slot, started by the calling thread
+    auto fetch = [&](int u, int slot) {
+      const int first = u * per_unit, v = min(per_unit, nr - first);
+      const uint32_t bar = full0 + 8 * slot, dst = smem_u32(ring) + slot * slot_bytes;
+      mbar_expect_tx(bar, static_cast<uint32_t>(kGated ? 2 * v : v) * kpad);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) amax_s[warp] = m;
-    __syncthreads();
-    rs = row_scale(__reduce_max_sync(0xffffffffu, amax_s[lane % kWarps]));
-    for (int i = tid * 8; i < kpad; i += kOneThreads * 8) {
-      float v[8];
-      one_load_x(p, i, v);
-      *reinterpret_cast<uint2*>(xq_s + i) = make_uint2(quant8x4(v[0], v[1], v[2], v[3], rs), quant8x4(v[4], v[5], v[6], v[7], rs));
-    }
-  } else {
-    rs.scale = p.x_scale[0];
-    for (int i = tid * 4; i < kpad; i += kOneThreads * 4) {
-      uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const int8_t*>(p.x) + i);
-      if (i + 4 > p.K) w = i < p.K ? w & ((1u << (8 * (p.K - i))) - 1u) : 0u;
-      *reinterpret_cast<uint32_t*>(xq_s + i) = w;
-    }
-  }
-  for (int i = tid; i < rows; i += kOneThreads) acc_s[i] = 0;
-  __syncthreads();
-  for (; c < chunks; c += step) {
-    const uint4 xq = k < p.K ? *reinterpret_cast<const uint4*>(xq_s + k) : make_uint4(0, 0, 0, 0);
-    auto use = [&](const uint4 (&w)[kAhead], int r0) {
-      if (r0 >= rows) return;
-      int mine = 0;
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        int d = __dp4a(static_cast<int>(w[u].x), static_cast<int>(xq.x), 0);
-        d = __dp4a(static_cast<int>(w[u].y), static_cast<int>(xq.y), d);
-        d = __dp4a(static_cast<int>(w[u].z), static_cast<int>(xq.z), d);
-        d = __dp4a(static_cast<int>(w[u].w), static_cast<int>(xq.w), d);
-        d = __reduce_add_sync(0xffffffffu, d);
-        if (lane == u) mine = d;
+      for (int half = 0; half < (kGated ? 2 : 1); ++half) {
+        const int8_t* src = p.w + (static_cast<int64_t>(half) * p.N + n0 + first) * p.w_stride;
+        const uint32_t to = dst + half * q.group * kpad;
+        if (p.w_stride == kpad) bulk_g2s(to, src, static_cast<uint32_t>(v) * kpad, bar);
+        else
+          for (int r = 0; r < v; ++r) bulk_g2s(to + r * kpad, src + r * p.w_stride, kpad, bar);
       }
-      const int r = r0 + lane * groups;
-      if (lane < kAhead && r < rows) atomicAdd(&acc_s[r], mine);
     };
-    for (int r0 = group; r0 < rows; r0 += 2 * kAhead * groups) {
-      use(wa, r0);
-      load(wa, r0 + 2 * kAhead * groups);
-      use(wb, r0 + kAhead * groups);
-      load(wb, r0 + 3 * kAhead * groups);
+    if (lane == 0) {
+      for (int i = 0; i < q.slots; ++i) { mbar_init(full0 + 8 * i, 1); mbar_init(empty0 + 8 * i, 1); }
+      abort_code = 0;
+      mbar_fence_init();
     }
-    k += step * kOneChunk;                                   // the next chunk of K, if this warp has one
-    if (c + step < chunks) {
-      load(wa, group);
-      load(wb, group + kAhead * groups);
+    __syncwarp();
+    if (lane < min(q.slots, units)) fetch(lane, lane);         // (at most 32 slots)
+    __syncwarp();
+    __syncthreads();
+    __syncthreads();
+    int slot = 0;
+    uint32_t ph = 0;
+    for (int u = q.slots; u < units; ++u) {
+      if (!mbar_wait(empty0 + 8 * slot, ph, &abort_code, 0x51)) break;
+      if (elect_one()) fetch(u, slot);
+      if (++slot == q.slots) { slot = 0; ph ^= 1; }
+    }
+    __syncwarp();
+  } else {
+    for (int j = tid; j < nr; j += 32 * kOneWarps) {
+      sw_s[j] = p.w_scale[n0 + j];
+      if (kGated) sb_s[j] = p.w_scale[p.N + n0 + j];
+      else if (p.bias) sb_s[j] = p.bias[n0 + j];
+    }
+    RowScale rs;
+    if (p.x_kind != kRowsInt8) {
+      uint32_t m = 0;
+      for (int i = tid * 8; i < p.K; i += 256 * kOneWarps) {
+        float v[8];
+        one_load_x(p, i, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+      }
+      m = __reduce_max_sync(0xffffffffu, m);
+      if (lane == 0) amax_s[warp] = m;
+      __syncthreads();
+      rs = row_scale(__reduce_max_sync(0xffffffffu, amax_s[lane % kOneWarps]));
+      for (int i = tid * 8; i < kpad; i += 256 * kOneWarps) {
+        float v[8];
+        one_load_x(p, i, v);
+        *reinterpret_cast<uint2*>(xq_s + i) = make_uint2(quant8x4(v[0], v[1], v[2], v[3], rs), quant8x4(v[4], v[5], v[6], v[7], rs));
+      }
+    } else {
+      rs.scale = p.x_scale[0];
+      for (int i = tid * 4; i < kpad; i += 128 * kOneWarps) {
+        uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const int8_t*>(p.x) + i);
+        if (i + 4 > p.K) w = i < p.K ? w & ((1u << (8 * (p.K - i))) - 1u) : 0u;
+        *reinterpret_cast<uint32_t*>(xq_s + i) = w;
+      }
+      __syncthreads();
+    }
+    __syncthreads();
+    // A parity wait tells phases one apart only, so a slot that is used again has to be the same warp's each time: with
+    // fewer slots than warps, as many warps work as there are slots.
+    const int step = min(q.slots, kOneWarps);
+    for (int u = warp < step ? warp : units; u < units; u += step) {
+      const int slot = u % q.slots;
+      if (!mbar_wait(full0 + 8 * slot, (u / q.slots) & 1, &abort_code, 0x52)) break;
+      const uint8_t* const base = ring + static_cast<size_t>(slot) * slot_bytes;
+      for (int g = 0; g < q.group; ++g) {
+        const int j = u * per_unit + (kGated ? g : 2 * g);     // the pair's (first) output
+        if (j >= nr) break;
+        const uint8_t* const a = base + (kGated ? g : 2 * g) * kpad;
+        const uint8_t* const b = kGated ? base + (q.group + g) * kpad : a + kpad;
+        int da = 0, db = 0;
+#pragma unroll 4
+        for (int k = lane * 16; k < kpad; k += 512) {
+          const uint4 x = *reinterpret_cast<const uint4*>(xq_s + k);
+          const uint4 wa = *reinterpret_cast<const uint4*>(a + k), wb = *reinterpret_cast<const uint4*>(b + k);
+          da = __dp4a(static_cast<int>(wa.x), static_cast<int>(x.x), da); db = __dp4a(static_cast<int>(wb.x), static_cast<int>(x.x), db);
+          da = __dp4a(static_cast<int>(wa.y), static_cast<int>(x.y), da); db = __dp4a(static_cast<int>(wb.y), static_cast<int>(x.y), db);
+          da = __dp4a(static_cast<int>(wa.z), static_cast<int>(x.z), da); db = __dp4a(static_cast<int>(wb.z), static_cast<int>(x.z), db);
+          da = __dp4a(static_cast<int>(wa.w), static_cast<int>(x.w), da); db = __dp4a(static_cast<int>(wb.w), static_cast<int>(x.w), db);
+        }
+        da = __reduce_add_sync(0xffffffffu, da);
+        db = __reduce_add_sync(0xffffffffu, db);               // (of a last row without a neighbour: not used)
+        if (kGated) {
+          if (lane == 0) store_out(p, n0 + j, silu_mul(int8_value(da, rs.scale, sw_s[j]), int8_value(db, rs.scale, sb_s[j])));
+        } else if (lane < 2 && j + lane < nr) {
+          float v = int8_value(lane ? db : da, rs.scale, sw_s[j + lane]);
+          if (p.bias) v = __fadd_rn(v, sb_s[j + lane]);
+          store_out(p, n0 + j + lane, v);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty0 + 8 * slot);
     }
   }
   __syncthreads();
-  for (int j = tid; j < nr; j += kOneThreads) {
-    const int n = n0 + j;
-    const bool first = j == tid;       // (n_mine is this output's column then)
-    float v = int8_value(acc_s[j], rs.scale, first ? sw_mine : p.w_scale[n]);
-    if (kGated) v = silu_mul(v, int8_value(acc_s[nr + j], rs.scale, first ? su_mine : p.w_scale[p.N + n]));
-    else if (p.bias) v = __fadd_rn(v, p.bias[n]);
-    store_out(p, n, v);
+  if (tid == 0 && abort_code != 0) {
+    atomicCAS(&g_int8_status, 0, abort_code);
+    const long long c0 = clock64();      // copies that are late get some time before the CTA's memory is another's
+    while (clock64() - c0 < kWaitLimitCycles / 100) {}
   }
 }
 
 cudaError_t launch_int8_one(const Int8Params& p, bool gated, cudaStream_t stream) {
-  int rpc = (p.N + 147) / 148;
-  const int most = gated ? kOneRowsMax / 2 : kOneRowsMax;
-  if (rpc > most) rpc = most;
-  const size_t smem = static_cast<size_t>(gated ? 2 : 1) * rpc * sizeof(int) + static_cast<size_t>((p.K + 15) & ~15);     // at most 20 KB
-  const dim3 grid((p.N + rpc - 1) / rpc), block(kOneThreads);
-  return gated ? launch_kernel(okc_int8_one<true>, grid, block, smem, stream, false, p, rpc)
-               : launch_kernel(okc_int8_one<false>, grid, block, smem, stream, false, p, rpc);
+  const int kpad = (p.K + 15) & ~15;
+  OneShape q;
+  q.outs = (p.N + 147) / 148;
+  if (q.outs > kOneOutMax) q.outs = kOneOutMax;
+  q.group = 4096 / kpad;               // short rows go several pairs to a slot
+  if (q.group < 1) q.group = 1;
+  if (q.group > 8) q.group = 8;
+  const int per_unit = gated ? q.group : 2 * q.group, units = (q.outs + per_unit - 1) / per_unit;
+  const int slot_bytes = 2 * q.group * kpad, scales = 8 * q.outs;
+  q.slots = (kOneSmem - kpad - scales) / slot_bytes;           // at K = 16384, the most, five
+  if (q.slots > kOneSlots) q.slots = kOneSlots;
+  if (q.slots > units) q.slots = units;
+  else if (q.slots > kOneWarps) q.slots = q.slots / kOneWarps * kOneWarps;     // a slot that is used again is always the same warp's
+  const size_t smem = static_cast<size_t>(kpad) + static_cast<size_t>(q.slots) * slot_bytes + scales;
+  const dim3 grid((p.N + q.outs - 1) / q.outs), block(kOneThreads);
+  auto kernel = gated ? okc_int8_one<true> : okc_int8_one<false>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  return launch_kernel(kernel, grid, block, smem, stream, false, p, q);
 }
 
 // ------------------------------------------------------------------ tcgen05 pieces shared by the two tiled kernels

@@ -125,7 +125,7 @@ def test_quantize_rows_strided_and_unaligned_input():
 
 
 # ------------------------------------------------------------------------------------------------ products
-SHAPES = [(1, 1, 1), (1, 16384, 40), (1, 16385, 9), (1, 9001, 1200), (1, 520, 3001), (1, 64, 160000), (2, 520, 3001), (1, 16, 5), (2, 511, 130), (3, 513, 7), (5, 1000, 301), (8, 4100, 149), (1, 20000, 33), (4, 16400, 64),
+SHAPES = [(1, 1, 1), (1, 16384, 40), (1, 16385, 9), (1, 9001, 1200), (1, 520, 3001), (1, 64, 160000), (1, 16384, 1500), (1, 5000, 9000), (1, 2048, 20000), (1, 300, 700), (1, 12000, 2960), (2, 520, 3001), (1, 16, 5), (2, 511, 130), (3, 513, 7), (5, 1000, 301), (8, 4100, 149), (1, 20000, 33), (4, 16400, 64),
           (9, 1, 1), (9, 128, 128), (16, 129, 127), (17, 1000, 301), (40, 4096, 640), (65, 333, 1000), (130, 2048, 257), (256, 520, 384),
           (257, 17, 3), (257, 128, 256), (300, 1000, 301), (513, 2047, 129), (1025, 640, 2050)]
 
@@ -209,7 +209,7 @@ def test_rows_that_are_not_finite_or_empty(T):
     assert not h[0].any() and h[1:3].isnan().all() and torch.isfinite(h[3:]).all()
 
 
-@pytest.mark.parametrize("T", [1, 6, 50, 400])
+@pytest.mark.parametrize("T", [1, 2, 6, 50, 400])
 def test_strides_padding_and_rows_behind_the_last(T):
     g = _gen(T + 77)
     K, N = 200, 120
