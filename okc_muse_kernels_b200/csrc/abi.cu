@@ -714,7 +714,7 @@ uint64_t okc_moe_int8_scratch_bytes(int x_kind, int32_t tokens, int32_t k) {
 static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   if (!a || a->tokens < 0 || a->k <= 0 || a->n <= 0 || a->x_kind < 0 || a->x_kind > 2) return OKC_ERR_BAD_ARG;
-  if (a->k > kInt8MaxK || a->n > (1 << 30)) return OKC_ERR_TOO_LARGE;
+  if (a->k > kInt8MaxK || a->n > (1 << 30) || a->tokens > (1 << 30)) return OKC_ERR_TOO_LARGE;
   if (a->tokens == 0) return OKC_OK;
   const int T = a->tokens, K = a->k, N = a->n;
   if (!a->x || !a->w || !a->w_scale || !a->out || (gated && a->bias)) return OKC_ERR_BAD_ARG;

@@ -107,6 +107,7 @@ def _int8_args(**kw):
 
 @pytest.mark.parametrize("kw,rc", [
     (dict(tokens=0), OK), (dict(tokens=-1), BAD), (dict(k=0), BAD), (dict(n=0), BAD), (dict(k=131072, x_stride=131072, w_stride=131072), LARGE),
+    (dict(tokens=(1 << 30) + 1), LARGE), (dict(n=(1 << 30) + 1, out_stride=1 << 31), LARGE),
     (dict(x=None), BAD), (dict(w=None), BAD), (dict(w_scale=None), BAD), (dict(out=None), BAD), (dict(scratch=None), BAD),
     (dict(w=0x2008), BAD), (dict(w_stride=72), BAD), (dict(w_stride=48), BAD), (dict(x_stride=63), BAD), (dict(out_stride=31), BAD),
     (dict(x=0x1001), BAD), (dict(x=0x1002, x_kind=1), BAD), (dict(out=0x4001), BAD), (dict(out=0x4002, out_f32=1), BAD), (dict(w_scale=0x3002), BAD),
