@@ -276,9 +276,10 @@ constexpr int kKb = 128;               // K elements of a stage: one 128-byte sw
 constexpr int kTileW = 128;            // weight rows of a tile
 
 struct Int8MidParams {
-  CUtensorMap wmap;      // int8 weight rows, box 128 x 128 rows (64 for the gated product: a gate and an up box)
+  CUtensorMap wmap;      // int8 weight rows, box 128 x outs rows (gated: a gate and an up box)
   CUtensorMap xmap;      // int8 token rows, box 128 x tn
   Int8Params p;
+  int outs;              // outputs of a tile: a multiple of 4, at most 128, gated 64 (the MMA's other rows are not looked at)
   int tn, stages, n_kb, tmem_cols;
 };
 
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   const Int8Params& p = q.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x % kSplits, tile = blockIdx.x / kSplits;
-  const int w0 = tile * (kGated ? kTileW / 2 : kTileW);      // first output of the tile
+  const int w0 = tile * q.outs;      // first output of the tile
   const int t0 = blockIdx.y * q.tn;
   const int kb0 = static_cast<int>(static_cast<long long>(q.n_kb) * rank / kSplits);
   const int nkb = static_cast<int>(static_cast<long long>(q.n_kb) * (rank + 1) / kSplits) - kb0;
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     auto load_w = [&](int i, uint32_t st) {
       const uint32_t bar = full0 + 8 * st, dst = smem0 + st * stage_bytes;
       if (elect_one()) {
-        mbar_expect_tx(bar, stage_bytes);
+        mbar_expect_tx(bar, static_cast<uint32_t>((kGated ? 2 : 1) * q.outs + q.tn) * kKb);
         tma_2d_g2s(dst, &q.wmap, (kb0 + i) * kKb, w0, bar);
         if (kGated) tma_2d_g2s(dst + kTileW / 2 * kKb, &q.wmap, (kb0 + i) * kKb, p.N + w0, bar);
       }
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     const int* src[kSplits];
 #pragma unroll
     for (int s = 0; s < kSplits; ++s) src[s] = (kSplits > 1 ? cluster.map_shared_rank(part, s) : part) + o4;
-    const int per = q.tn / kSplits, last = min((rank + 1) * per, p.T - t0);
+    const int per = q.tn / kSplits, last = o4 < q.outs ? min((rank + 1) * per, p.T - t0) : 0;
 #pragma unroll 2
     for (int col = rank * per + tid / kQuads; col < last; col += kMidThreads / kQuads) {
       int4 a[kSplits], b[kSplits];
@@ -470,7 +471,7 @@ static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 
 // 7168, plain and gated), where the two differ by up to 2 either way, the choice costs 0.14 % of the better one's time on
 // average and 13 % at worst.
 struct TileShape {
-  int tokens;        // mid: tokens of a tile
+  int tokens, outs;  // mid: tokens and outputs of a tile
   int t_tiles, tiles, splits;
   int bn;            // many: weight rows of a tile
   double us;
@@ -481,18 +482,31 @@ static double stage_us(double alone, double kbytes, double ctas) {
 }
 static TileShape mid_shape(int T, int K, int N, bool gated) {
   TileShape s = {};
-  const int per_tile = gated ? kTileW / 2 : kTileW, n_kb = (K + kKb - 1) / kKb;
-  s.tiles = (N + per_tile - 1) / per_tile;
+  const int most = gated ? kTileW / 2 : kTileW, n_kb = (K + kKb - 1) / kKb;
+  s.outs = most;
+  s.tiles = (N + most - 1) / most;
   s.t_tiles = (T + 255) / 256;
   s.tokens = ((T + s.t_tiles - 1) / s.t_tiles + 15) & ~15;
   // As many CTAs a cluster as one round of them fits the SMs (a cluster lives in one group of 16 to 20 SMs: 33 clusters of
   // 4 and 15 of 8 fit at once).  K = 4096, N = 4096, 16 tokens (32 tiles), 1 / 2 / 4 / 8 CTAs a cluster: 10.5 / 7.8 / 6.6 /
   // 13.9 us; gated, K = 7168, 2 x 2048 rows, 128 tokens: 18.4 / 12.9 / 10.6 / 26.0 us.
   const int64_t clusters = static_cast<int64_t>(s.tiles) * s.t_tiles;
-  s.splits = clusters <= 14 ? 8 : clusters <= 32 ? 4 : clusters <= 74 ? 2 : 1;
+  const int fit = clusters <= 14 ? 14 : clusters <= 32 ? 32 : clusters <= 74 ? 74 : 148;
+  s.splits = fit == 14 ? 8 : fit == 32 ? 4 : fit == 74 ? 2 : 1;
   while (s.splits > n_kb) s.splits /= 2;
-  const double ctas = static_cast<double>(clusters) * s.splits, rounds = static_cast<double>((clusters * s.splits + 147) / 148);
-  s.us = 3.0 + rounds * (0.021 * s.tokens + (n_kb + s.splits - 1) / s.splits * stage_us(0.21, 16 + s.tokens / 8.0, ctas));
+  // Tiles of fewer weight rows, down to half, where SMs had none.  K = 7168, N = 512, 128 tokens: 8 tiles of 64 in place of 4
+  // of 128, 7.6 us in place of 8.7; K = 1024, N = 2048, 16 tokens: 32 of 64, 4.6 in place of 4.8; gated, K = 1000, 2 x 523 rows,
+  // 77 tokens: 14 of 40, 6.1 in place of 6.6.  With clusters of 2 it gained nothing (K = 4096, N = 5120: 11.2 against 11.0).
+  if (clusters < fit && s.splits >= 4) {
+    const int tiles = fit / s.t_tiles;
+    int outs = ((N + tiles - 1) / tiles + 3) & ~3;
+    if (outs < most / 2) outs = most / 2;
+    if (outs < s.outs) { s.outs = outs; s.tiles = (N + outs - 1) / outs; }
+  }
+  const double ctas = static_cast<double>(s.tiles) * s.t_tiles * s.splits;
+  const double rounds = static_cast<double>((static_cast<int64_t>(s.tiles) * s.t_tiles * s.splits + 147) / 148);
+  const double kbytes = (gated ? 2 : 1) * s.outs / 8.0 + s.tokens / 8.0;
+  s.us = 3.0 + rounds * (0.021 * s.tokens + (n_kb + s.splits - 1) / s.splits * stage_us(0.21, kbytes, ctas));
   return s;
 }
 static TileShape many_shape(int T, int K, int N, bool gated) {
@@ -518,14 +532,15 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here
   Int8MidParams q;
   q.p = p;
   const TileShape shape = mid_shape(p.T, p.K, p.N, gated);
-  const int per_tile = gated ? kTileW / 2 : kTileW, tiles = shape.tiles, ttiles = shape.t_tiles, splits = shape.splits;
+  const int tiles = shape.tiles, ttiles = shape.t_tiles, splits = shape.splits;
+  q.outs = shape.outs;
   q.tn = shape.tokens;
   q.n_kb = (p.K + kKb - 1) / kKb;
   const int stage = kTileW * kKb + q.tn * kKb;
   q.stages = 216 * 1024 / stage;
   if (q.stages > kMidMaxStages) q.stages = kMidMaxStages;
   q.tmem_cols = tmem_cols_for(q.tn);
-  if (!encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(gated ? 2 : 1) * p.N, p.K, p.w_stride, per_tile) ||
+  if (!encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(gated ? 2 : 1) * p.N, p.K, p.w_stride, q.outs) ||
       !encode_bytes_map(&q.xmap, p.x, p.T, p.K, p.x_stride, q.tn))
     return cudaErrorInvalidValue;
   size_t smem = 1024 + static_cast<size_t>(q.stages) * stage;
