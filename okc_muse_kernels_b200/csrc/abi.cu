@@ -55,6 +55,23 @@ bool encode_bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The same rows as [K / 128 blocks][halves][rows][128], box = blocks x halves x box_rows x 128, for copies of several
+// blocks (K a multiple of 128 then; box_rows of 8); one block: as above, the halves as rows.
+bool encode_blocks_map(CUtensorMap* map, const void* base, uint64_t rows, uint32_t halves, uint64_t K, uint64_t row_stride,
+                       uint32_t box_rows, uint32_t blocks) {
+  if (blocks == 1) return encode_bytes_map(map, base, rows * halves, K, row_stride, box_rows);
+  EncodeFn f = encode_fn();
+  if (!f || K % 128) return false;
+  const int rank = halves == 1 ? 3 : 4;
+  cuuint64_t dims[4] = {128, rows, halves, K / 128}, strides[3] = {row_stride, rows * row_stride, 128};
+  cuuint32_t box[4] = {128, box_rows, halves, blocks};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  if (rank == 3) { dims[2] = dims[3]; strides[1] = strides[2]; box[2] = box[3]; }
+  return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool encode_bf16_out_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t row_stride) {
   EncodeFn f = encode_fn();
   if (!f) return false;

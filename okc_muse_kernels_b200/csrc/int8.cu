@@ -271,24 +271,31 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 }
 // ------------------------------------------------------------------ some hundred tokens
 constexpr int kMidThreads = 256;       // warps 0..3 read the accumulator, 4 TMA producer, 5 MMA issuer; all finish the rows
-constexpr int kMidMaxStages = 8;
+constexpr int kMidMaxStages = 16;
+constexpr int kMidRing = 216 * 1024;
+constexpr int kMidMinSmem = 116 * 1024;      // one CTA an SM: clusters cannot wait for each other's tensor memory
+constexpr int kMidMaxBlocks = 8;       // most K blocks of a stage
 constexpr int kKb = 128;               // K elements of a stage: one 128-byte swizzled row
 constexpr int kTileW = 128;            // weight rows of a tile
 
 struct Int8MidParams {
-  CUtensorMap wmap;      // int8 weight rows, box 128 x outs rows (gated: a gate and an up box)
-  CUtensorMap xmap;      // int8 token rows, box 128 x tn
+  CUtensorMap wmap;      // int8 weight rows: [block] (gated: [gate, up]) [outs rows] [128]; of single blocks 2D, box 128 x outs rows
+  CUtensorMap xmap;      // int8 token rows: [block] [tn rows] [128]
   Int8Params p;
-  int outs;              // outputs of a tile: a multiple of 4, at most 128, gated 64 (the MMA's other rows are not looked at)
+  int outs;              // outputs of a tile: a multiple of 8, at most 128, gated 64 (the MMA's other rows are not looked at)
+  int blocks;            // K blocks of 128 a stage
   int tn, stages, n_kb, tmem_cols;
 };
 
-// The producer and the issuer run as whole warps with one elected lane acting: in code that only one thread runs, every
+// The producers and the issuer run as whole warps with one elected lane acting: in code that only one thread runs, every
 // MMA costs it about 100 cycles (its operands go through vector registers), which with four MMAs and a commit a stage was
 // more than the stage's copy takes (K = 4096, N = 4096, 16 tokens, no split: 20.0 us; as whole warps 10.4).
+// A copy costs an SM some 150 cycles besides its bytes, however many warps issue them, so a stage takes several K blocks with
+// one copy of weights and one of tokens (8 tokens, K = 7168, N = 2048, blocks 1 / 2 / 7: 7.9 / 7.4 / 6.5 us; gated, 32 tokens,
+// K = 4096, 2 x 2560 rows, 1 / 2 / 4: 8.6 / 8.0 / 7.0), and the first weights are on their way before the CTA has set itself up.
 // Bounded by the copies into the SMs for most sizes: 32 tokens, K = 4096, N = 7168 7.9 us (29.4 MB of weights), gated, 128
-// tokens, K = 7168, 2 x 2048 rows 10.3 us (29.4 MB), of which about 4 us are the launch and the sums' way through the cluster.
-template <bool kGated, int kSplits>
+// tokens, K = 7168, 2 x 2048 rows 10.5 us (29.4 MB), of which about 4 us are the launch and the sums' way through the cluster.
+template <bool kGated, int kSplits, bool kSingle>      // kSingle: one K block a stage
 __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constant__ Int8MidParams q) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = smem_u32(smem_raw);
@@ -304,15 +311,48 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   const int t0 = blockIdx.y * q.tn;
   const int kb0 = static_cast<int>(static_cast<long long>(q.n_kb) * rank / kSplits);
   const int nkb = static_cast<int>(static_cast<long long>(q.n_kb) * (rank + 1) / kSplits) - kb0;
-  const uint32_t stage_bytes = kTileW * kKb + static_cast<uint32_t>(q.tn) * kKb;
+  const int blocks = kSingle ? 1 : q.blocks;
+  const int nst = (nkb + blocks - 1) / blocks, first = min(nst, q.stages);
+  const int a_rows = kGated ? 2 * q.outs : q.outs;
+  const uint32_t a_bytes = static_cast<uint32_t>(a_rows) * kKb, x_bytes = static_cast<uint32_t>(q.tn) * kKb;
+  const uint32_t a_stage = a_bytes * blocks, x_stage = x_bytes * blocks, stage_bytes = a_stage + x_stage;
+  const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
 
-  if (tid == 0) {
-    for (int i = 0; i < kMidMaxStages; ++i) { mbar_init(smem_u32(&bar_full[i]), 1); mbar_init(smem_u32(&bar_empty[i]), 1); }
-    mbar_init(smem_u32(&bar_done), 1);
-    abort_code = 0;
-    mbar_fence_init();
-  }
+  auto load_w = [&](int i, uint32_t st) {
+    const uint32_t bar = full0 + 8 * st, dst = smem0 + st * stage_bytes;
+    const int kb = kb0 + i * blocks;
+    if (elect_one()) {
+      mbar_expect_tx(bar, a_stage);
+      if (!kSingle) {
+        if (kGated) tma_4d_g2s(dst, &q.wmap, 0, w0, 0, kb, bar);
+        else tma_3d_g2s(dst, &q.wmap, 0, w0, kb, bar);
+      } else {
+        tma_2d_g2s(dst, &q.wmap, kb * kKb, w0, bar);
+        if (kGated) tma_2d_g2s(dst + q.outs * kKb, &q.wmap, kb * kKb, p.N + w0, bar);
+      }
+    }
+  };
+  auto load_x = [&](int i, uint32_t st) {
+    const uint32_t bar = full0 + 8 * st, dst = smem0 + st * stage_bytes + a_stage;
+    const int kb = kb0 + i * blocks;
+    if (elect_one()) {
+      mbar_expect_tx(bar, x_stage);
+      if (!kSingle) tma_3d_g2s(dst, &q.xmap, 0, t0, kb, bar);
+      else tma_2d_g2s(dst, &q.xmap, kb * kKb, t0, bar);
+    }
+  };
   if (warp == 4) {
+    if (lane == 0) {
+      for (int i = 0; i < q.stages; ++i) { mbar_init(full0 + 8 * i, 2); mbar_init(empty0 + 8 * i, 1); }
+      mbar_init(smem_u32(&bar_done), 1);
+      abort_code = 0;
+      mbar_fence_init();
+    }
+    __syncwarp();
+    // the weights do not depend on the kernel before this one, the token rows may
+    for (int i = 0; i < first; ++i) load_w(i, i);
+    __syncwarp();
+  } else if (warp == 5) {
     tmem_alloc(smem_u32(&tmem_base_s), static_cast<uint32_t>(q.tmem_cols));
     tmem_relinquish();
   }
@@ -320,7 +360,6 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
-  const uint32_t full0 = smem_u32(&bar_full[0]), empty0 = smem_u32(&bar_empty[0]);
   cg::cluster_group cluster = cg::this_cluster();
   int* const part = reinterpret_cast<int*>(smem_raw + (smem0 - smem_base));
   // a thread finishes four neighbouring outputs of every few tokens
@@ -335,32 +374,20 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     else if (p.bias) sb[j] = in ? __ldg(p.bias + n + j) : 0.f;
   }
 
-  if (warp == 4) {
-    auto load_w = [&](int i, uint32_t st) {
-      const uint32_t bar = full0 + 8 * st, dst = smem0 + st * stage_bytes;
-      if (elect_one()) {
-        mbar_expect_tx(bar, static_cast<uint32_t>((kGated ? 2 : 1) * q.outs + q.tn) * kKb);
-        tma_2d_g2s(dst, &q.wmap, (kb0 + i) * kKb, w0, bar);
-        if (kGated) tma_2d_g2s(dst + kTileW / 2 * kKb, &q.wmap, (kb0 + i) * kKb, p.N + w0, bar);
-      }
-    };
-    auto load_x = [&](int i, uint32_t st) {
-      if (elect_one()) tma_2d_g2s(smem0 + st * stage_bytes + kTileW * kKb, &q.xmap, (kb0 + i) * kKb, t0, full0 + 8 * st);
-    };
-    // the weights of the first stages do not depend on the kernel before this one, the token rows may
-    const int first = min(nkb, q.stages);
-    for (int i = 0; i < first; ++i) load_w(i, i);
-    griddep_wait();
-    for (int i = 0; i < first; ++i) load_x(i, i);
+  if (warp == 4 || warp == 6) {
+    const bool tokens = warp == 6;
     int i = first;
+    if (tokens) {
+      griddep_wait();
+      for (i = 0; i < first; ++i) load_x(i, i);
+    }
     uint32_t st = 0, ph = 0;
-    for (; i < nkb; ++i) {
+    for (; i < nst; ++i) {
       if (!mbar_wait(empty0 + 8 * st, ph, &abort_code, 0x61)) break;
-      load_w(i, st);
-      load_x(i, st);
+      if (tokens) load_x(i, st); else load_w(i, st);
       if (++st == static_cast<uint32_t>(q.stages)) { st = 0; ph ^= 1; }
     }
-    if (i < nkb) {
+    if (i < nst) {
       // giving up: the copies in flight get a bounded chance to land before the CTA retires
       const long long c0 = clock64();
       for (int j = max(0, i - q.stages); j < i; ++j)
@@ -370,18 +397,23 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   } else if (warp == 5) {
     const uint32_t idesc = idesc_i8(128, static_cast<uint32_t>(q.tn));
     const uint32_t lo0 = desc_lo(smem0);
-    uint32_t st = 0, ph = 0;
-    for (int i = 0; i < nkb; ++i) {
+    uint32_t st = 0, ph = 0, more = 0;
+    for (int left = nkb; left > 0; left -= blocks) {
       if (!mbar_wait(full0 + 8 * st, ph, &abort_code, 0x62)) break;
       tc_fence_after();
-      const uint32_t a = lo0 + st * (stage_bytes >> 4), b = a + (kTileW * kKb >> 4);
-      if (elect_one()) {
-        mma_i8(tmem, a, b, kDescHi, idesc, i != 0);          // K = 32 each: 32 bytes further along the swizzled rows
-        mma_i8(tmem, a + 2, b + 2, kDescHi, idesc, 1);
-        mma_i8(tmem, a + 4, b + 4, kDescHi, idesc, 1);
-        mma_i8(tmem, a + 6, b + 6, kDescHi, idesc, 1);
-        mma_commit(empty0 + 8 * st);
+      uint32_t a = lo0 + st * (stage_bytes >> 4), b = a + (a_stage >> 4);
+      for (int j = min(left, blocks); j > 0; --j) {
+        if (elect_one()) {
+          mma_i8(tmem, a, b, kDescHi, idesc, more);          // K = 32 each: 32 bytes further along the swizzled rows
+          mma_i8(tmem, a + 2, b + 2, kDescHi, idesc, 1);
+          mma_i8(tmem, a + 4, b + 4, kDescHi, idesc, 1);
+          mma_i8(tmem, a + 6, b + 6, kDescHi, idesc, 1);
+        }
+        more = 1;
+        a += a_bytes >> 4;
+        b += x_bytes >> 4;
       }
+      if (elect_one()) mma_commit(empty0 + 8 * st);
       if (++st == static_cast<uint32_t>(q.stages)) { st = 0; ph ^= 1; }
     }
     if (elect_one()) mma_commit(smem_u32(&bar_done));
@@ -391,7 +423,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     for (int i = tid; i < q.tn; i += 128) xs[i] = t0 + i < p.T ? p.x_scale[t0 + i] : 0.f;
     const bool ok = mbar_wait<20>(smem_u32(&bar_done), 0, &abort_code, 0x63);
     tc_fence_after();
-    if (ok) {
+    if (ok && warp * 32 < a_rows) {
       // this CTA's sums, [token][weight row], over the ring slots (every copy has landed and every MMA has read them)
       const uint32_t taddr = tmem + (static_cast<uint32_t>(warp * 32) << 16);
       int* mine = part + warp * 32 + lane;
@@ -428,7 +460,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
 #pragma unroll
       for (int s = 0; s < kSplits; ++s) {
         a[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW);
-        if (kGated) b[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW + kTileW / 2);
+        if (kGated) b[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW + q.outs);
       }
 #pragma unroll
       for (int s = 1; s < kSplits; ++s) {
@@ -456,7 +488,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     }
   }
   if (kSplits > 1) cluster.sync(); else __syncthreads();   // no CTA leaves while another reads its sums
-  if (warp == 4) {
+  if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, static_cast<uint32_t>(q.tmem_cols));
   }
@@ -471,7 +503,7 @@ static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 
 // 7168, plain and gated), where the two differ by up to 2 either way, the choice costs 0.14 % of the better one's time on
 // average and 13 % at worst.
 struct TileShape {
-  int tokens, outs;  // mid: tokens and outputs of a tile
+  int tokens, outs, blocks;      // mid: tokens and outputs of a tile, K blocks of a stage
   int t_tiles, tiles, splits;
   int bn;            // many: weight rows of a tile
   double us;
@@ -494,15 +526,26 @@ static TileShape mid_shape(int T, int K, int N, bool gated) {
   const int fit = clusters <= 14 ? 14 : clusters <= 32 ? 32 : clusters <= 74 ? 74 : 148;
   s.splits = fit == 14 ? 8 : fit == 32 ? 4 : fit == 74 ? 2 : 1;
   while (s.splits > n_kb) s.splits /= 2;
-  // Tiles of fewer weight rows, down to half, where SMs had none.  K = 7168, N = 512, 128 tokens: 8 tiles of 64 in place of 4
-  // of 128, 7.6 us in place of 8.7; K = 1024, N = 2048, 16 tokens: 32 of 64, 4.6 in place of 4.8; gated, K = 1000, 2 x 523 rows,
-  // 77 tokens: 14 of 40, 6.1 in place of 6.6.  With clusters of 2 it gained nothing (K = 4096, N = 5120: 11.2 against 11.0).
-  if (clusters < fit && s.splits >= 4) {
+  // Tiles of fewer weight rows, down to half, where many SMs had none.  K = 7168, N = 512, 128 tokens: 8 tiles of 64 in place
+  // of 4 of 128, 7.6 us in place of 8.7; gated, K = 4096, 2 x 2560 rows, 32 tokens: 64 of 40 in place of 40, 7.1 in place of 7.5.
+  // Not for fewer SMs (K = 4096, N = 7168, 128 tokens, 69 in place of 56: 11.7 against 11.6) or more tokens, which each tile
+  // copies (K = 4096, N = 5120, 200 tokens: 13.2 against 12.5).
+  if (clusters * 4 <= fit * 3 && s.tokens <= 128) {
     const int tiles = fit / s.t_tiles;
-    int outs = ((N + tiles - 1) / tiles + 3) & ~3;
+    int outs = ((N + tiles - 1) / tiles + 7) & ~7;
     if (outs < most / 2) outs = most / 2;
     if (outs < s.outs) { s.outs = outs; s.tiles = (N + outs - 1) / outs; }
   }
+  // K blocks of a stage: what a third of the ring takes, two (which gain less) a quarter (128 tokens, K = 4096, N = 7168, of
+  // 32 KB a block: 11.7 us with two, 11.3 with one), in stages of equal size, two at least.  Only whole blocks can go several
+  // to a copy.
+  const int per = (n_kb + s.splits - 1) / s.splits, block = ((gated ? 2 : 1) * s.outs + s.tokens) * kKb;
+  s.blocks = K % kKb ? 1 : kMidRing / 3 / block;
+  if (s.blocks < 3 && s.blocks > kMidRing / 4 / block) s.blocks = kMidRing / 4 / block;
+  if (s.blocks > (per + 1) / 2) s.blocks = (per + 1) / 2;
+  if (s.blocks > kMidMaxBlocks) s.blocks = kMidMaxBlocks;
+  if (s.blocks < 1) s.blocks = 1;
+  s.blocks = (per + (per + s.blocks - 1) / s.blocks - 1) / ((per + s.blocks - 1) / s.blocks);
   const double ctas = static_cast<double>(s.tiles) * s.t_tiles * s.splits;
   const double rounds = static_cast<double>((static_cast<int64_t>(s.tiles) * s.t_tiles * s.splits + 147) / 148);
   const double kbytes = (gated ? 2 : 1) * s.outs / 8.0 + s.tokens / 8.0;
@@ -528,6 +571,13 @@ static TileShape many_shape(int T, int K, int N, bool gated) {
   return s;
 }
 
+using MidKernel = void (*)(const Int8MidParams);
+template <bool kGated, bool kSingle>
+static MidKernel mid_kernel(int splits) {
+  return splits == 1 ? okc_int8_mid<kGated, 1, kSingle> : splits == 2 ? okc_int8_mid<kGated, 2, kSingle>
+       : splits == 4 ? okc_int8_mid<kGated, 4, kSingle> : okc_int8_mid<kGated, 8, kSingle>;
+}
+
 cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream) {
   Int8MidParams q;
   q.p = p;
@@ -536,18 +586,25 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here
   q.outs = shape.outs;
   q.tn = shape.tokens;
   q.n_kb = (p.K + kKb - 1) / kKb;
-  const int stage = kTileW * kKb + q.tn * kKb;
-  q.stages = 216 * 1024 / stage;
+  q.blocks = shape.blocks;
+  const int a_bytes = (gated ? 2 : 1) * q.outs * kKb, x_bytes = q.tn * kKb, stage = (a_bytes + x_bytes) * q.blocks;
+  q.stages = kMidRing / stage;
   if (q.stages > kMidMaxStages) q.stages = kMidMaxStages;
+  const int most = (q.n_kb + splits * q.blocks - 1) / (splits * q.blocks) + 1;      // stages of a CTA (or one more)
+  if (q.stages > most) q.stages = most;
   q.tmem_cols = tmem_cols_for(q.tn);
-  if (!encode_bytes_map(&q.wmap, p.w, static_cast<uint64_t>(gated ? 2 : 1) * p.N, p.K, p.w_stride, q.outs) ||
-      !encode_bytes_map(&q.xmap, p.x, p.T, p.K, p.x_stride, q.tn))
+  if (!encode_blocks_map(&q.wmap, p.w, p.N, gated ? 2 : 1, p.K, p.w_stride, q.outs, q.blocks) ||
+      !encode_blocks_map(&q.xmap, p.x, p.T, 1, p.K, p.x_stride, q.tn, q.blocks))
     return cudaErrorInvalidValue;
-  size_t smem = 1024 + static_cast<size_t>(q.stages) * stage;
+  // the MMA reads 128 rows, of the last block past the stage's end where a tile has fewer
+  const int past = kTileW * kKb - a_bytes - x_bytes * q.blocks;
+  size_t smem = 1024 + static_cast<size_t>(q.stages) * stage + (past > 0 ? past : 0);
+  if (smem < kMidMinSmem) smem = kMidMinSmem;
   const size_t sums = 1024 + static_cast<size_t>(q.tn) * kTileW * 4;
   if (smem < sums) smem = sums;
-  auto kernel = gated ? (splits == 1 ? okc_int8_mid<true, 1> : splits == 2 ? okc_int8_mid<true, 2> : splits == 4 ? okc_int8_mid<true, 4> : okc_int8_mid<true, 8>)
-                      : (splits == 1 ? okc_int8_mid<false, 1> : splits == 2 ? okc_int8_mid<false, 2> : splits == 4 ? okc_int8_mid<false, 4> : okc_int8_mid<false, 8>);
+  const bool one = q.blocks == 1;
+  auto kernel = gated ? (one ? mid_kernel<true, true>(splits) : mid_kernel<true, false>(splits))
+                      : (one ? mid_kernel<false, true>(splits) : mid_kernel<false, false>(splits));
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};

@@ -182,6 +182,8 @@ bool int8_use_many(int T, int K, int N, bool gated);
 cudaError_t int8_read_status(cudaStream_t stream, int32_t* code);
 // Tensor map of int8 rows (abi.cu): box = 128 bytes x box_rows, 128-byte swizzle, zero fill outside.
 bool encode_bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t row_stride, uint32_t box_rows);
+bool encode_blocks_map(CUtensorMap* map, const void* base, uint64_t rows, uint32_t halves, uint64_t K, uint64_t row_stride,
+                       uint32_t box_rows, uint32_t blocks);
 // Tensor map of bf16 result rows (row stride in elements): box = 32 columns x 32 rows, 64-byte swizzle.
 bool encode_bf16_out_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t row_stride);
 
