@@ -15,6 +15,8 @@
 // Every wait on a barrier is bounded; one that runs out is reported through a status word (okc_moe_dense_status).
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "rows.cuh"
 
 namespace okc {
@@ -270,7 +272,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "memory");
 }
 // ------------------------------------------------------------------ some hundred tokens
-constexpr int kMidThreads = 256;       // warps 0..3 read the accumulator, 4 TMA producer, 5 MMA issuer; all finish the rows
+constexpr int kMidThreads = 256;       // warps 0..3 read the accumulator, 4 and 6 bring weights and tokens, 5 issues the MMAs; all finish the rows
 constexpr int kMidMaxStages = 16;
 constexpr int kMidRing = 216 * 1024;
 constexpr int kMidMinSmem = 116 * 1024;      // one CTA an SM: clusters cannot wait for each other's tensor memory
@@ -365,13 +367,13 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   // a thread finishes four neighbouring outputs of every few tokens
   constexpr int kQuads = kGated ? kTileW / 8 : kTileW / 4;
   const int o4 = (tid % kQuads) * 4, n = w0 + o4;
-  float sw[4], su[4] = {}, sb[4] = {};
+  float sw[4], su[4] = {}, sb[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const bool in = n + j < p.N;
     sw[j] = in ? __ldg(p.w_scale + n + j) : 0.f;
     if (kGated) su[j] = in ? __ldg(p.w_scale + p.N + n + j) : 0.f;
-    else if (p.bias) sb[j] = in ? __ldg(p.bias + n + j) : 0.f;
+    sb[j] = !kGated && p.bias && in ? __ldg(p.bias + n + j) : -0.f;      // v + -0 is v, whatever v
   }
 
   if (warp == 4 || warp == 6) {
@@ -448,44 +450,61 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   if (kSplits > 1) cluster.sync(); else __syncthreads();
 
   // Each CTA of the cluster finishes tn / kSplits tokens: it adds the integer sums of all CTAs (the loads from all of them
-  // under way at once) and stores the rows.
+  // under way at once) and stores the rows.  A few tokens of a thread go together, all loads and arithmetic first, and what
+  // differs between calls is decided once for them: with eight warps an SM, one token at a time was a chain of latencies
+  // (256 tokens, K = 256, N = 2048, no split: 8.8 us; so 6.3).  What is left, and rows off the 8-byte grid, go one by one.
   {
     const int* src[kSplits];
 #pragma unroll
     for (int s = 0; s < kSplits; ++s) src[s] = (kSplits > 1 ? cluster.map_shared_rank(part, s) : part) + o4;
     const int per = q.tn / kSplits, last = o4 < q.outs ? min((rank + 1) * per, p.T - t0) : 0;
-#pragma unroll 2
-    for (int col = rank * per + tid / kQuads; col < last; col += kMidThreads / kQuads) {
-      int4 a[kSplits], b[kSplits];
+    const bool vec = p.out_vec && n + 4 <= p.N;
+    constexpr int kStep = kMidThreads / kQuads, kBatch = kSplits >= 4 ? 2 : 4;
+    auto finish = [&](auto tokens, int col0) {
+      constexpr int kTokens = decltype(tokens)::value;
+      float v[kTokens][4];
 #pragma unroll
-      for (int s = 0; s < kSplits; ++s) {
-        a[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW);
-        if (kGated) b[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW + q.outs);
-      }
+      for (int u = 0; u < kTokens; ++u) {
+        const int col = col0 + u * kStep;
+        int4 a[kSplits], b[kSplits];
 #pragma unroll
-      for (int s = 1; s < kSplits; ++s) {
-        a[0].x += a[s].x; a[0].y += a[s].y; a[0].z += a[s].z; a[0].w += a[s].w;
-        if (kGated) { b[0].x += b[s].x; b[0].y += b[s].y; b[0].z += b[s].z; b[0].w += b[s].w; }
-      }
-      const float sx = xs[col];
-      const int av[4] = {a[0].x, a[0].y, a[0].z, a[0].w}, bv[4] = {b[0].x, b[0].y, b[0].z, b[0].w};
-      float v[4];
+        for (int s = 0; s < kSplits; ++s) {
+          a[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW);
+          if (kGated) b[s] = *reinterpret_cast<const int4*>(src[s] + col * kTileW + q.outs);
+        }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = int8_value(av[j], sx, sw[j]);
-        if (kGated) v[j] = silu_mul(v[j], int8_value(bv[j], sx, su[j]));
-        else if (p.bias) v[j] = __fadd_rn(v[j], sb[j]);
+        for (int s = 1; s < kSplits; ++s) {
+          a[0].x += a[s].x; a[0].y += a[s].y; a[0].z += a[s].z; a[0].w += a[s].w;
+          if (kGated) { b[0].x += b[s].x; b[0].y += b[s].y; b[0].z += b[s].z; b[0].w += b[s].w; }
+        }
+        const float sx = xs[col];
+        const int av[4] = {a[0].x, a[0].y, a[0].z, a[0].w}, bv[4] = {b[0].x, b[0].y, b[0].z, b[0].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[u][j] = int8_value(av[j], sx, sw[j]);
+          if (kGated) v[u][j] = silu_mul(v[u][j], int8_value(bv[j], sx, su[j]));
+          else v[u][j] = __fadd_rn(v[u][j], sb[j]);
+        }
       }
-      const int64_t o = static_cast<int64_t>(t0 + col) * p.out_stride + n;
-      if (p.out_vec && n + 4 <= p.N) {
-        if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = make_float4(v[0], v[1], v[2], v[3]);
-        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-      } else {
+      const int64_t o = static_cast<int64_t>(t0 + col0) * p.out_stride + n, step = static_cast<int64_t>(kStep) * p.out_stride;
+      if (vec && p.out_f32) {
+#pragma unroll
+        for (int u = 0; u < kTokens; ++u)
+          *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o + u * step) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+      } else if (vec) {
+#pragma unroll
+        for (int u = 0; u < kTokens; ++u)
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o + u * step) = make_uint2(pack_bf16x2(v[u][0], v[u][1]), pack_bf16x2(v[u][2], v[u][3]));
+      } else if (kTokens == 1) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (n + j < p.N) store_out(p, o + j, v[j]);
+          if (n + j < p.N) store_out(p, o + j, v[0][j]);
       }
-    }
+    };
+    int col = rank * per + tid / kQuads;
+    if (vec)
+      for (; col + (kBatch - 1) * kStep < last; col += kBatch * kStep) finish(std::integral_constant<int, kBatch>{}, col);
+    for (; col < last; col += kStep) finish(std::integral_constant<int, 1>{}, col);
   }
   if (kSplits > 1) cluster.sync(); else __syncthreads();   // no CTA leaves while another reads its sums
   if (warp == 5) {
@@ -498,20 +517,16 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
 static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
 
 // How the two tiled kernels would cut a product, and what each is expected to take.  The estimates are a start-up time, a
-// time for the end of a tile, and a time for each stage: what a CTA needs for it alone, or, with all SMs busy, what its
-// bytes take at the 90 KB/us that an SM takes in then.  Of 196 measured shapes (3 to 512 tokens, K 300 to 7168, N 300 to
-// 7168, plain and gated), where the two differ by up to 2 either way, the choice costs 0.14 % of the better one's time on
-// average and 13 % at worst.
+// time for the end of a tile, and a time for the K blocks: what a CTA needs for one alone, or, with all SMs busy, what its
+// bytes take at the 83 to 90 KB/us that an SM takes in then.  Of 323 measured shapes (3 to 512 tokens, K 256 to 7168, N 300
+// to 7168, plain and gated), where the two differ by up to 2 either way, the choice costs 0.4 % of the better one's time on
+// average and 30 % at worst, and the split over a cluster 0.4 % on average.
 struct TileShape {
   int tokens, outs, blocks;      // mid: tokens and outputs of a tile, K blocks of a stage
   int t_tiles, tiles, splits;
   int bn;            // many: weight rows of a tile
   double us;
 };
-static double stage_us(double alone, double kbytes, double ctas) {
-  const double busy = kbytes / 90.0 * (ctas < 148 ? ctas / 148.0 : 1.0);
-  return busy > alone ? busy : alone;
-}
 static TileShape mid_shape(int T, int K, int N, bool gated) {
   TileShape s = {};
   const int most = gated ? kTileW / 2 : kTileW, n_kb = (K + kKb - 1) / kKb;
@@ -525,13 +540,20 @@ static TileShape mid_shape(int T, int K, int N, bool gated) {
   const int64_t clusters = static_cast<int64_t>(s.tiles) * s.t_tiles;
   const int fit = clusters <= 14 ? 14 : clusters <= 32 ? 32 : clusters <= 74 ? 74 : 148;
   s.splits = fit == 14 ? 8 : fit == 32 ? 4 : fit == 74 ? 2 : 1;
-  while (s.splits > n_kb) s.splits /= 2;
+  // A cluster costs 1.2 us and adding up more with more tokens, so there have to be K blocks for it, for eight or four CTAs one
+  // or two each, for two, which gain least, more (32 tokens, K = 1024, N = 1024, 1 / 2 / 4 / 8: 4.9 / 5.2 / 4.7 / 5.0 us; 256
+  // tokens, K = 512, N = 2048, 1 / 2 / 4: 6.9 / 8.1 / 8.5).  A gated tile has half the outputs, and where outputs are stored
+  // one by one, sharing them out is worth it by itself (333 tokens, K = 1000, N = 1537: 11.8 / 10.7 / 8.8).
+  const bool odd = N % 4 != 0;
+  auto too_few = [&](int splits) { return n_kb < (splits == 2 ? 9 : splits == 4 ? 4 : 10) + (gated || odd ? 0.0 : splits * s.tokens / 128.0); };
+  while (s.splits > 1 && too_few(s.splits)) s.splits /= 2;
   // Tiles of fewer weight rows, down to half, where many SMs had none.  K = 7168, N = 512, 128 tokens: 8 tiles of 64 in place
   // of 4 of 128, 7.6 us in place of 8.7; gated, K = 4096, 2 x 2560 rows, 32 tokens: 64 of 40 in place of 40, 7.1 in place of 7.5.
   // Not for fewer SMs (K = 4096, N = 7168, 128 tokens, 69 in place of 56: 11.7 against 11.6) or more tokens, which each tile
   // copies (K = 4096, N = 5120, 200 tokens: 13.2 against 12.5).
-  if (clusters * 4 <= fit * 3 && s.tokens <= 128) {
-    const int tiles = fit / s.t_tiles;
+  const int room = s.splits == 8 ? 14 : s.splits == 4 ? 32 : s.splits == 2 ? 74 : 148;
+  if (clusters * 4 <= room * 3 && s.tokens <= 128) {
+    const int tiles = room / s.t_tiles;
     int outs = ((N + tiles - 1) / tiles + 7) & ~7;
     if (outs < most / 2) outs = most / 2;
     if (outs < s.outs) { s.outs = outs; s.tiles = (N + outs - 1) / outs; }
@@ -549,7 +571,9 @@ static TileShape mid_shape(int T, int K, int N, bool gated) {
   const double ctas = static_cast<double>(s.tiles) * s.t_tiles * s.splits;
   const double rounds = static_cast<double>((static_cast<int64_t>(s.tiles) * s.t_tiles * s.splits + 147) / 148);
   const double kbytes = (gated ? 2 : 1) * s.outs / 8.0 + s.tokens / 8.0;
-  s.us = 3.0 + rounds * (0.021 * s.tokens + (n_kb + s.splits - 1) / s.splits * stage_us(0.21, kbytes, ctas));
+  const double alone = kbytes / 126.0, busy = kbytes / 83.0 * (ctas < 148 ? ctas / 148.0 : 1.0);
+  const double token = 0.010 + ((gated ? 0.006 : 0.0) + (odd ? 0.026 : 0.0)) / s.splits;
+  s.us = (s.splits > 1 ? 4.95 : 3.75) + rounds * (token * s.tokens + per * (alone > busy ? alone : busy));
   return s;
 }
 static TileShape many_shape(int T, int K, int N, bool gated) {
@@ -567,7 +591,8 @@ static TileShape many_shape(int T, int K, int N, bool gated) {
   }
   const double ctas = 2.0 * s.tiles * s.t_tiles;
   const double alone = s.bn <= 96 ? 0.19 : 0.00088 * (s.bn + 120);
-  s.us = 3.0 + rounds * (0.02 * s.bn + n_kb * stage_us(alone, 16 + s.bn / 16.0, ctas));
+  const double busy = (16 + s.bn / 16.0) / 90.0 * (ctas < 148 ? ctas / 148.0 : 1.0);
+  s.us = 4.3 + rounds * (0.018 * s.bn + n_kb * (alone > busy ? alone : busy));
   return s;
 }
 
