@@ -275,7 +275,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 constexpr int kMidThreads = 256;       // warps 0..3 read the accumulator, 4 and 6 bring weights and tokens, 5 issues the MMAs; all finish the rows
 constexpr int kMidMaxStages = 16;
 constexpr int kMidRing = 216 * 1024;
-constexpr int kMidMinSmem = 116 * 1024;      // one CTA an SM: clusters cannot wait for each other's tensor memory
+constexpr int kMidMinSmem = 200 * 1024;      // one CTA an SM, and little beside it: clusters cannot wait in a circle for tensor memory
 constexpr int kMidMaxBlocks = 8;       // most K blocks of a stage
 constexpr int kKb = 128;               // K elements of a stage: one 128-byte swizzled row
 constexpr int kTileW = 128;            // weight rows of a tile
