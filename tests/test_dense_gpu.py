@@ -159,6 +159,26 @@ def test_int8_gated(T, K, N):
     assert okc.dense_status() == (0, 0)
 
 
+@pytest.mark.parametrize("T,K,N", [(7, 7168, 2048), (40, 7168, 2040), (31, 4096, 2560), (100, 2304, 2568), (33, 16512, 130), (9, 2944, 4100),
+                                   (16, 1408, 520), (200, 512, 1536), (250, 384, 600), (130, 1152, 9601), (2, 131068 // 128 * 128, 24)])
+def test_products_of_several_k_blocks_a_copy(T, K, N):
+    """K of whole blocks of 128, in stages of different lengths; weight and token rows with other values behind their columns."""
+    g = _gen(T + K + N + 2)
+    wide = torch.randint(-127, 128, (2 * N, K + 144), generator=g, device="cuda", dtype=torch.int8)
+    x = okc.QuantRows(torch.randint(-127, 128, (T, K + 16), generator=g, device="cuda", dtype=torch.int8)[:, :K],
+                      torch.rand(T, generator=g, device="cuda") * 1e-2 + 1e-4)
+    scale = torch.rand(2 * N, generator=g, device="cuda") * (0.2 / math.sqrt(K))
+    w, both = okc.QuantRows(wide[:N, :K], scale[:N]), okc.QuantRows(wide[:, :K], scale)
+    for out_f32 in (False, True):
+        y, h = okc.int8_linear(x, w, out_f32=out_f32), okc.int8_gated(x, both, out_f32=out_f32)
+        _close(y, *_linear_ref(x.q, x.scale, w, None, y.dtype), f"linear f32 {out_f32}")
+        _close(h, *_gated_ref(x.q, x.scale, both, h.dtype), f"gated f32 {out_f32}")
+    store = torch.full((T + 1, N + 5), 7.0, device="cuda")
+    okc.int8_linear(x, w, out_f32=True, out=store[:T, 3:3 + N])
+    assert torch.equal(store[:T, 3:3 + N], y) and (store[T] == 7).all() and (store[:, :3] == 7).all() and (store[:, 3 + N:] == 7).all()
+    assert okc.dense_status() == (0, 0)
+
+
 def test_gated_far_tails():
     """Gate values of thousands: silu is g or 0, never NaN."""
     for T in (2, 20, 300):
