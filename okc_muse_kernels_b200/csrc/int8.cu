@@ -75,10 +75,10 @@ struct OneShape {
 // a warp takes a slot: pairs of rows (two neighbours, or a gate row and its up row) against the token, 16 bytes a lane of
 // each, integer dot products, one warp sum a row, and the outputs leave from there.
 // The 16 bytes at a row's end may reach past K, never past the row's next 16-byte boundary; the token is zero there.
-// bf16 token, weights of three layers in turn: K = 4096, N = 4096 4.3 us (the quantiser and okc_int8_mid: 7.4; rows held in
-// registers, 16 a warp on their way: 5.7), gated, K = 7168, 2 x 2048 rows 6.6 (8.7; 8.2);
-// a token and one weight tile alone take 3.3.  More tokens go through the tiles: the dot-product instruction gives an SM
-// some 14 lanes a clock, and 2 / 4 / 8 tokens took 5.3 / 7.3 / 11.6 us here (gated 9.7 / 13.2 / 22.8) against 7.4 (8.8).
+// bf16 token, weights of three layers in turn: K = 4096, N = 4096 4.4 us (the quantiser and okc_int8_mid: 6.5; rows held in
+// registers, 16 a warp on their way: 5.7), gated, K = 7168, 2 x 2048 rows 5.5 (8.3; 8.2); a token and one weight tile alone
+// take 3.3.  More tokens go through the tiles: the dot-product instruction gives an SM some 14 lanes a clock, and 2 / 4 / 8
+// tokens took 5.3 / 7.3 / 11.6 us here (gated 9.7 / 13.2 / 22.8) against 6.5 (8.3).
 template <bool kGated>
 __global__ void __launch_bounds__(kOneThreads) okc_int8_one(const Int8Params p, const OneShape q) {
   extern __shared__ __align__(16) uint8_t one_smem[];
