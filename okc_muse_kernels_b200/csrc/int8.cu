@@ -918,10 +918,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
         // A thread has 32 neighbouring results of its own row.  As bf16 they leave through shared memory and a TMA store a
         // warp, whole sectors at a time (stored by the threads themselves, 16 bytes each, 4096x1024x4096 takes 28.6 us for
         // 25.3); as f32 the thread has whole sectors.
+        // A store that ends a row off a 16-byte boundary fills up to that with zeros, over what a caller has behind the row:
+        // such last columns go the third way.
         const int col = tw * width + c0;
         if (q.tma_out) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
+        }
+        if (q.tma_out && (col + 32 <= p.N || p.N % 8 == 0)) {
           stage_bf16_row(at, lane, r);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();

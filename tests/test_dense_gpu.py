@@ -254,6 +254,21 @@ def test_strides_padding_and_rows_behind_the_last(T):
     _close(okc.int8_linear(x, w2), *_linear_ref(q, scale, w2, None, torch.bfloat16), "strided scales")
 
 
+@pytest.mark.parametrize("T", [1, 3, 40, 106, 300, 600])
+@pytest.mark.parametrize("N", [1, 8, 33, 36, 37, 40, 71, 266])
+def test_columns_behind_the_last_are_left_alone(T, N):
+    """Rows on 16-byte boundaries with a caller's columns behind them, of every remainder."""
+    g = _gen(T + N)
+    for K in (128, 1000):
+        x, w, both = okc.quantize_rows(_randn((T, K), g)), _weight(N, K, g), _weight(2 * N, K, g)
+        for dtype in (torch.bfloat16, torch.float32):
+            for fn, weight in ((okc.int8_linear, w), (okc.int8_gated, both)):
+                store = torch.full((T + 1, (N + 7) // 8 * 8 + 32), 7.0, device="cuda", dtype=dtype)
+                y = fn(x, weight, out_f32=dtype is torch.float32, out=store[:T, :N])
+                assert torch.equal(y, fn(x, weight, out_f32=dtype is torch.float32))
+                assert (store[:, N:] == 7).all() and (store[T] == 7).all(), (K, dtype, fn.__name__)
+
+
 @pytest.mark.parametrize("T", [6, 40, 300])
 def test_outputs_and_inputs_beyond_32_bit_offsets(T):
     """Row strides that put the last rows more than 2^32 bytes into a buffer."""
