@@ -225,7 +225,7 @@ cudaError_t launch_int8_one(const Int8Params& p, bool gated, cudaStream_t stream
   const size_t smem = static_cast<size_t>(kpad) + static_cast<size_t>(q.slots) * slot_bytes + scales;
   const dim3 grid((p.N + q.outs - 1) / q.outs), block(kOneThreads);
   auto kernel = gated ? okc_int8_one<true> : okc_int8_one<false>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOneSmem);     // (never less: see params.cuh)
   if (e != cudaSuccess) return e;
   return launch_kernel(kernel, grid, block, smem, stream, false, p, q);
 }
@@ -275,6 +275,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 constexpr int kMidThreads = 256;       // warps 0..3 read the accumulator, 4 and 6 bring weights and tokens, 5 issues the MMAs; all finish the rows
 constexpr int kMidMaxStages = 16;
 constexpr int kMidRing = 216 * 1024;
+constexpr int kMidMaxSmem = 225 * 1024;      // an SM's 227 KB less what the kernel declares itself (1.3 KB)
 constexpr int kMidMinSmem = 200 * 1024;      // one CTA an SM, and little beside it: clusters cannot wait in a circle for tensor memory
 constexpr int kMidMaxBlocks = 8;       // most K blocks of a stage
 constexpr int kKb = 128;               // K elements of a stage: one 128-byte swizzled row
@@ -630,7 +631,8 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here
   const bool one = q.blocks == 1;
   auto kernel = gated ? (one ? mid_kernel<true, true>(splits) : mid_kernel<true, false>(splits))
                       : (one ? mid_kernel<false, true>(splits) : mid_kernel<false, false>(splits));
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (smem > kMidMaxSmem) return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMidMaxSmem);     // (never less: see params.cuh)
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * splits, ttiles);

@@ -574,7 +574,7 @@ static bool try_stream(const BlockNormParams& p, int64_t rows, bool vec, cudaStr
   auto kernel = !vec ? (chunks == 1 ? okc_block_norm_stream_any<1> : chunks == 2 ? okc_block_norm_stream_any<2> : okc_block_norm_stream_any<4>)
               : q ? (chunks == 1 ? okc_block_norm_stream<1, true> : chunks == 2 ? okc_block_norm_stream<2, true> : okc_block_norm_stream<4, true>)
                   : (chunks == 1 ? okc_block_norm_stream<1, false> : chunks == 2 ? okc_block_norm_stream<2, false> : okc_block_norm_stream<4, false>);
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kStreamSmem);     // (never less: see params.cuh)
   if (e == cudaSuccess) e = launch_kernel(kernel, grid, block, smem, stream, false, p, static_cast<int>(rows), row_bytes);
   return true;
 }

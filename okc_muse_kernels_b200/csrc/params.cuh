@@ -187,6 +187,10 @@ bool encode_blocks_map(CUtensorMap* map, const void* base, uint64_t rows, uint32
 // Tensor map of bf16 result rows (row stride in elements): box = 32 columns x 32 rows, 64-byte swizzle.
 bool encode_bf16_out_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t row_stride);
 
+// The largest dynamic shared memory a kernel may be launched with is state of the kernel on its device, not of a call: a
+// launch sets it to one constant of the kernel, the most that any call asks for.  Set to each call's own size, a call of
+// another thread lowers it between this call's setting and its launch, which then fails.
+//
 // Launch with (pdl = true) or without the programmatic-serialization attribute.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
