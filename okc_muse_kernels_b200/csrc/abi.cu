@@ -28,31 +28,38 @@ static EncodeFn encode_fn() {
   return f;
 }
 
+// The driver's encoder wants a current context, and a host thread has none before its first launch (the runtime gives it one
+// then, or when it sets its device): a call that fails is made again behind that.
+template <typename... Args>
+static bool encode_tiled(Args... args) {
+  EncodeFn f = encode_fn();
+  if (!f) return false;
+  if (f(args...) == CUDA_SUCCESS) return true;
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && f(args...) == CUDA_SUCCESS;
+}
+
 // bf16 [rows, K] row-major (rows row_stride elements apart; 0: K), box = 64 elements x box_rows, 128-byte swizzle,
 // zero fill outside.
 static bool encode_rows_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t K, uint32_t box_rows,
                             uint64_t row_stride = 0) {
-  EncodeFn f = encode_fn();
-  if (!f) return false;
   const cuuint64_t dims[2] = {K, rows};
   const cuuint64_t strides[1] = {(row_stride ? row_stride : K) * 2};
   const cuuint32_t box[2] = {64, box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return f(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 bool encode_bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t row_stride, uint32_t box_rows) {
-  EncodeFn f = encode_fn();
-  if (!f) return false;
   const cuuint64_t dims[2] = {K, rows};
   const cuuint64_t strides[1] = {row_stride};
   const cuuint32_t box[2] = {128, box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 // The same rows as [K / 128 blocks][halves][rows][128], box = blocks x halves x box_rows x 128, for copies of several
@@ -60,27 +67,24 @@ bool encode_bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_
 bool encode_blocks_map(CUtensorMap* map, const void* base, uint64_t rows, uint32_t halves, uint64_t K, uint64_t row_stride,
                        uint32_t box_rows, uint32_t blocks) {
   if (blocks == 1) return encode_bytes_map(map, base, rows * halves, K, row_stride, box_rows);
-  EncodeFn f = encode_fn();
-  if (!f || K % 128) return false;
+  if (K % 128) return false;
   const int rank = halves == 1 ? 3 : 4;
   cuuint64_t dims[4] = {128, rows, halves, K / 128}, strides[3] = {row_stride, rows * row_stride, 128};
   cuuint32_t box[4] = {128, box_rows, halves, blocks};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   if (rank == 3) { dims[2] = dims[3]; strides[1] = strides[2]; box[2] = box[3]; }
-  return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 bool encode_bf16_out_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t row_stride) {
-  EncodeFn f = encode_fn();
-  if (!f) return false;
   const cuuint64_t dims[2] = {cols, rows};
   const cuuint64_t strides[1] = {row_stride * 2};
   const cuuint32_t box[2] = {32, 32};
   const cuuint32_t estr[2] = {1, 1};
-  return f(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-           CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
 static int sm_count() {
