@@ -353,16 +353,16 @@ cudaError_t launch_ep_push_route_sort(const EpParams& p, const RouteParams& rp, 
   const dim3 grid(gx, p.world), block(kRouteThreads);
   cudaError_t e;
   if (p.E <= 128) {
-    e = cudaFuncSetAttribute(okc_ep_push_route_sort<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    e = cudaFuncSetAttribute(okc_ep_push_route_sort<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
     if (e != cudaSuccess) return e;
     return launch_kernel(okc_ep_push_route_sort<4>, grid, block, smem, stream, true, p, rp);
   }
   if (p.E <= 256) {
-    e = cudaFuncSetAttribute(okc_ep_push_route_sort<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    e = cudaFuncSetAttribute(okc_ep_push_route_sort<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
     if (e != cudaSuccess) return e;
     return launch_kernel(okc_ep_push_route_sort<8>, grid, block, smem, stream, true, p, rp);
   }
-  e = cudaFuncSetAttribute(okc_ep_push_route_sort<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  e = cudaFuncSetAttribute(okc_ep_push_route_sort<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
   if (e != cudaSuccess) return e;
   return launch_kernel(okc_ep_push_route_sort<16>, grid, block, smem, stream, true, p, rp);
 }

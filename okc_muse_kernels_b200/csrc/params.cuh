@@ -190,7 +190,8 @@ bool encode_bf16_out_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t c
 // The largest dynamic shared memory a kernel may be launched with is state of the kernel on its device, not of a call: a
 // launch sets it to one constant of the kernel, the most that any call asks for.  Set to each call's own size, a call of
 // another thread lowers it between this call's setting and its launch, which then fails.
-//
+constexpr int kMostDynamicSmem = 226 * 1024;      // for kernels that declare less than a kilobyte themselves
+
 // Launch with (pdl = true) or without the programmatic-serialization attribute.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,

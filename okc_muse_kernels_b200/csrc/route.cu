@@ -308,7 +308,7 @@ cudaError_t launch_wait_timeout_probe(int32_t* status, cudaStream_t stream) {
 
 cudaError_t launch_route(const RouteParams& p, cudaStream_t stream) {
   const size_t smem = route_smem_bytes(p.T * p.kk, p.slots, kRouteThreads);
-  cudaError_t e = cudaFuncSetAttribute(okc_route_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  cudaError_t e = cudaFuncSetAttribute(okc_route_sort, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
   if (e != cudaSuccess) return e;
   if (p.logits != nullptr || p.router_w != nullptr || p.router_w_split != nullptr) {
     // the router proper: ids / weights of every token, then the sort below reads them back
@@ -340,14 +340,14 @@ cudaError_t launch_route(const RouteParams& p, cudaStream_t stream) {
       // a small step with its logits given: top-k and sort in one CTA
       const dim3 one(1);
       if (p.E <= 128) {
-        e = cudaFuncSetAttribute(okc_route_topk_sort<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        e = cudaFuncSetAttribute(okc_route_topk_sort<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
         return e != cudaSuccess ? e : launch_kernel(okc_route_topk_sort<4>, one, threads, smem, stream, false, q, lg, n_part);
       }
       if (p.E <= 256) {
-        e = cudaFuncSetAttribute(okc_route_topk_sort<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        e = cudaFuncSetAttribute(okc_route_topk_sort<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
         return e != cudaSuccess ? e : launch_kernel(okc_route_topk_sort<8>, one, threads, smem, stream, false, q, lg, n_part);
       }
-      e = cudaFuncSetAttribute(okc_route_topk_sort<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      e = cudaFuncSetAttribute(okc_route_topk_sort<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
       return e != cudaSuccess ? e : launch_kernel(okc_route_topk_sort<16>, one, threads, smem, stream, false, q, lg, n_part);
     }
     // the tokens over many SMs, the last CTA sorts.  Split-K partial sums: a CTA per token, the partial rows staged
@@ -358,14 +358,14 @@ cudaError_t launch_route(const RouteParams& p, cudaStream_t stream) {
     const size_t smem_g = stage_parts && stage_bytes > smem ? stage_bytes : smem;
     const dim3 grid((p.T + per_cta - 1) / per_cta);
     if (p.E <= 128) {
-      e = cudaFuncSetAttribute(okc_route_topk_sort_grid<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_g));
+      e = cudaFuncSetAttribute(okc_route_topk_sort_grid<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
       return e != cudaSuccess ? e : launch_kernel(okc_route_topk_sort_grid<4>, grid, threads, smem_g, stream, n_part > 0, q, lg, n_part, per_cta, stage_parts);
     }
     if (p.E <= 256) {
-      e = cudaFuncSetAttribute(okc_route_topk_sort_grid<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_g));
+      e = cudaFuncSetAttribute(okc_route_topk_sort_grid<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
       return e != cudaSuccess ? e : launch_kernel(okc_route_topk_sort_grid<8>, grid, threads, smem_g, stream, n_part > 0, q, lg, n_part, per_cta, stage_parts);
     }
-    e = cudaFuncSetAttribute(okc_route_topk_sort_grid<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_g));
+    e = cudaFuncSetAttribute(okc_route_topk_sort_grid<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
     return e != cudaSuccess ? e : launch_kernel(okc_route_topk_sort_grid<16>, grid, threads, smem_g, stream, n_part > 0, q, lg, n_part, per_cta, stage_parts);
   }
   return launch_kernel(okc_route_sort, dim3(1), dim3(kRouteThreads), smem, stream, true, p);

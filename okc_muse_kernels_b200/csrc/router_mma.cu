@@ -169,7 +169,7 @@ cudaError_t launch_router_mma(const CUtensorMap& wmap, const CUtensorMap& hmap, 
   p.tmem_cols = p.tpad <= 32 ? 32 : p.tpad <= 64 ? 64 : p.tpad <= 128 ? 128 : 256;
   const int splits = (p.n_kb + kb_per_cta - 1) / kb_per_cta;
   const size_t smem = router_mma_smem_bytes(kb_per_cta, p.tpad);
-  cudaError_t e = cudaFuncSetAttribute(okc_router_mma, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  cudaError_t e = cudaFuncSetAttribute(okc_router_mma, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostDynamicSmem);
   if (e != cudaSuccess) return e;
   okc_router_mma<<<dim3((E + kRmTileE - 1) / kRmTileE, splits), 128, smem, stream>>>(p);
   return cudaGetLastError();
