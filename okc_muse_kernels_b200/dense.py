@@ -49,13 +49,15 @@ def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     return dev
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream     # the current stream of a device as an integer
-_current_device = torch._C._cuda_getDevice           # (a CUDA tensor is at hand: CUDA is initialised)
 _empty = torch.empty_strided                         # the cheapest of torch's ways to uninitialised memory
+# A torch without CUDA lacks the names below.  The package imports all the same (the layouts and synthetic weights need no
+# GPU), and no call gets to them: each refuses tensors that are not on a CUDA device first.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # the current stream of a device as an integer
+_current_device = getattr(torch._C, "_cuda_getDevice", None)           # (a CUDA tensor is at hand: CUDA is initialised)
 # Memory of torch's caching allocator without a tensor around it (0.5 us, an empty tensor 1.5): on the current device, for
 # work on the given stream; after the free it goes to later work on that stream, as a tensor's would.
-_alloc = torch._C._cuda_cudaCachingAllocator_raw_alloc
-_free = torch._C._cuda_cudaCachingAllocator_raw_delete
+_alloc = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None)
+_free = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None)
 
 
 def _call(fn, name: str, dev: int, args) -> None:
