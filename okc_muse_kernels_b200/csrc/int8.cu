@@ -377,6 +377,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     sb[j] = !kGated && p.bias && in ? __ldg(p.bias + n + j) : -0.f;      // v + -0 is v, whatever v
   }
 
+  int posted = 0;        // stages whose copies this warp has started
   if (warp == 4 || warp == 6) {
     const bool tokens = warp == 6;
     int i = first;
@@ -390,12 +391,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
       if (tokens) load_x(i, st); else load_w(i, st);
       if (++st == static_cast<uint32_t>(q.stages)) { st = 0; ph ^= 1; }
     }
-    if (i < nst) {
-      // giving up: the copies in flight get a bounded chance to land before the CTA retires
-      const long long c0 = clock64();
-      for (int j = max(0, i - q.stages); j < i; ++j)
-        while (!mbar_try(full0 + 8 * (j % q.stages), (j / q.stages) & 1) && clock64() - c0 < kWaitLimitCycles) {}
-    }
+    posted = i;
     __syncwarp();
   } else if (warp == 5) {
     const uint32_t idesc = idesc_i8(128, static_cast<uint32_t>(q.tn));
@@ -506,6 +502,13 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     if (vec)
       for (; col + (kBatch - 1) * kStep < last; col += kBatch * kStep) finish(std::integral_constant<int, kBatch>{}, col);
     for (; col < last; col += kStep) finish(std::integral_constant<int, 1>{}, col);
+  }
+  // A wait ran out, whoever's it was (the producers of a short K have started all their copies by then and are done): the
+  // copies on their way get a bounded chance to land before the CTA's memory is another's.
+  if (abort_code != 0) {
+    const long long c0 = clock64();
+    for (int j = max(0, posted - q.stages); j < posted; ++j)
+      while (!mbar_try(full0 + 8 * (j % q.stages), (j / q.stages) & 1) && clock64() - c0 < kWaitLimitCycles) {}
   }
   if (kSplits > 1) cluster.sync(); else __syncthreads();   // no CTA leaves while another reads its sums
   if (warp == 5) {

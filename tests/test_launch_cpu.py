@@ -15,3 +15,14 @@ def test_shared_memory_limits_are_constants_of_the_kernels():
                 assert re.fullmatch(r"k[A-Z]\w*", limit), f"{name}: {limit}"
                 found += 1
     assert found >= 10
+
+
+def test_the_split_product_drains_its_copies_whichever_wait_ran_out():
+    """A wait that runs out leaves copies on their way into shared memory.  In okc_int8_mid it may be the issuer's, when both
+    producers have started everything and left their loops: the drain stands behind all of them, in front of the last barrier,
+    and asks for the flag that every wait sets."""
+    with open(os.path.join(CSRC, "int8.cu")) as f:
+        body = f.read().split("okc_int8_mid(const")[1].split("static int tmem_cols_for")[0]
+    tail = body[body.rindex("finish(std::integral_constant<int, 1>"):body.rindex("cluster.sync()")]
+    assert re.search(r"if \(abort_code != 0\) \{[^}]*mbar_try\(full0[^}]*kWaitLimitCycles", tail)
+    assert body.count("mbar_wait") == 3 and "mbar_wait" not in tail
