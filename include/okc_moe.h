@@ -345,8 +345,12 @@ uint64_t okc_moe_int8_scratch_bytes(int x_kind, int32_t tokens, int32_t k);
 int okc_moe_int8_linear(const okc_int8_args* args, okc_stream_t stream);
 int okc_moe_int8_gated(const okc_int8_args* args, okc_stream_t stream);
 /* Synchronises `stream`; 0, or OKC_ERR_TIMEOUT with *detail naming a device wait of these operators that ran out on the
- * current device since the last call of this function (the call it happened in has undefined results). */
+ * current device and that this function has not reported yet (the call it happened in has undefined results).  Of the waits of
+ * the norms, and of those of the products, the first since the last report is kept; each call reports one. */
 int okc_moe_dense_status(okc_stream_t stream, int32_t* detail);
+/* Failure-detection self test, as okc_moe_probe_wait_timeout: one warp waits, with a short limit, on a barrier that nothing
+ * completes, and records the code of its wait where the norms (product = 0: code 0x7d) or the products (1: 0x7c) do. */
+int okc_moe_probe_dense_timeout(int product, okc_stream_t stream);
 
 /* Copies the sorted-route tables out of `workspace` for inspection (host or device pointers are
  * NOT interchangeable: all four are device pointers; any may be NULL).  counts: int32

@@ -107,6 +107,7 @@ SIGNATURES = {
     "okc_moe_int8_linear": (C.c_int, [_P, _P]),
     "okc_moe_int8_gated": (C.c_int, [_P, _P]),
     "okc_moe_dense_status": (C.c_int, [_P, C.POINTER(C.c_int32)]),
+    "okc_moe_probe_dense_timeout": (C.c_int, [C.c_int, _P]),
     "okc_ep_buffer_bytes": (C.c_uint64, [C.c_int32, C.c_int32, C.c_int32]),
     "okc_ep_views": (C.c_int, [_COMM, C.POINTER(_P), C.POINTER(_P), C.POINTER(_P)]),
     "okc_ep_gather_tokens": (C.c_int, [_COMM, _P, C.c_int64, _P, _P]),

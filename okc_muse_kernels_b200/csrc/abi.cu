@@ -203,7 +203,7 @@ using namespace okc;
 
 extern "C" {
 
-int okc_moe_version(void) { return 102; }
+int okc_moe_version(void) { return 103; }
 
 const char* okc_moe_strerror(int code) {
   switch (code) {
@@ -771,14 +771,20 @@ static int int8_product(const okc_int8_args* a, bool gated, okc_stream_t stream_
 int okc_moe_int8_linear(const okc_int8_args* args, okc_stream_t stream) { return int8_product(args, false, stream); }
 int okc_moe_int8_gated(const okc_int8_args* args, okc_stream_t stream) { return int8_product(args, true, stream); }
 
-int okc_moe_dense_status(okc_stream_t stream, int32_t* detail) {
-  int32_t norm = 0, product = 0;
-  if (norm_read_status(reinterpret_cast<cudaStream_t>(stream), &norm) != cudaSuccess ||
-      int8_read_status(reinterpret_cast<cudaStream_t>(stream), &product) != cudaSuccess)
-    return OKC_ERR_CUDA;
-  const int32_t code = product ? product : norm;
+int okc_moe_dense_status(okc_stream_t stream_, int32_t* detail) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  int32_t code = 0;
+  if (int8_read_status(stream, &code) != cudaSuccess) return OKC_ERR_CUDA;
+  if (code == 0 && norm_read_status(stream, &code) != cudaSuccess) return OKC_ERR_CUDA;      // (a norm's code waits for the next call)
   if (detail) *detail = code;
   return code ? OKC_ERR_TIMEOUT : OKC_OK;
+}
+
+int okc_moe_probe_dense_timeout(int product, okc_stream_t stream_) {
+  if (product != 0 && product != 1) return OKC_ERR_BAD_ARG;
+  if (!is_sm100()) return OKC_ERR_NO_DEVICE;
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  return (product ? launch_int8_probe_timeout(stream) : launch_norm_probe_timeout(stream)) == cudaSuccess ? OKC_OK : OKC_ERR_CUDA;
 }
 
 }  // extern "C"

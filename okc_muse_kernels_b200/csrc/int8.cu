@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kOneThreads) okc_int8_one(const Int8Params p, 
   }
   __syncthreads();
   if (tid == 0 && abort_code != 0) {
-    atomicCAS(&g_int8_status, 0, abort_code);
+    publish_timeout(&g_int8_status, abort_code);
     const long long c0 = clock64();      // copies that are late get some time before the CTA's memory is another's
     while (clock64() - c0 < kWaitLimitCycles / 100) {}
   }
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, static_cast<uint32_t>(q.tmem_cols));
   }
-  if (tid == 0 && abort_code != 0) atomicCAS(&g_int8_status, 0, abort_code);
+  if (tid == 0 && abort_code != 0) publish_timeout(&g_int8_status, abort_code);
 }
 
 static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
@@ -991,7 +991,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kManyThreads) okc_in
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
-  if (tid == 0 && abort_code != 0) atomicCAS(&g_int8_status, 0, abort_code);
+  if (tid == 0 && abort_code != 0) publish_timeout(&g_int8_status, abort_code);
 }
 
 bool int8_use_many(int T, int K, int N, bool gated) { return T > 512 || many_shape(T, K, N, gated).us < mid_shape(T, K, N, gated).us; }
@@ -1018,15 +1018,21 @@ cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool quantised_her
   return launch_kernel(kernel, dim3(grid), dim3(kManyThreads), kManySmem, stream, quantised_here, q);
 }
 
-__global__ void okc_int8_clear_status() { g_int8_status = 0; }
+__global__ void okc_int8_probe_timeout() { probe_timeout(&g_int8_status, 0x7c); }
+cudaError_t launch_int8_probe_timeout(cudaStream_t stream) {
+  okc_int8_probe_timeout<<<1, 32, 0, stream>>>();
+  return cudaGetLastError();
+}
 
+// Reads the word and, where it holds a code, clears that code: one that another stream's kernel records after the read stays.
+__global__ void okc_int8_clear_status(int32_t code) { atomicCAS(&g_int8_status, code, 0); }
 cudaError_t int8_read_status(cudaStream_t stream, int32_t* code) {
   cudaError_t e = cudaMemcpyFromSymbolAsync(code, g_int8_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, stream);
-  if (e != cudaSuccess) return e;
-  okc_int8_clear_status<<<1, 1, 0, stream>>>();
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (e != cudaSuccess || *code == 0) return e;
+  okc_int8_clear_status<<<1, 1, 0, stream>>>(*code);
   e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  return cudaStreamSynchronize(stream);
+  return e != cudaSuccess ? e : cudaStreamSynchronize(stream);
 }
 
 }  // namespace okc

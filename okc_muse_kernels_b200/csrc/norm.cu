@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
   }
   __syncthreads();
   if (tid == 0 && abort_code != 0) {
-    atomicCAS(&g_norm_status, 0, abort_code);
+    publish_timeout(&g_norm_status, abort_code);
     const long long c0 = clock64();      // copies that are late get some time before the CTA's memory is another's
     while (clock64() - c0 < kWaitLimitCycles / 100) {}
   }
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
   }
   __syncthreads();
   if (tid == 0 && abort_code != 0) {
-    atomicCAS(&g_norm_status, 0, abort_code);
+    publish_timeout(&g_norm_status, abort_code);
     const long long c0 = clock64();
     while (clock64() - c0 < kWaitLimitCycles / 100) {}
   }
@@ -608,15 +608,21 @@ cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool x_v
   return vec ? launch_kernel(okc_quantize_rows<4, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_quantize_rows<4, false>, grid, block, 0, stream, false, p);
 }
 
-__global__ void okc_norm_clear_status() { g_norm_status = 0; }
+__global__ void okc_norm_probe_timeout() { probe_timeout(&g_norm_status, 0x7d); }
+cudaError_t launch_norm_probe_timeout(cudaStream_t stream) {
+  okc_norm_probe_timeout<<<1, 32, 0, stream>>>();
+  return cudaGetLastError();
+}
 
+// Reads the word and, where it holds a code, clears that code: one that another stream's kernel records after the read stays.
+__global__ void okc_norm_clear_status(int32_t code) { atomicCAS(&g_norm_status, code, 0); }
 cudaError_t norm_read_status(cudaStream_t stream, int32_t* code) {
   cudaError_t e = cudaMemcpyFromSymbolAsync(code, g_norm_status, sizeof(int32_t), 0, cudaMemcpyDeviceToHost, stream);
-  if (e != cudaSuccess) return e;
-  okc_norm_clear_status<<<1, 1, 0, stream>>>();
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (e != cudaSuccess || *code == 0) return e;
+  okc_norm_clear_status<<<1, 1, 0, stream>>>(*code);
   e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  return cudaStreamSynchronize(stream);
+  return e != cudaSuccess ? e : cudaStreamSynchronize(stream);
 }
 
 }  // namespace okc

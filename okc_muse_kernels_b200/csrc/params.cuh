@@ -157,6 +157,7 @@ struct QuantizeParams {
 };
 cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool x_vec, bool q_vec, cudaStream_t stream);
 cudaError_t norm_read_status(cudaStream_t stream, int32_t* code);
+cudaError_t launch_norm_probe_timeout(cudaStream_t stream);
 
 // The int8 products (int8.cu).
 struct Int8Params {
@@ -180,6 +181,7 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here
 cudaError_t launch_int8_many(const Int8Params& p, bool gated, bool quantised_here, cudaStream_t stream);
 bool int8_use_many(int T, int K, int N, bool gated);
 cudaError_t int8_read_status(cudaStream_t stream, int32_t* code);
+cudaError_t launch_int8_probe_timeout(cudaStream_t stream);
 // Tensor map of int8 rows (abi.cu): box = 128 bytes x box_rows, 128-byte swizzle, zero fill outside.
 bool encode_bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint64_t row_stride, uint32_t box_rows);
 bool encode_blocks_map(CUtensorMap* map, const void* base, uint64_t rows, uint32_t halves, uint64_t K, uint64_t row_stride,

@@ -207,4 +207,21 @@ __device__ __forceinline__ uint32_t cta_max(uint32_t x, uint32_t* red) {
   return __reduce_max_sync(0xffffffffu, x);
 }
 
+// The code of a wait that ran out, into the module's status word: the first since the word was read stays.
+__device__ __forceinline__ void publish_timeout(int32_t* word, int code) { atomicCAS(word, 0, code); }
+// A wait, with a short limit, on a barrier that nothing completes (one warp): what the kernels do when theirs run out.
+__device__ __forceinline__ void probe_timeout(int32_t* word, int code) {
+  __shared__ uint64_t bar;
+  __shared__ int abort_code;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bar), 1);
+    abort_code = 0;
+    mbar_fence_init();
+  }
+  __syncthreads();
+  mbar_wait(smem_u32(&bar), 0, &abort_code, code, 1u << 14);
+  __syncthreads();
+  if (threadIdx.x == 0 && abort_code != 0) publish_timeout(word, abort_code);
+}
+
 }  // namespace okc

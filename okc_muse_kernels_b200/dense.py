@@ -242,8 +242,9 @@ def int8_ffn(x, w13, w2, *, bias: torch.Tensor | None = None, out_f32: bool = Fa
 
 
 def dense_status() -> tuple[int, int]:
-    """(status, detail) of this module's operators on the current device since the last call: (0, 0), or (OKC_ERR_TIMEOUT, code)
-    when a bounded device wait ran out.  Synchronises the current stream."""
+    """(status, detail) of this module's operators on the current device since the last report: (0, 0), or (OKC_ERR_TIMEOUT, code)
+    when a bounded device wait ran out (a product's first; a norm's is reported by the next call).  Synchronises the current
+    stream."""
     detail = C.c_int32(0)
     rc = _lib.lib().okc_moe_dense_status(torch.cuda.current_stream().cuda_stream, C.byref(detail))
     return rc, detail.value
