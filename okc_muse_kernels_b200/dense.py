@@ -94,13 +94,28 @@ def _vector(t: torch.Tensor | None, n: int, what: str) -> torch.Tensor | None:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory from a's first to its last element touches b's."""
+    """Whether the memory from a's first to its last element touches b's; of rows that are equally far apart, whether the
+    rows themselves do (columns side by side in one buffer do not)."""
     if a.data_ptr() > b.data_ptr():
         a, b = b, a
     gap = b.data_ptr() - a.data_ptr()
     if gap >= a.untyped_storage().nbytes() or not a.numel() or not b.numel():
         return False
-    return gap < (1 + sum((n - 1) * st for n, st in zip(a.shape, a.stride()))) * a.element_size()
+    if gap >= (1 + sum((n - 1) * st for n, st in zip(a.shape, a.stride()))) * a.element_size():
+        return False
+    (rows_a, apart_a, len_a), (rows_b, apart_b, len_b) = _row_bytes(a), _row_bytes(b)
+    apart = apart_a if rows_a > 1 else apart_b
+    if rows_a == rows_b == 1 or (rows_a > 1 and rows_b > 1 and apart_a != apart_b) or apart <= 0:
+        return True
+    return gap % apart < len_a or gap % apart + len_b > apart
+
+
+def _row_bytes(t: torch.Tensor) -> tuple[int, int, int]:
+    """Rows, how many bytes they are apart, and the bytes from a row's first to its last column."""
+    size = t.element_size()
+    if t.dim() != 2:
+        return 1, 0, (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * size
+    return t.shape[0], t.stride(0) * size, (1 + (t.shape[1] - 1) * t.stride(1)) * size
 
 
 def _check_out(out: torch.Tensor, R: int, cols: int, dtype: torch.dtype, what: str, inputs) -> int:
