@@ -23,6 +23,8 @@ __all__ = ["QuantRows", "quantize_rows", "int8_rows", "int8_linear", "int8_gated
 
 BLOCK_NORM_MAX_HIDDEN = 16384
 INT8_MAX_K = 131071           # the integer sums stay in 32 bits
+MAX_ROWS = (1 << 31) - 1      # rows of a call
+INT8_MAX_ROWS = 1 << 30       # tokens, and outputs, of a product
 INT8_ONE_MAX_K = 16384        # up to here the product of one token quantises it itself and needs no scratch
 _BF16, _F32, _I8 = torch.bfloat16, torch.float32, torch.int8
 _ROWS_KIND = {_BF16: 0, _F32: 1, _I8: 2}
@@ -146,6 +148,8 @@ def quantize_rows(x: torch.Tensor) -> QuantRows:
     x, R, cols, stride = _rows(x, "x")
     if cols < 1 or cols > INT8_MAX_K:
         raise ValueError(f"rows of 1 to {INT8_MAX_K} columns, got {cols}")
+    if R > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows, got {R}")
     dev = _device(x)
     q = _empty_rows(x, R, cols)
     scale = _empty((R,), (1,), dtype=_F32, device=x.device)
@@ -204,6 +208,8 @@ def _product(name: str, x, weight, bias, out_f32: bool, out, halves: int) -> tor
         x_dev, x_ptr, kind, x_scale, xs_ptr, scratch = x.get_device(), x.data_ptr(), _ROWS_KIND[x.dtype], None, 0, T > 1 or K > INT8_ONE_MAX_K
     if cols != K or K < 1 or K > INT8_MAX_K:
         raise ValueError(f"x has {cols} columns and weight {K}; 1 to {INT8_MAX_K}, and as many in both")
+    if T > INT8_MAX_ROWS or N > INT8_MAX_ROWS:
+        raise ValueError(f"at most {INT8_MAX_ROWS} tokens and outputs, got {T} and {N}")
     if x_dev != dev or dev < 0 or bias is not None or out is not None:
         _device(x, w, bias, out)
     device, bias_ptr = x.device, 0
@@ -289,6 +295,8 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
     res, T, H, res_stride = _rows(residual, "residual")
     if H < 1 or H > BLOCK_NORM_MAX_HIDDEN:
         raise ValueError(f"rows of 1 to {BLOCK_NORM_MAX_HIDDEN} columns, got {H}")
+    if T > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} rows, got {T}")
     dev = _device(res, block, post_gain, gate, pre_gain, residual_out)
     post_gain, pre_gain = _vector(post_gain, H, "post_gain"), _vector(pre_gain, H, "pre_gain")
     dtype = res.dtype
