@@ -288,6 +288,15 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
     or "int8" (``QuantRows``, quantised as ``quantize_rows`` does, ready for ``int8_linear``).  All arithmetic is f32; x is
     made from r' before its rounding.  ``block`` None: the norm before a first block alone, r' is ``residual`` itself.
     H <= 16384; T may be 0."""
+    new, x, dev, args, held = check_norm(residual, block, post_gain, gate, gate_sigmoid, residual_scale, block_scale, pre_gain, eps, out, residual_out)
+    if args is not None:
+        _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, args)
+    return new, x
+
+
+def check_norm(residual, block, post_gain, gate, gate_sigmoid, residual_scale, block_scale, pre_gain, eps, out, residual_out) -> tuple:
+    """``block_norm`` up to its launch: its two results, the device, the arguments of the C entry (None without rows), and the
+    tensors that they point into."""
     if out not in _OUT:
         raise ValueError('out is "bf16", "f32" or "int8"')
     if not eps >= 0:
@@ -300,6 +309,7 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
     dev = _device(res, block, post_gain, gate, pre_gain, residual_out)
     post_gain, pre_gain = _vector(post_gain, H, "post_gain"), _vector(pre_gain, H, "pre_gain")
     dtype = res.dtype
+    blk = None
     kind = gate_stride = gate_f32 = blk_stride = new_stride = blk_ptr = blk_f32 = 0
     if block is None:
         if post_gain is not None or gate is not None or residual_out is not None or residual_scale != 1.0 or block_scale != 1.0:
@@ -332,14 +342,23 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
             x_stride = max(x.stride(0), H)
         else:
             x, x_stride = _empty((T, H), (H, 1), dtype=kind_of_x, device=res.device), H
+    args = None
     if T:
-        _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, _pack_block_norm(
+        args = _pack_block_norm(
             res.data_ptr(), blk_ptr, gate.data_ptr() if kind else 0,
             0 if post_gain is None else post_gain.data_ptr(), 0 if pre_gain is None else pre_gain.data_ptr(),
             new.data_ptr() if blk_ptr else 0, 0 if x is None else x.data_ptr(), 0 if scale is None else scale.data_ptr(),
             T, res_stride, blk_stride, gate_stride, new_stride, x_stride, H, dtype is _F32, blk_f32, gate_f32, kind,
-            bool(gate_sigmoid), code, residual_scale, block_scale, eps))
-    return new, (QuantRows(x, scale) if scale is not None else x)
+            bool(gate_sigmoid), code, residual_scale, block_scale, eps)
+    return new, x if scale is None else QuantRows(x, scale), dev, args, (res, blk, gate, post_gain, pre_gain)
+
+
+def launch_norm(norm: tuple) -> tuple:
+    """Launches what ``check_norm`` returned; returns its results."""
+    new, x, dev, args, _ = norm
+    if args is not None:
+        _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, args)
+    return new, x
 
 
 def _gate(gate: torch.Tensor, T: int, H: int) -> tuple[torch.Tensor, int, int]:

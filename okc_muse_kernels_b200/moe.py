@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from ._lib import OkcError, Plan, Sizes
-from .dense import block_norm
+from .dense import check_norm, launch_norm
 
 __all__ = ["MoEPlan", "prepare", "kernel_fn", "moe_step", "route", "sorted_routes", "unpack_bf16", "read_status", "split_router",
            "experts_profiled", "experts_ep", "cast_bf16", "HostStep", "route_hidden", "moe_layer_step", "moe_block_step", "OkcError"]
@@ -333,6 +333,21 @@ def split_router(router_w: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _check_router(router_w: torch.Tensor, bias: torch.Tensor | None, mode: str, plan: MoEPlan) -> bool:
+    """Whether the router matrix is a split one."""
+    _need_cuda(router_w, bias)
+    split = router_w.dtype == torch.bfloat16
+    if split and tuple(router_w.shape) != (2 * plan.n_experts, plan.hidden):
+        raise ValueError(f"a split router matrix must be bf16 [{2 * plan.n_experts}, {plan.hidden}]")
+    if not split and (router_w.dtype != torch.float32 or tuple(router_w.shape) != (plan.n_experts, plan.hidden)):
+        raise ValueError(f"router_w must be f32 [{plan.n_experts}, {plan.hidden}]")
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (plan.n_experts,)):
+        raise ValueError(f"bias must be f32 [{plan.n_experts}]")
+    if mode not in ("softmax", "sigmoid"):
+        raise ValueError("mode is 'softmax' or 'sigmoid'")
+    return split
+
+
 def route_hidden(hidden_states: torch.Tensor, router_w: torch.Tensor, state: dict, *, bias: torch.Tensor | None = None,
                  mode: str = "softmax", multiplier: float = SIGMOID_MULTIPLIER, own_tokens=None):
     """Router logits ``hidden . router_w^T`` (never materialised) + top-k + the token->expert sort.  ``router_w``:
@@ -344,16 +359,7 @@ def route_hidden(hidden_states: torch.Tensor, router_w: torch.Tensor, state: dic
     Returns views of the state's ``ids`` and ``wts`` buffers."""
     plan: MoEPlan = state["plan"]
     hidden, stride = _check_hidden(hidden_states, plan)
-    _need_cuda(router_w, bias)
-    split = router_w.dtype == torch.bfloat16
-    if split and tuple(router_w.shape) != (2 * plan.n_experts, plan.hidden):
-        raise ValueError(f"a split router matrix must be bf16 [{2 * plan.n_experts}, {plan.hidden}]")
-    if not split and (router_w.dtype != torch.float32 or tuple(router_w.shape) != (plan.n_experts, plan.hidden)):
-        raise ValueError(f"router_w must be f32 [{plan.n_experts}, {plan.hidden}]")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (plan.n_experts,)):
-        raise ValueError(f"bias must be f32 [{plan.n_experts}]")
-    if mode not in ("softmax", "sigmoid"):
-        raise ValueError("mode is 'softmax' or 'sigmoid'")
+    split = _check_router(router_w, bias, mode, plan)
     T = hidden.shape[0]
     t0, t1 = _own(plan, T, own_tokens)
     router_w = router_w.contiguous()
@@ -390,10 +396,22 @@ def moe_block_step(residual: torch.Tensor, router_w: torch.Tensor, state: dict, 
     experts as ``moe_layer_step`` (their f32 sums, not rounded in between), then the norm after it with gate, scales and
     residual sum, and, with ``next_gain``, the norm before the next block.  Returns ``(r', x)`` as ``block_norm``, whose
     arguments the others are; ``out="int8"`` gives x as int8 rows for the next layer's ``int8_linear``."""
-    _, hidden = block_norm(residual, pre_gain=pre_gain, eps=eps)
-    y = moe_layer_step(hidden, router_w, state, bias=bias, mode=mode, multiplier=multiplier, out_f32=True, own_tokens=own_tokens)
-    return block_norm(residual, y, post_gain=post_gain, gate=gate, gate_sigmoid=gate_sigmoid, residual_scale=residual_scale,
-                      block_scale=block_scale, pre_gain=next_gain, eps=eps, out=out, residual_out=residual_out)
+    plan: MoEPlan = state["plan"]
+    dev = state["workspace"].device
+    for t, what in ((residual, "residual"), (router_w, "router_w"), (bias, "bias")):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what} on {t.device} and the state on {dev}")
+    # everything is checked before the first launch
+    before = check_norm(residual, None, None, None, False, 1.0, 1.0, pre_gain, eps, "bf16", None)
+    hidden = before[1]
+    _check_hidden(hidden, plan)
+    _check_router(router_w, bias, mode, plan)
+    y = torch.empty(hidden.shape, dtype=torch.float32, device=dev)
+    after = check_norm(residual, y, post_gain, gate, gate_sigmoid, residual_scale, block_scale, next_gain, eps, out, residual_out)
+    with torch.cuda.device(dev):      # of the tensors, whichever is current
+        launch_norm(before)
+        moe_layer_step(hidden, router_w, state, bias=bias, mode=mode, multiplier=multiplier, out_f32=True, own_tokens=own_tokens, out=y)
+        return launch_norm(after)
 
 
 def moe_step(hidden_states: torch.Tensor, router_logits: torch.Tensor, state: dict, *, out_f32: bool = False,
