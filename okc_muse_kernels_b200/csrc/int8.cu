@@ -445,6 +445,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     tc_fence_before();
   }
   if (kSplits > 1) cluster.sync(); else __syncthreads();
+  const int gave_up = abort_code;
 
   // Each CTA of the cluster finishes tn / kSplits tokens: it adds the integer sums of all CTAs (the loads from all of them
   // under way at once) and stores the rows.  A few tokens of a thread go together, all loads and arithmetic first, and what
@@ -505,7 +506,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
   }
   // A wait ran out, whoever's it was (the producers of a short K have started all their copies by then and are done): the
   // copies on their way get a bounded chance to land before the CTA's memory is another's.
-  if (abort_code != 0) {
+  if (gave_up != 0) {
     const long long c0 = clock64();
     for (int j = max(0, posted - q.stages); j < posted; ++j)
       while (!mbar_try(full0 + 8 * (j % q.stages), (j / q.stages) & 1) && clock64() - c0 < kWaitLimitCycles) {}
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem, static_cast<uint32_t>(q.tmem_cols));
   }
-  if (tid == 0 && abort_code != 0) publish_timeout(&g_int8_status, abort_code);
+  if (tid == 0 && gave_up != 0) publish_timeout(&g_int8_status, gave_up);
 }
 
 static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }

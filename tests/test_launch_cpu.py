@@ -24,5 +24,6 @@ def test_the_split_product_drains_its_copies_whichever_wait_ran_out():
     with open(os.path.join(CSRC, "int8.cu")) as f:
         body = f.read().split("okc_int8_mid(const")[1].split("static int tmem_cols_for")[0]
     tail = body[body.rindex("finish(std::integral_constant<int, 1>"):body.rindex("cluster.sync()")]
-    assert re.search(r"if \(abort_code != 0\) \{[^}]*mbar_try\(full0[^}]*kWaitLimitCycles", tail)
-    assert body.count("mbar_wait") == 3 and "mbar_wait" not in tail
+    assert re.search(r"if \(gave_up != 0\) \{[^}]*mbar_try\(full0[^}]*kWaitLimitCycles", tail)
+    read = body.index("const int gave_up = abort_code;")        # behind every wait and the barrier after them
+    assert body.rindex("mbar_wait") < body.index("cluster.sync()") < read < body.index("auto finish")
