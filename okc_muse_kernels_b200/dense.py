@@ -287,7 +287,8 @@ def block_norm(residual: torch.Tensor, block: torch.Tensor | None = None, *, pos
     bf16 or f32: [H] (or [1, H]) per channel, [T, 1] per token, [T, H] per element.  ``out``: the type of x, "bf16", "f32"
     or "int8" (``QuantRows``, quantised as ``quantize_rows`` does, ready for ``int8_linear``).  All arithmetic is f32; x is
     made from r' before its rounding.  ``block`` None: the norm before a first block alone, r' is ``residual`` itself.
-    H <= 16384; T may be 0."""
+    A row's result depends on that row alone, but the order of its sums goes by the number of rows and their alignment, so
+    its last bits may differ between batches of different sizes.  H <= 16384; T may be 0."""
     new, x, dev, args, held = check_norm(residual, block, post_gain, gate, gate_sigmoid, residual_scale, block_scale, pre_gain, eps, out, residual_out)
     if args is not None:
         _call(_lib.lib().okc_moe_block_norm, "okc_moe_block_norm", dev, args)
