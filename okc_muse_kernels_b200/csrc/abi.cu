@@ -728,7 +728,7 @@ int okc_moe_quantize_rows(const void* x, int x_f32, int64_t x_stride, int64_t ro
 static uint64_t int8_row_bytes(int K) { return (static_cast<uint64_t>(K) + 15) / 16 * 16; }
 
 uint64_t okc_moe_int8_scratch_bytes(int x_kind, int32_t tokens, int32_t k) {
-  if (x_kind == kRowsInt8 || k <= 0 || (tokens == 1 && k <= kInt8OneMaxK)) return 0;
+  if (x_kind == kRowsInt8 || tokens <= 0 || k <= 0 || (tokens == 1 && k <= kInt8OneMaxK)) return 0;
   return static_cast<uint64_t>(tokens) * (int8_row_bytes(k) + 4);
 }
 

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import okc_muse_kernels_b200 as okc
+from okc_muse_kernels_b200 import _lib
 
 
 @pytest.mark.parametrize("rows", [(1 << 30) + 1, (1 << 31) + 5])
@@ -24,3 +25,9 @@ def test_more_rows_than_a_call_takes():
     for call in (lambda: okc.quantize_rows(x), lambda: okc.block_norm(x, x), lambda: okc.block_norm(x, pre_gain=torch.empty(8, device="meta"))):
         with pytest.raises(ValueError, match="at most"):
             call()
+
+
+def test_scratch_of_no_tokens():
+    need = _lib.lib().okc_moe_int8_scratch_bytes
+    assert need(0, 0, 4096) == 0 and need(0, -1, 4096) == 0 and need(1, -(1 << 31), 16) == 0 and need(0, 5, 0) == 0 and need(0, 5, -7) == 0
+    assert need(0, 1 << 30, 131071) == (1 << 30) * (131072 + 4)
