@@ -75,10 +75,11 @@ struct OneShape {
 // a warp takes a slot: pairs of rows (two neighbours, or a gate row and its up row) against the token, 16 bytes a lane of
 // each, integer dot products, one warp sum a row, and the outputs leave from there.
 // The 16 bytes at a row's end may reach past K, never past the row's next 16-byte boundary; the token is zero there.
-// bf16 token, weights of three layers in turn: K = 4096, N = 4096 4.4 us (the quantiser and okc_int8_mid: 6.5; rows held in
-// registers, 16 a warp on their way: 5.7), gated, K = 7168, 2 x 2048 rows 5.5 (8.3; 8.2); a token and one weight tile alone
-// take 3.3.  More tokens go through the tiles: the dot-product instruction gives an SM some 14 lanes a clock, and 2 / 4 / 8
-// tokens took 5.3 / 7.3 / 11.6 us here (gated 9.7 / 13.2 / 22.8) against 6.5 (8.3).
+// bf16 token, in a graph: K = 4096, N = 4096 3.9 us with the weights of three layers in turn (50 MB, in L2) and 5.6 with all of
+// them from HBM (16.8 MB: 3.0 TB/s), gated, K = 7168, 2 x 2048 rows 6.0 and 8.5 (29.4 MB: 3.5 TB/s).  Measured side by side, in
+// L2: the quantiser and okc_int8_mid 6.5 us, rows held in registers, 16 a warp on their way, 5.7, this kernel 4.4 (gated 8.3,
+// 8.2, 5.5); a token and one weight tile alone 3.3.  More tokens go through the tiles: the dot-product instruction gives an SM
+// some 14 lanes a clock, and 2 / 4 / 8 tokens took 5.3 / 7.3 / 11.6 us here (gated 9.7 / 13.2 / 22.8) against 6.5 (8.3).
 template <bool kGated>
 __global__ void __launch_bounds__(kOneThreads) okc_int8_one(const Int8Params p, const OneShape q) {
   extern __shared__ __align__(16) uint8_t one_smem[];
@@ -296,8 +297,9 @@ struct Int8MidParams {
 // A copy costs an SM some 150 cycles besides its bytes, however many warps issue them, so a stage takes several K blocks with
 // one copy of weights and one of tokens (8 tokens, K = 7168, N = 2048, blocks 1 / 2 / 7: 7.9 / 7.4 / 6.5 us; gated, 32 tokens,
 // K = 4096, 2 x 2560 rows, 1 / 2 / 4: 8.6 / 8.0 / 7.0), and the first weights are on their way before the CTA has set itself up.
-// Bounded by the copies into the SMs for most sizes: 32 tokens, K = 4096, N = 7168 7.9 us (29.4 MB of weights), gated, 128
-// tokens, K = 7168, 2 x 2048 rows 10.5 us (29.4 MB), of which about 4 us are the launch and the sums' way through the cluster.
+// Bounded by the copies into the SMs for most sizes while the weights are in L2, by those and the way from HBM when they are not:
+// int8 tokens, 32, K = 4096, N = 7168 7.1 / 10.3 us (29.4 MB of weights, in L2 / from HBM), gated, 128 tokens, K = 7168, 2 x
+// 2048 rows 9.8 / 12.0 us (29.4 MB), of which about 4 us are the launch and the sums' way through the cluster.
 template <bool kGated, int kSplits, bool kSingle>      // kSingle: one K block a stage
 __global__ void __launch_bounds__(kMidThreads) okc_int8_mid(const __grid_constant__ Int8MidParams q) {
   extern __shared__ uint8_t smem_raw[];
@@ -523,9 +525,10 @@ static int tmem_cols_for(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 
 
 // How the two tiled kernels would cut a product, and what each is expected to take.  The estimates are a start-up time, a
 // time for the end of a tile, and a time for the K blocks: what a CTA needs for one alone, or, with all SMs busy, what its
-// bytes take at the 83 to 90 KB/us that an SM takes in then.  Of 323 measured shapes (3 to 512 tokens, K 256 to 7168, N 300
-// to 7168, plain and gated), where the two differ by up to 2 either way, the choice costs 0.4 % of the better one's time on
-// average and 30 % at worst, and the split over a cluster 0.4 % on average.
+// bytes take at the 83 to 90 KB/us that an SM takes in then (from L2: the fit is to weights that are there).  Of 323 measured
+// shapes (3 to 512 tokens, K 256 to 7168, N 300 to 7168, plain and gated) the choice of the kernel and of the split over a
+// cluster costs 0.5 % of the best of the five on average and 20 % at worst with the weights in L2, 0.6 % and 16 % with all
+// of them from HBM.
 struct TileShape {
   int tokens, outs, blocks;      // mid: tokens and outputs of a tile, K blocks of a stage
   int t_tiles, tiles, splits;
@@ -658,8 +661,9 @@ cudaError_t launch_int8_mid(const Int8Params& p, bool gated, bool quantised_here
 // rows into shared memory, the leader issues the MMAs of both (cta_group::2), each keeps its rows of the sums in its own
 // tensor memory, two tiles side by side, so that the end of one tile runs under the next one's MMAs.  Half the operand
 // bytes a CTA against two single tiles is what the rate needs: 64 bytes a clock and SM at 256 x 256.
-// 4096 x 7168 x 7168: 127 us, 3.3e15 operations/s (twice the bf16 rate of the measured peaks is 3.25e15: bounded by the
-// tensor cores under the power limit); gated 4096 x 5120 x 2 x 2048 54 us, 3.2e15.
+// Bounded by the tensor cores, in long runs by the power they draw: 4096 x 7168 x 7168 123 us at 1965 MHz (3.4e15 operations/s;
+// twice the bf16 burst of the measured peaks is 3.25e15) and 147 us at the 1340 MHz that seconds of it leave (2.9e15; 2.8e15);
+// gated 4096 x 5120 x 2 x 2048 59 us (2.9e15: 3.5 rounds of tiles) and 66 us at 1560 MHz.
 constexpr int kManyThreads = 384;      // warps 0 TMA producer, 1 MMA issuer (leader CTA), 2 TMEM, 3 weight scales, 4..11 epilogue
 constexpr int kManyEpilogueWarps = 8;  // one warp a scheduler kept up with one instruction in five cycles only
 constexpr int kManyStages = 6;

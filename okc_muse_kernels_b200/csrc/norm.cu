@@ -123,7 +123,10 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_block_norm(const Blo
 // The same for many rows that 16-byte accesses can reach: persistent CTAs, each with a ring of rows in shared memory that
 // bulk copies fill ahead of it, so that HBM does not wait for the two dependent sums of a row.  What is left is issue
 // slots: pairs of f32 an instruction, and as many CTAs an SM as registers allow (the gains stay in L1, not in shared
-// memory, for that).  4096 x 5120, everything bf16, a gate per element: 39.4 us (210 MB: 5.3 TB/s); a CTA per row 65.1 us.
+// memory, for that).  4096 x 5120, everything bf16, a gate per element, inputs larger than L2: 43.0 us in a graph (210 MB: 4.9
+// TB/s), 45.3 call after call (4.6); with one vector for both gains 38.6, a CTA per row then 65.1.  Without the gate 32.8 us
+// (168 MB: 5.1 TB/s).  f32 residual, 4096 x 4096 int8 rows out: 39.7 us with a bf16 block (184 MB: 4.6 TB/s), 46 with an f32
+// one (218 MB: 4.7).
 constexpr int kStreamStages = 2;                 // rows of a ring; more do not help (4096 x 4096: 2 / 3 / 8 rows 37.8 / 38.7 / 39.4 us)
 constexpr int kStreamSmem = 200 * 1024;          // an SM's shared memory for rings; L1 keeps the rest, for the gains
 template <int kChunks, bool kInt8>
@@ -302,8 +305,9 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
 
 // The same ring for rows of any width and alignment: a copy takes the 16-byte pieces that a row lies in (never past the
 // row's last piece, so never out of its allocation), and the threads find the row behind the bytes in front of it.
-// Neighbouring threads take neighbouring columns.  4096 x 5121, bf16, a gate per element: 86.7 us, a CTA per row with
-// plain loads 138.5.
+// Neighbouring threads take neighbouring columns.  Bounded by its instructions: one element an access, to shared memory and to
+// global memory, where the aligned rows move eight (and 40 bytes of spills a thread at 32 values).  4096 x 5121, bf16, a gate per
+// element: 86.7 us (210 MB: 2.4 TB/s), a CTA per row with plain loads 138.5.
 template <int kChunks>
 __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stream_any(const BlockNormParams p, int rows, int row_bytes) {
   extern __shared__ __align__(16) uint8_t ring[];
@@ -476,7 +480,7 @@ __global__ void __launch_bounds__(row_threads(kChunks)) okc_quantize_rows(const 
 // Nothing waits on other warps, and a dozen warps an SM have their whole rows on the way at once.  A row may start
 // anywhere: the loads are those of the 16-byte pieces that it lies in (with up to 7 values before and behind it, which
 // count as zeros), and the int8 values move down by as many lanes' bytes before they are stored eight at a time.
-// 4096 x 7168: a CTA per row 27.7 us, this kernel 16.7 (88 MB: 5.3 TB/s).
+// 4096 x 7168: a CTA per row 27.7 us, this kernel 15.1 (88 MB: 5.8 TB/s); 4096 x 7167 24.9.
 template <int kVecs>
 __global__ void __launch_bounds__(128) okc_quantize_rows_warp(const QuantizeParams p, int64_t rows) {
   if (p.product_follows) griddep_launch_dependents();
@@ -550,7 +554,8 @@ static void row_shape(int64_t rows, int cols, int& threads, int& chunks) {
   if (threads > row_threads(chunks)) threads = row_threads(chunks);
 }
 
-// The streaming kernels, if the rows are many (4 an SM and more: bf16, a gate per channel, 500 / 600 rows of 4096 take 6.3 us
+// The streaming kernels, if there is a block (without one a CTA per row takes them: 4096 x 5120 bf16 26 to 27 us for 84 MB, not
+// looked at further) and the rows are many (4 an SM and more: bf16, a gate per channel, 500 / 600 rows of 4096 take 6.3 us
 // a CTA each and 7.2 streamed; at 4096 rows the streamed ones take 29.6 of 44) and a ring fits; false: not launched.
 static bool try_stream(const BlockNormParams& p, int64_t rows, bool vec, cudaStream_t stream, cudaError_t& e) {
   if (!p.blk || rows < 4 * 148 || rows > INT32_MAX / 2) return false;
@@ -590,6 +595,8 @@ cudaError_t launch_block_norm(const BlockNormParams& p, int64_t rows, bool vec, 
   return vec ? launch_kernel(okc_block_norm<4, true>, grid, block, 0, stream, false, p) : launch_kernel(okc_block_norm<4, false>, grid, block, 0, stream, false, p);
 }
 
+// f32 rows, and bf16 rows of more than 8192 columns, do not fit a warp's registers and take a CTA each: 4096 x 7168 f32 30.9 us
+// (147 MB: 4.8 TB/s), 4096 x 14336 bf16 38.9 (176 MB: 4.5 TB/s).
 cudaError_t launch_quantize_rows(const QuantizeParams& p, int64_t rows, bool x_vec, bool q_vec, cudaStream_t stream) {
   const bool vec = x_vec && q_vec && (p.cols % 8) == 0;
   const int span = vec ? p.cols : p.cols + 7;
