@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     }
     // a wait that runs out does not leave the loop (the other threads count on this one's barriers): the row's result is
     // then undefined and the status word says so
-    mbar_wait(smem_u32(&bar_full[st]), ph, &abort_code, 0x81);
+    const bool landed = mbar_wait(smem_u32(&bar_full[st]), ph, &abort_code, 0x81);
     const uint8_t* const src = ring + st * row_bytes;
     F2 r[kChunks][4];
     {
@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     }
     // every thread has read its part of the slot once it is past that sum's barrier
     if (!p.pre_gain || nt == 32) __syncthreads();
-    if (tid == 0 && row + static_cast<int64_t>(kStreamStages) * gridDim.x < rows) fetch(row + kStreamStages * gridDim.x, st);
+    // (not into a slot whose copy is late: its barrier still counts that one)
+    if (tid == 0 && row + static_cast<int64_t>(kStreamStages) * gridDim.x < rows && landed) fetch(row + kStreamStages * gridDim.x, st);
     if (p.pre_gain) {
       const F2 rstd2 = f2_pack(rstd, rstd);
       uint32_t amax = 0;
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(512, kChunks == 4 ? 1 : 2) okc_block_norm_stre
     float rstd = 0.f;
     if (p.pre_gain) rstd = rsqrtf(cta_sum(ss, red_pre[n & 1]) * over_h + p.eps);
     if (!p.pre_gain || nt == 32) __syncthreads();
-    if (tid == 0 && row + static_cast<int64_t>(kStreamStages) * gridDim.x < rows) fetch(row + kStreamStages * gridDim.x, st);
+    if (tid == 0 && row + static_cast<int64_t>(kStreamStages) * gridDim.x < rows && abort_code == 0) fetch(row + kStreamStages * gridDim.x, st);
     if (p.pre_gain) {
       take(p.pre_gain, true, y);
 #pragma unroll

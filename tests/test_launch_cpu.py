@@ -27,3 +27,18 @@ def test_the_split_product_drains_its_copies_whichever_wait_ran_out():
     assert re.search(r"if \(gave_up != 0\) \{[^}]*mbar_try\(full0[^}]*kWaitLimitCycles", tail)
     read = body.index("const int gave_up = abort_code;")        # behind every wait and the barrier after them
     assert body.rindex("mbar_wait") < body.index("cluster.sync()") < read < body.index("auto finish")
+
+
+def test_the_streamed_norms_start_no_copy_behind_one_that_is_late():
+    """Their threads stay in the loop over the rows when a wait has run out.  A slot's barrier then still counts the copy that is
+    late, and another arrival on it is one too many: no further row may be fetched."""
+    with open(os.path.join(CSRC, "norm.cu")) as f:
+        kernels = f.read().split("__global__")
+    streamed = [k for k in kernels if " okc_block_norm_stream" in k.split("{")[0]]
+    assert len(streamed) == 2
+    for body in streamed:
+        wait = body.index("mbar_wait(")
+        again = [line for line in body[wait:].splitlines() if "fetch(" in line]
+        assert len(again) == 1
+        own = re.search(r"const bool (\w+) = mbar_wait\(", body)          # whether this thread's wait saw the copy land
+        assert "&& abort_code == 0) fetch(" in again[0] or own and f"&& {own[1]}) fetch(" in again[0]
